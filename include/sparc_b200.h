@@ -378,13 +378,108 @@ size_t sparc_complex_workspace_bytes(long long batch, long long length, long lon
 int sparc_complex_scan_forward(const SparcComplexFwdArgs* args, void* stream);
 int sparc_complex_scan_backward(const SparcComplexBwdArgs* args, void* stream);
 
+/* Gated linear recurrence over [batch, length, channels] (no counterpart in the reference): with s
+ * the logistic function and nu = e^{nu_log} per channel,
+ *   a_t = exp(-nu s(retention_t)),  h_t = c_t h_{t-1} + sqrt(1 - a_t^2) s(write_t) x_t,
+ * c_t = a_t, or 0 where token t starts a segment (segment_pos == 0; what came before is dropped,
+ * infinities and NaN included). x and the gates are read in `dtype` with their own batch and
+ * token strides (in elements; the channels are adjacent), so that they may be columns of one
+ * projection; y and the gradients are dense, in `dtype`; the arithmetic, the states and nu_log
+ * are float32. `segment_pos` (optional) is [batch, length] integers of segment_pos_bytes bytes each. `carry`
+ * (NULL when no backward follows) receives the state entering every chunk of
+ * sparc_gated_chunk_tokens() tokens, [batch, sparc_gated_carry_chunks(length), channels] float32.
+ * The backward takes dy (its own strides) and optionally the gradient of the last state, and
+ * writes the gradients of x, the gates, nu_log ([channels]) and, optionally, h0. Its workspace,
+ * sparc_gated_workspace_bytes bytes, 8-byte aligned, needs no initial contents. Results are
+ * bitwise reproducible. */
+typedef struct SparcGatedFwdArgs {
+  const void* x;
+  const void* retention_gate;
+  const void* write_gate;
+  const float* nu_log;                 /* [channels] */
+  const float* h0;                     /* [batch, channels] or NULL (zero) */
+  const void* segment_pos;             /* [batch, length] or NULL */
+  int segment_pos_bytes;               /* 1, 2, 4 or 8 */
+  void* y;                             /* [batch, length, channels] out */
+  float* last;                         /* [batch, channels] out, or NULL */
+  float* carry;                        /* out, or NULL */
+  long long x_batch_stride;
+  long long x_token_stride;
+  long long retention_batch_stride;
+  long long retention_token_stride;
+  long long write_batch_stride;
+  long long write_token_stride;
+  long long batch;
+  long long length;
+  long long channels;
+  int dtype;
+} SparcGatedFwdArgs;
+
+typedef struct SparcGatedBwdArgs {
+  const void* x;
+  const void* retention_gate;
+  const void* write_gate;
+  const float* nu_log;
+  const void* dy;
+  const float* carry;                  /* the forward's carry output */
+  const float* grad_last;              /* [batch, channels] or NULL */
+  const void* segment_pos;             /* as given to the forward */
+  int segment_pos_bytes;
+  void* grad_x;                        /* [batch, length, channels] out (dtype) */
+  void* grad_retention_gate;
+  void* grad_write_gate;
+  float* grad_nu_log;                  /* [channels] out */
+  float* grad_h0;                      /* [batch, channels] out, or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+  long long x_batch_stride;
+  long long x_token_stride;
+  long long retention_batch_stride;
+  long long retention_token_stride;
+  long long write_batch_stride;
+  long long write_token_stride;
+  long long dy_batch_stride;
+  long long dy_token_stride;
+  long long batch;
+  long long length;
+  long long channels;
+  int dtype;
+} SparcGatedBwdArgs;
+
+/* One token of it: x and the gates [batch, channels] (dtype, row strides in elements), state
+ * [batch, channels] float32 in, y (dtype) and new_state (float32, may be `state` itself) out. */
+typedef struct SparcGatedStepArgs {
+  const void* x;
+  const void* retention_gate;
+  const void* write_gate;
+  const float* nu_log;
+  const float* state;
+  const void* segment_pos;             /* [batch] or NULL */
+  int segment_pos_bytes;
+  void* y;
+  float* new_state;
+  long long x_stride;
+  long long retention_stride;
+  long long write_stride;
+  long long batch;
+  long long channels;
+  int dtype;
+} SparcGatedStepArgs;
+
+long long sparc_gated_chunk_tokens(void);
+long long sparc_gated_carry_chunks(long long length);
+size_t sparc_gated_workspace_bytes(long long batch, long long length, long long channels);
+int sparc_gated_scan_forward(const SparcGatedFwdArgs* args, void* stream);
+int sparc_gated_scan_backward(const SparcGatedBwdArgs* args, void* stream);
+int sparc_gated_step(const SparcGatedStepArgs* args, void* stream);
+
 /* Diagnostics: per-kernel device time. While enabled, every kernel launch of this library is
  * bracketed by CUDA events on its stream (launches inside a stream capture are not timed).
  * sparc_timing_read waits for the recorded launches, writes per-kernel totals (milliseconds) and
  * launch counts for up to n kernel kinds (either pointer may be NULL), resets them, and returns
  * the number of kernel kinds, SPARC_TIMING_KERNELS; sparc_timing_kernel_name names kind `id`.
  * sparc_timing_enable returns the previous setting. */
-#define SPARC_TIMING_KERNELS 23
+#define SPARC_TIMING_KERNELS 27
 int sparc_timing_enable(int on);
 const char* sparc_timing_kernel_name(int id);
 int sparc_timing_read(double* ms, long long* launches, int n);

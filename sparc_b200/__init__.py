@@ -14,6 +14,7 @@ from .projection import SPARCSequenceLayer, sparc_projection_states, sparc_seque
 from .rtrl import SPARCRTRLCell, initialize_carry, initialize_traces, rtrl_step, stored_rtrl_step
 from .real import real_chunk_scan, real_scan, real_scan_with_last
 from .complex import complex_scan, complex_scan_with_last
+from .gated import gated_scan, gated_scan_step
 from .scan import (sparc_chunk_scan, sparc_scan, sparc_scan_precomputed_decay, sparc_scan_with_last,
                    sparc_tiled_serial_scan, sparc_training_scan_dispatch)
 from . import _lib
@@ -42,6 +43,7 @@ __all__ = ["SPARCMixer", "sparc_mixer", "sparc_block", "SPARCBlock", "SPARCStack
            "SPARCSequenceLayer", "sparc_sequence_layer", "sparc_projection_states",
            "SPARCRTRLCell", "rtrl_step", "stored_rtrl_step", "initialize_carry", "initialize_traces",
            "real_scan", "real_chunk_scan", "real_scan_with_last", "complex_scan", "complex_scan_with_last",
+           "gated_scan", "gated_scan_step",
            "sparc_scan", "sparc_chunk_scan",
            "sparc_scan_with_last", "sparc_tiled_serial_scan", "sparc_training_scan_dispatch",
            "sparc_scan_precomputed_decay", "run_sequence", "prepare_decode", "run_decode_step", "check_status",

@@ -6,6 +6,7 @@ There is no fallback: if the library or a CUDA device is missing, every entry po
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -107,6 +108,38 @@ class ComplexBwdArgs(ctypes.Structure):
     ]
 
 
+class GatedFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("retention_gate", _vp), ("write_gate", _vp), ("nu_log", _vp), ("h0", _vp),
+        ("segment_pos", _vp), ("segment_pos_bytes", ctypes.c_int), ("y", _vp), ("last", _vp), ("carry", _vp),
+        ("x_batch_stride", _ll), ("x_token_stride", _ll), ("retention_batch_stride", _ll),
+        ("retention_token_stride", _ll), ("write_batch_stride", _ll), ("write_token_stride", _ll),
+        ("batch", _ll), ("length", _ll), ("channels", _ll), ("dtype", ctypes.c_int),
+    ]
+
+
+class GatedBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("retention_gate", _vp), ("write_gate", _vp), ("nu_log", _vp), ("dy", _vp), ("carry", _vp),
+        ("grad_last", _vp), ("segment_pos", _vp), ("segment_pos_bytes", ctypes.c_int), ("grad_x", _vp),
+        ("grad_retention_gate", _vp), ("grad_write_gate", _vp), ("grad_nu_log", _vp), ("grad_h0", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("x_batch_stride", _ll), ("x_token_stride", _ll), ("retention_batch_stride", _ll),
+        ("retention_token_stride", _ll), ("write_batch_stride", _ll), ("write_token_stride", _ll),
+        ("dy_batch_stride", _ll), ("dy_token_stride", _ll),
+        ("batch", _ll), ("length", _ll), ("channels", _ll), ("dtype", ctypes.c_int),
+    ]
+
+
+class GatedStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("retention_gate", _vp), ("write_gate", _vp), ("nu_log", _vp), ("state", _vp),
+        ("segment_pos", _vp), ("segment_pos_bytes", ctypes.c_int), ("y", _vp), ("new_state", _vp),
+        ("x_stride", _ll), ("retention_stride", _ll), ("write_stride", _ll),
+        ("batch", _ll), ("channels", _ll), ("dtype", ctypes.c_int),
+    ]
+
+
 class RtrlStepArgs(ctypes.Structure):
     _fields_ = [
         ("x", _vp), ("content", _vp), ("projections", _vp), ("reset", _vp), ("state", _vp), ("new_state", _vp),
@@ -177,6 +210,12 @@ SIGNATURES = {
     "sparc_complex_workspace_bytes": (ctypes.c_size_t, [_ll, _ll, _ll]),
     "sparc_complex_scan_forward": (ctypes.c_int, [ctypes.POINTER(ComplexFwdArgs), _vp]),
     "sparc_complex_scan_backward": (ctypes.c_int, [ctypes.POINTER(ComplexBwdArgs), _vp]),
+    "sparc_gated_chunk_tokens": (_ll, []),
+    "sparc_gated_carry_chunks": (_ll, [_ll]),
+    "sparc_gated_workspace_bytes": (ctypes.c_size_t, [_ll, _ll, _ll]),
+    "sparc_gated_scan_forward": (ctypes.c_int, [ctypes.POINTER(GatedFwdArgs), _vp]),
+    "sparc_gated_scan_backward": (ctypes.c_int, [ctypes.POINTER(GatedBwdArgs), _vp]),
+    "sparc_gated_step": (ctypes.c_int, [ctypes.POINTER(GatedStepArgs), _vp]),
     "sparc_read_status": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint), _vp]),
     "sparc_clear_status": (ctypes.c_int, [_vp, _vp]),
     "sparc_rtrl_saved_floats": (ctypes.c_int, []),
@@ -257,6 +296,15 @@ def ptr(t):
 
 def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is CUDA's current device (a launch has to go to a stream of the
+    current device); nothing to do, and nothing done, where it already is."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
 
 
 class _Workspaces:

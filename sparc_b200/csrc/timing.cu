@@ -31,7 +31,9 @@ const char* const kNames[kTimeKernels] = {
     "proj_gemm_kernel",         "peer_allreduce_kernel",        "proj_rowdot_kernel",
     "proj_colsum_kernel",       "proj_gemm_finish_kernel",      "complex_fwd_summary_kernel",
     "complex_carry_scan(fwd)",  "complex_fwd_replay_kernel",    "complex_bwd_summary_kernel",
-    "complex_carry_scan(bwd)",  "complex_bwd_grad_kernel"};
+    "complex_carry_scan(bwd)",  "complex_bwd_grad_kernel",
+    "gated_fwd_kernel",         "gated_bwd_kernel",             "gated_reduce_kernel",
+    "gated_step_kernel"};
 
 cudaEvent_t take_event() {
   if (!g_pool.empty()) {

@@ -43,6 +43,10 @@ enum KernelId {
   kTimeComplexBwdSummary,
   kTimeComplexBwdScan,
   kTimeComplexBwdGrad,
+  kTimeGatedFwd,
+  kTimeGatedBwd,
+  kTimeGatedReduce,
+  kTimeGatedStep,
   kTimeKernels
 };
 
