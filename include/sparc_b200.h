@@ -473,13 +473,81 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* args, void* stream);
 int sparc_gated_scan_backward(const SparcGatedBwdArgs* args, void* stream);
 int sparc_gated_step(const SparcGatedStepArgs* args, void* stream);
 
+/* Layer norm over the last dimension (the reference's networks put one before each layer,
+ * sparc-impl/sparc/networks/sequence_classifier.py): y = (x - mean) rstd weight + bias with
+ * rstd = (var + eps)^(-1/2), per row of x [rows, width] (dtype; row strides in elements, the
+ * columns adjacent). weight, bias (optional), the statistics and the sums are float32; y and dx
+ * are dense, in dtype. `mean` and `rstd` ([rows], together, NULL when no backward follows) are
+ * what the backward reads. The backward writes dx and, where given, the weight's and bias's
+ * gradients [width] (then with a workspace of sparc_layer_norm_workspace_bytes bytes, 4-byte
+ * aligned, no initial contents needed), summed in a fixed order. */
+typedef struct SparcLayerNormFwdArgs {
+  const void* x;
+  const float* weight;                 /* [width] */
+  const float* bias;                   /* [width] or NULL */
+  void* y;                             /* [rows, width] out */
+  float* mean;                         /* [rows] out, or NULL (with rstd) */
+  float* rstd;
+  long long x_row_stride;
+  long long rows;
+  long long width;
+  float eps;
+  int dtype;
+} SparcLayerNormFwdArgs;
+
+typedef struct SparcLayerNormBwdArgs {
+  const void* x;
+  const void* dy;
+  const float* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;                            /* [rows, width] out */
+  float* grad_weight;                  /* [width] out, or NULL */
+  float* grad_bias;                    /* [width] out, or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+  long long x_row_stride;
+  long long dy_row_stride;
+  long long rows;
+  long long width;
+  int dtype;
+} SparcLayerNormBwdArgs;
+
+size_t sparc_layer_norm_workspace_bytes(long long rows, long long width);
+int sparc_layer_norm_forward(const SparcLayerNormFwdArgs* args, void* stream);
+int sparc_layer_norm_backward(const SparcLayerNormBwdArgs* args, void* stream);
+
+/* The norm of all elements of `tensors` gradient tensors together, and the gradients scaled by it:
+ * norm = sqrt(sum g^2) (float32, on the device), out[i] = grads[i] min(1, max_norm / (norm +
+ * eps)). `grads`, `out`, `counts` (elements) and `dtypes` are host arrays, read before the call
+ * returns; the tensors are dense device arrays, float32 or bfloat16. out[i] may be grads[i] (in
+ * place: written only where something is clipped) but may overlap nothing else; with out NULL
+ * only the norm is computed. No host synchronisation; squares are summed so that none overflows
+ * or underflows, in a fixed order. The workspace (sparc_grad_clip_workspace_bytes bytes, 8-byte
+ * aligned) needs no initial contents. */
+typedef struct SparcGradClipArgs {
+  const void* const* grads;
+  void* const* out;                    /* or NULL */
+  const long long* counts;
+  const int* dtypes;
+  int tensors;
+  float max_norm;                      /* not negative; infinity never clips */
+  float eps;
+  float* norm;                         /* [1] out */
+  void* workspace;
+  size_t workspace_bytes;
+} SparcGradClipArgs;
+
+size_t sparc_grad_clip_workspace_bytes(int tensors);
+int sparc_grad_clip(const SparcGradClipArgs* args, void* stream);
+
 /* Diagnostics: per-kernel device time. While enabled, every kernel launch of this library is
  * bracketed by CUDA events on its stream (launches inside a stream capture are not timed).
  * sparc_timing_read waits for the recorded launches, writes per-kernel totals (milliseconds) and
  * launch counts for up to n kernel kinds (either pointer may be NULL), resets them, and returns
  * the number of kernel kinds, SPARC_TIMING_KERNELS; sparc_timing_kernel_name names kind `id`.
  * sparc_timing_enable returns the previous setting. */
-#define SPARC_TIMING_KERNELS 27
+#define SPARC_TIMING_KERNELS 32
 int sparc_timing_enable(int on);
 const char* sparc_timing_kernel_name(int id);
 int sparc_timing_read(double* ms, long long* launches, int n);

@@ -15,6 +15,8 @@ from .rtrl import SPARCRTRLCell, initialize_carry, initialize_traces, rtrl_step,
 from .real import real_chunk_scan, real_scan, real_scan_with_last
 from .complex import complex_scan, complex_scan_with_last
 from .gated import gated_scan, gated_scan_step
+from .grads import clip_grad_norm_, clip_grads, grad_norm
+from .norm import LayerNorm, layer_norm
 from .scan import (sparc_chunk_scan, sparc_scan, sparc_scan_precomputed_decay, sparc_scan_with_last,
                    sparc_tiled_serial_scan, sparc_training_scan_dispatch)
 from . import _lib
@@ -43,7 +45,7 @@ __all__ = ["SPARCMixer", "sparc_mixer", "sparc_block", "SPARCBlock", "SPARCStack
            "SPARCSequenceLayer", "sparc_sequence_layer", "sparc_projection_states",
            "SPARCRTRLCell", "rtrl_step", "stored_rtrl_step", "initialize_carry", "initialize_traces",
            "real_scan", "real_chunk_scan", "real_scan_with_last", "complex_scan", "complex_scan_with_last",
-           "gated_scan", "gated_scan_step",
+           "gated_scan", "gated_scan_step", "layer_norm", "LayerNorm", "grad_norm", "clip_grads", "clip_grad_norm_",
            "sparc_scan", "sparc_chunk_scan",
            "sparc_scan_with_last", "sparc_tiled_serial_scan", "sparc_training_scan_dispatch",
            "sparc_scan_precomputed_decay", "run_sequence", "prepare_decode", "run_decode_step", "check_status",

@@ -140,6 +140,29 @@ class GatedStepArgs(ctypes.Structure):
     ]
 
 
+class LayerNormFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("weight", _vp), ("bias", _vp), ("y", _vp), ("mean", _vp), ("rstd", _vp),
+        ("x_row_stride", _ll), ("rows", _ll), ("width", _ll), ("eps", ctypes.c_float), ("dtype", ctypes.c_int),
+    ]
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("dy", _vp), ("weight", _vp), ("mean", _vp), ("rstd", _vp), ("dx", _vp), ("grad_weight", _vp),
+        ("grad_bias", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("x_row_stride", _ll),
+        ("dy_row_stride", _ll), ("rows", _ll), ("width", _ll), ("dtype", ctypes.c_int),
+    ]
+
+
+class GradClipArgs(ctypes.Structure):
+    _fields_ = [
+        ("grads", ctypes.POINTER(_vp)), ("out", ctypes.POINTER(_vp)), ("counts", ctypes.POINTER(_ll)),
+        ("dtypes", ctypes.POINTER(ctypes.c_int)), ("tensors", ctypes.c_int), ("max_norm", ctypes.c_float),
+        ("eps", ctypes.c_float), ("norm", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class RtrlStepArgs(ctypes.Structure):
     _fields_ = [
         ("x", _vp), ("content", _vp), ("projections", _vp), ("reset", _vp), ("state", _vp), ("new_state", _vp),
@@ -216,6 +239,11 @@ SIGNATURES = {
     "sparc_gated_scan_forward": (ctypes.c_int, [ctypes.POINTER(GatedFwdArgs), _vp]),
     "sparc_gated_scan_backward": (ctypes.c_int, [ctypes.POINTER(GatedBwdArgs), _vp]),
     "sparc_gated_step": (ctypes.c_int, [ctypes.POINTER(GatedStepArgs), _vp]),
+    "sparc_layer_norm_workspace_bytes": (ctypes.c_size_t, [_ll, _ll]),
+    "sparc_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(LayerNormFwdArgs), _vp]),
+    "sparc_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormBwdArgs), _vp]),
+    "sparc_grad_clip_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int]),
+    "sparc_grad_clip": (ctypes.c_int, [ctypes.POINTER(GradClipArgs), _vp]),
     "sparc_read_status": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint), _vp]),
     "sparc_clear_status": (ctypes.c_int, [_vp, _vp]),
     "sparc_rtrl_saved_floats": (ctypes.c_int, []),
@@ -355,7 +383,7 @@ def kernel_times(reset_only: bool = False):
     """Per-kernel device time recorded since the last call while timing was enabled
     (sparc_timing_enable): {kernel name: (total ms, launches)} for kernels that ran."""
     L = lib()
-    n = 32
+    n = 64
     ms = (ctypes.c_double * n)()
     cnt = (ctypes.c_longlong * n)()
     k = L.sparc_timing_read(ms, cnt, n)

@@ -142,10 +142,11 @@ __device__ __forceinline__ float exp_neg(float v) {
   }
 }
 
-// a = e^u and a - 1 for u <= 0: below 1/2 from the series of e^u - 1 (through u^8 / 8!: the next
+// a = e^u and a - 1 for u <= 0: above -1/2 from the series of e^u - 1 (through u^8 / 8!: the next
 // term is below 2^-26 of the first), which keeps 1 - a^2 = -(a - 1)(2 + (a - 1)) exact to a few
-// ulp where a is near 1 and holds the decay of long sequences; else the hardware exp2.
-__device__ __forceinline__ float expm1_neg(float u) {
+// ulp where a is near 1 and holds the decay of long sequences; else the hardware exp2, which keeps
+// a to a few ulp where it is small.
+__device__ __forceinline__ float2 exp_expm1_neg(float u) {  // (a, a - 1)
   float p = 2.4801587301587302e-5f;             // 1/8!
   p = fmaf(p, u, 1.9841269841269841e-4f);       // 1/7!
   p = fmaf(p, u, 1.3888888888888889e-3f);       // 1/6!
@@ -154,8 +155,9 @@ __device__ __forceinline__ float expm1_neg(float u) {
   p = fmaf(p, u, 1.6666666666666667e-1f);       // 1/3!
   p = fmaf(p, u, 0.5f);
   const float small = fmaf(p * u, u, u);
-  const float big = ex2_approx(u * kLog2e) - 1.0f;
-  return u > -0.5f ? small : big;
+  const float e = ex2_approx(u * kLog2e);
+  const bool near = u > -0.5f;
+  return make_float2(near ? 1.0f + small : e, near ? small : e - 1.0f);
 }
 
 // -nu of a channel, held finite so that nu s(retention) never meets 0 x infinity.
@@ -165,9 +167,9 @@ template <typename T>
 __device__ __forceinline__ void gated_ab(float x, float r, float w, float minus_nu, float* a, float* b) {
   const float sr = rcp_approx(1.0f + exp_neg<T>(r));
   const float sw = rcp_approx(1.0f + exp_neg<T>(w));
-  const float p = expm1_neg(minus_nu * sr);
-  *a = 1.0f + p;
-  *b = sqrt_approx(-p * (2.0f + p)) * sw * x;
+  const float2 e = exp_expm1_neg(minus_nu * sr);
+  *a = e.x;
+  *b = sqrt_approx(-e.y * (2.0f + e.y)) * sw * x;
 }
 
 // 1 - s(v) = e^{-v} s(v) without cancellation, given e = e^{-v} (which may be infinite).
@@ -408,9 +410,11 @@ __global__ void __launch_bounds__(kGatedWarps * 32) gated_bwd_kernel(const __gri
         for (int v = 0; v < VEC; ++v) {
           const float er = exp_neg<T>(r[v]), ew = exp_neg<T>(w[v]);
           const float sr = rcp_approx(1.0f + er), sw = rcp_approx(1.0f + ew);
-          const float u = nu[v] * sr, pm = expm1_neg(u), m = -pm * (2.0f + pm);
+          const float u = nu[v] * sr;
+          const float2 e = exp_expm1_neg(u);
+          const float av = e.x, m = -e.y * (2.0f + e.y);
           const float rs = rsqrt_approx(fmaxf(m, 1.17549435e-38f));
-          const float av = 1.0f + pm, xs = x[v] * sw;
+          const float xs = x[v] * sw;
           a[k][v] = av;
           g[k][v] = m * rs * sw;
           b[k][v] = m * rs * xs;

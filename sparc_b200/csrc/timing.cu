@@ -33,7 +33,8 @@ const char* const kNames[kTimeKernels] = {
     "complex_carry_scan(fwd)",  "complex_fwd_replay_kernel",    "complex_bwd_summary_kernel",
     "complex_carry_scan(bwd)",  "complex_bwd_grad_kernel",
     "gated_fwd_kernel",         "gated_bwd_kernel",             "gated_reduce_kernel",
-    "gated_step_kernel"};
+    "gated_step_kernel",        "layer_norm_fwd_kernel",        "layer_norm_bwd_kernel",
+    "layer_norm_reduce_kernel", "grad_norm_kernel",             "grad_clip_kernel"};
 
 cudaEvent_t take_event() {
   if (!g_pool.empty()) {

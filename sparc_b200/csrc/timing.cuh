@@ -47,6 +47,11 @@ enum KernelId {
   kTimeGatedBwd,
   kTimeGatedReduce,
   kTimeGatedStep,
+  kTimeLnFwd,
+  kTimeLnBwd,
+  kTimeLnReduce,
+  kTimeGradNorm,
+  kTimeGradClip,
   kTimeKernels
 };
 

@@ -5,6 +5,9 @@ multi-GPU workload trains. RMSNorm has a float32 weight initialised to ones and 
 block runs as one fused call of the mixer kernels (`sparc_block`: the norm is applied to the
 tiles as they are read and the residual added as the output is written), so no separate norm or
 residual pass touches HBM. `RMSNorm` stays available as a module for unfused use.
+
+With ``norm="layer"`` the blocks are x <- x + SPARCMixer(LayerNorm(x)), on the layer norm's own
+kernels (`norm.py`) with the residual added after the mixer.
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .mixer import SPARCMixer, sparc_block
+from .norm import LayerNorm
 
 
 class RMSNorm(nn.Module):
@@ -25,16 +29,23 @@ class RMSNorm(nn.Module):
         return F.rms_norm(x, (x.shape[-1],), self.weight.to(x.dtype), self.eps)
 
 
-class SPARCBlock(nn.Module):
-    """x + SPARCMixer(RMSNorm(x)) in one fused call (parameters: norm.weight, mixer.*)."""
+def _make_norm(norm: str, width: int, eps: float):
+    if norm not in ("rms", "layer"):
+        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+    return RMSNorm(width, eps) if norm == "rms" else LayerNorm(width, eps)
 
-    def __init__(self, width: int, eps: float = 1e-6):
+
+class SPARCBlock(nn.Module):
+    """x + SPARCMixer(RMSNorm(x)) in one fused call (parameters: norm.weight, mixer.*), or with
+    norm="layer" x + SPARCMixer(LayerNorm(x)) (norm.bias too)."""
+
+    def __init__(self, width: int, eps: float = 1e-6, norm: str = "rms"):
         super().__init__()
-        self.norm = RMSNorm(width, eps)
+        self.norm = _make_norm(norm, width, eps)
         self.mixer = SPARCMixer(width)
 
     def forward(self, x, fused: bool = True):
-        if not fused:
+        if not fused or isinstance(self.norm, LayerNorm):
             y, _ = self.mixer(self.norm(x))
             return x + y
         out, _ = sparc_block(x, self.mixer._params(), self.norm.weight, self.norm.eps, max_spin=self.mixer.max_spin)
@@ -42,12 +53,13 @@ class SPARCBlock(nn.Module):
 
 
 class SPARCStack(nn.Module):
-    """`layers` blocks; the state dict keeps the layout norms.<i>.weight, mixers.<i>.*."""
+    """`layers` blocks; the state dict keeps the layout norms.<i>.weight (and .bias with
+    norm="layer"), mixers.<i>.*."""
 
-    def __init__(self, width: int, layers: int = 4, eps: float = 1e-6, fused: bool = True):
+    def __init__(self, width: int, layers: int = 4, eps: float = 1e-6, fused: bool = True, norm: str = "rms"):
         super().__init__()
-        self.fused = fused
-        self.norms = nn.ModuleList(RMSNorm(width, eps) for _ in range(layers))
+        self.fused = fused and norm == "rms"
+        self.norms = nn.ModuleList(_make_norm(norm, width, eps) for _ in range(layers))
         self.mixers = nn.ModuleList(SPARCMixer(width) for _ in range(layers))
 
     def forward(self, x):
