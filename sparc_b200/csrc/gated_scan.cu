@@ -9,17 +9,18 @@
 //   dretention_t = du_t u_t (1 - s(retention_t)),  dnu_log = sum_{b,t} du_t u_t,  dh_0 = c_0 lam_0.
 // u / sqrt(1 - a^2) stays finite as a -> 1 (it goes to -sqrt(-u/2)), so du u is formed from it.
 //
-// Decomposition: one launch each way, every tensor read once and written once. A lane owns VEC
-// adjacent channels and a warp K consecutive tokens; a CTA's warps own consecutive spans of K
-// tokens (a tile), and a thread-block cluster's CTAs consecutive tiles; the cluster walks the
-// sequence. A thread turns its K tokens into an affine map (A, H): h_out = A h_in + H in
-// registers, the maps of the CTA's warps are composed through shared memory, those of the
-// cluster's CTAs through distributed shared memory (one cluster barrier per step, buffers of two
-// parities), and the thread then replays its tokens from the state entering them. The backward
-// does both directions in one step: the states from the forward's saved chunk carries (float32,
-// one per kGatedChunk tokens, so that the states are not rounded to the activations' type), the
+// Decomposition: one launch each way, every tensor read once and written once. A lane owns two
+// adjacent channels (packed f32x2 arithmetic) and a warp K consecutive tokens; a CTA's eight warps
+// own consecutive spans of K tokens (a tile), and a thread-block cluster's CTAs consecutive tiles;
+// the cluster walks the sequence. A thread turns its K tokens into an affine map (A, H): h_out =
+// A h_in + H in registers; one warp of the CTA runs the state through the warps' maps (and, over
+// distributed shared memory and one cluster barrier, through the maps of the cluster's CTAs) and
+// hands every warp the state entering its tokens, from which they are replayed. The backward does
+// both directions in one step: the states from the forward's saved chunk carries (float32, one
+// per kGatedChunk tokens, so that the states are not rounded to the activations' type), the
 // adjoints from the step before. The cluster size grows as rows x channels shrink. All orders are
-// fixed: results are bitwise reproducible.
+// fixed: results are bitwise reproducible. Each warp copies its own tokens to shared memory
+// asynchronously, kStages - 1 steps ahead, so nothing but the copies' own completion orders them.
 //
 // A segment start drops what came before it, infinities and NaN included: its factor is kept as
 // -0 (a_t >= +0, so the sign marks it through products), and composing with it selects instead of
@@ -37,6 +38,7 @@ constexpr int kGatedWarps = 8;   // warps per CTA
 constexpr int kFwdK = 8;         // tokens per thread and step, forward
 constexpr int kBwdK = 4;         // tokens per thread and step, backward (a chunk per CTA and step)
 constexpr int kGatedMaxCluster = 8;
+constexpr int kFwdStages = 2, kBwdStages = 3;  // steps of inputs held in shared memory
 static_assert(kBwdK * kGatedWarps == kGatedChunk, "the backward's tile is one chunk");
 static_assert(kGatedChunk % kFwdK == 0, "a carry is some thread's entering state");
 
@@ -46,7 +48,7 @@ struct GatedIn {
 };
 
 struct GatedParams {
-  GatedIn x, r, w, dy;
+  GatedIn in[4];       // x, retention gate, write gate; backward: dy
   void* y;             // [B, L, D] (forward)
   void *dx, *dr, *dw;  // [B, L, D] (backward)
   const float* nu_log; // [D]
@@ -55,49 +57,38 @@ struct GatedParams {
   float* carry;        // [B, chunks, D]: the state entering each chunk, or null (forward)
   const float* grad_last;  // [B, D] or null
   float* grad_h0;      // [B, D] or null
-  double* part;        // [rows, D] partial sums of dnu_log
+  double* part;        // [rows * cluster, D] partial sums of dnu_log
   const void* pos;     // segment positions [B, L] or null
   int pos_bytes;
   long long B, L, chunks;
   int D, groups, cluster, rows;  // rows: clusters per channel group, each walking rows of the batch
 };
 
-// ---------------------------------------------------------------- VEC adjacent values
-template <typename T, int VEC> struct Pack;
-template <> struct Pack<float, 1> {
-  using type = float;
-  static __device__ __forceinline__ void get(float v, float* f) { f[0] = v; }
-  static __device__ __forceinline__ float make(const float* f) { return f[0]; }
-};
-template <> struct Pack<float, 2> {
+// ---------------------------------------------------------------- two adjacent channels
+template <typename T> struct Duo;
+template <> struct Duo<float> {
   using type = float2;
-  static __device__ __forceinline__ void get(float2 v, float* f) { f[0] = v.x, f[1] = v.y; }
-  static __device__ __forceinline__ float2 make(const float* f) { return make_float2(f[0], f[1]); }
+  static __device__ __forceinline__ float2 get(float2 v) { return v; }
+  static __device__ __forceinline__ float2 make(float2 v) { return v; }
+  static __device__ __forceinline__ float2 join(float a, float b) { return make_float2(a, b); }
+  static __device__ __forceinline__ float bits(const float* p) { return __ldg(p); }
 };
-template <> struct Pack<__nv_bfloat16, 1> {
-  using type = unsigned short;
-  static __device__ __forceinline__ void get(unsigned short v, float* f) { f[0] = __uint_as_float((unsigned)v << 16); }
-  static __device__ __forceinline__ unsigned short make(const float* f) {
-    return __bfloat16_as_ushort(__float2bfloat16_rn(f[0]));
-  }
-};
-template <> struct Pack<__nv_bfloat16, 2> {
+template <> struct Duo<__nv_bfloat16> {
   using type = unsigned;
-  static __device__ __forceinline__ void get(unsigned v, float* f) {
-    f[0] = __uint_as_float(v << 16);
-    f[1] = __uint_as_float(v & 0xffff0000u);
+  static __device__ __forceinline__ float2 get(unsigned v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
-  static __device__ __forceinline__ unsigned make(const float* f) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(f[0], f[1]);
-    return *reinterpret_cast<const unsigned*>(&v);
+  static __device__ __forceinline__ unsigned make(float2 v) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+    return *reinterpret_cast<const unsigned*>(&b);
+  }
+  static __device__ __forceinline__ unsigned join(unsigned short a, unsigned short b) {
+    return (unsigned)a | (unsigned)b << 16;
+  }
+  static __device__ __forceinline__ unsigned short bits(const __nv_bfloat16* p) {
+    return __ldg(reinterpret_cast<const unsigned short*>(p));
   }
 };
-
-template <typename T, int VEC>
-__device__ __forceinline__ typename Pack<T, VEC>::type gated_load(const GatedIn& in, long long b, long long t, int ch) {
-  return __ldg(reinterpret_cast<const typename Pack<T, VEC>::type*>(static_cast<const T*>(in.p) + b * in.sb +
-                                                                     t * in.st + ch));
-}
 
 __device__ __forceinline__ bool gated_starts(const void* pos, int bytes, long long i) {
   switch (bytes) {
@@ -106,6 +97,85 @@ __device__ __forceinline__ bool gated_starts(const void* pos, int bytes, long lo
     case 4: return __ldg(static_cast<const unsigned*>(pos) + i) == 0;
     default: return __ldg(static_cast<const unsigned long long*>(pos) + i) == 0;
   }
+}
+
+// How a warp reads its tokens: pieces of 16 bytes or of one pair of channels, copied to shared
+// memory ahead of their use, or single channels read where they are used (odd widths, strides or
+// bases, which no asynchronous copy of two bytes exists for).
+enum GatedMode { kModeWide, kModePair, kModeSingle };
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool valid) {
+  const int n = valid ? BYTES : 0;  // the rest is filled with zeros
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A warp's tokens t0 .. t0 + K - 1 of NT tensors, in stage[tensor][token][lane].
+template <typename T, int MODE, int K, int NT>
+__device__ __forceinline__ void gated_issue(const GatedParams& p, typename Duo<T>::type* stage, long long bt,
+                                            long long t0, int ch0, int lane) {
+  using R = typename Duo<T>::type;
+  if constexpr (MODE != kModeSingle) {
+    constexpr int BYTES = MODE == kModeWide ? 16 : (int)sizeof(R);
+    constexpr int ROW = 32 * (int)sizeof(R) / BYTES;  // pieces per token
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const T* base = static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb;
+#pragma unroll
+      for (int c = lane; c < K * ROW; c += 32) {
+        const int k = c / ROW, e = c % ROW * (BYTES / (int)sizeof(T));
+        const bool valid = t0 + k < p.L && ch0 + e < p.D;
+        const T* src = valid ? base + (t0 + k) * p.in[n].st + ch0 + e : static_cast<const T*>(p.in[n].p);
+        copy_async<BYTES>(smem_addr(stage + n * K * 32) + c * BYTES, src, valid);
+      }
+    }
+    copy_commit();
+  }
+}
+
+template <typename T, int MODE, int K>
+__device__ __forceinline__ void gated_read(const GatedParams& p, int n, const typename Duo<T>::type* stage, long long bt,
+                                           long long t0, int ch, int lane, typename Duo<T>::type* v) {
+  if constexpr (MODE != kModeSingle) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = stage[(n * K + k) * 32 + lane];
+  } else {
+    const T* base = static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + ch;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool ok = t0 + k < p.L;
+      const T* q = base + (t0 + k) * p.in[n].st;
+      v[k] = Duo<T>::join(ok && ch < p.D ? Duo<T>::bits(q) : 0, ok && ch + 1 < p.D ? Duo<T>::bits(q + 1) : 0);
+    }
+  }
+}
+
+template <typename T, int MODE>
+__device__ __forceinline__ void gated_store(void* out, long long i, int ch, int D, float2 v) {
+  T* o = static_cast<T*>(out) + i;
+  if constexpr (MODE != kModeSingle) {
+    if (ch < D) *reinterpret_cast<typename Duo<T>::type*>(o) = Duo<T>::make(v);
+  } else {
+    if (ch < D) Io<T>::store(o, v.x);
+    if (ch + 1 < D) Io<T>::store(o + 1, v.y);
+  }
+}
+
+// float32 pairs of a [.., D] array
+__device__ __forceinline__ float2 load_pair(const float* a, long long i, int ch, int D) {
+  return make_float2(a != nullptr && ch < D ? a[i] : 0.0f, a != nullptr && ch + 1 < D ? a[i + 1] : 0.0f);
+}
+__device__ __forceinline__ void store_pair(float* a, long long i, int ch, int D, float2 v) {
+  if (ch < D) a[i] = v.x;
+  if (ch + 1 < D) a[i + 1] = v.y;
 }
 
 // ---------------------------------------------------------------- gates
@@ -124,429 +194,402 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }
 
 // e^{-v}. float32: the product with log2 e is carried in two terms (its rounding alone would cost
 // |v| 2^-24 in the result), with v held to +-88 so that both stay finite; 1 / (1 + e^88) flushes
 // to the exact 0 that s(-inf) is.
 template <typename T>
-__device__ __forceinline__ float exp_neg(float v) {
+__device__ __forceinline__ float2 exp_neg(float2 v) {
   if constexpr (sizeof(T) == 2) {
-    return ex2_approx(v * -kLog2e);
+    return ex2_2(mul2(v, bcast2(-kLog2e)));
   } else {
     constexpr float kLog2eLo = 1.9259630e-8f;  // log2 e - kLog2e
-    v = min_nan(max_nan(v, -88.0f), 88.0f);
-    const float t = v * -kLog2e;
-    const float lo = fmaf(v, -kLog2eLo, fmaf(v, -kLog2e, -t));
-    const float e = ex2_approx(t);
-    return fmaf(e, lo * 0.6931471805599453f, e);
+    v = make_float2(min_nan(max_nan(v.x, -88.0f), 88.0f), min_nan(max_nan(v.y, -88.0f), 88.0f));
+    const float2 t = mul2(v, bcast2(-kLog2e));
+    const float2 lo = fma2(v, bcast2(-kLog2eLo), fma2(v, bcast2(-kLog2e), neg2(t)));
+    const float2 e = ex2_2(t);
+    return fma2(e, mul2(lo, bcast2(0.6931471805599453f)), e);
+  }
+}
+__device__ __forceinline__ float2 logistic_of(float2 e) { return rcp_2(add2(e, bcast2(1.0f))); }
+
+// For w = -u >= 0: a = e^{-w} and q = 1 - a. Below 1/2 from the series of q (through w^8 / 8!: the
+// next term is below 2^-26 of the first), which keeps 1 - a^2 = q (1 + a) exact to a few ulp where
+// a is near 1 and holds the decay of long sequences; else the hardware exp2, which keeps a to a few
+// ulp where it is small. NEAR: nu <= 1/2 in every channel of the warp, so w never leaves the series.
+constexpr float kGatedNear = 0.5f;
+template <bool NEAR>
+__device__ __forceinline__ void decay(float2 w, float2& a, float2& q) {
+  float2 s = bcast2(-2.4801587301587302e-5f);        // -1/8!
+  s = fma2(s, w, bcast2(1.9841269841269841e-4f));    // 1/7!
+  s = fma2(s, w, bcast2(-1.3888888888888889e-3f));   // -1/6!
+  s = fma2(s, w, bcast2(8.3333333333333333e-3f));    // 1/5!
+  s = fma2(s, w, bcast2(-4.1666666666666667e-2f));   // -1/4!
+  s = fma2(s, w, bcast2(1.6666666666666667e-1f));    // 1/3!
+  s = fma2(s, w, bcast2(-0.5f));
+  q = fma2(mul2(s, w), w, w);
+  a = sub2(bcast2(1.0f), q);
+  if constexpr (!NEAR) {
+    const float2 e = ex2_2(mul2(w, bcast2(-kLog2e))), f = sub2(bcast2(1.0f), e);
+    const bool nx = w.x < kGatedNear, ny = w.y < kGatedNear;
+    a = make_float2(nx ? a.x : e.x, ny ? a.y : e.y);
+    q = make_float2(nx ? q.x : f.x, ny ? q.y : f.y);
   }
 }
 
-// a = e^u and a - 1 for u <= 0: above -1/2 from the series of e^u - 1 (through u^8 / 8!: the next
-// term is below 2^-26 of the first), which keeps 1 - a^2 = -(a - 1)(2 + (a - 1)) exact to a few
-// ulp where a is near 1 and holds the decay of long sequences; else the hardware exp2, which keeps
-// a to a few ulp where it is small.
-__device__ __forceinline__ float2 exp_expm1_neg(float u) {  // (a, a - 1)
-  float p = 2.4801587301587302e-5f;             // 1/8!
-  p = fmaf(p, u, 1.9841269841269841e-4f);       // 1/7!
-  p = fmaf(p, u, 1.3888888888888889e-3f);       // 1/6!
-  p = fmaf(p, u, 8.3333333333333333e-3f);       // 1/5!
-  p = fmaf(p, u, 4.1666666666666667e-2f);       // 1/4!
-  p = fmaf(p, u, 1.6666666666666667e-1f);       // 1/3!
-  p = fmaf(p, u, 0.5f);
-  const float small = fmaf(p * u, u, u);
-  const float e = ex2_approx(u * kLog2e);
-  const bool near = u > -0.5f;
-  return make_float2(near ? 1.0f + small : e, near ? small : e - 1.0f);
-}
+// nu of a channel, held finite so that nu s(retention) never meets 0 x infinity.
+__device__ __forceinline__ float gated_nu(float nu_log) { return min_nan(expf(nu_log), 3.402823466e38f); }
 
-// -nu of a channel, held finite so that nu s(retention) never meets 0 x infinity.
-__device__ __forceinline__ float gated_minus_nu(float nu_log) { return -min_nan(expf(nu_log), 3.402823466e38f); }
-
-template <typename T>
-__device__ __forceinline__ void gated_ab(float x, float r, float w, float minus_nu, float* a, float* b) {
-  const float sr = rcp_approx(1.0f + exp_neg<T>(r));
-  const float sw = rcp_approx(1.0f + exp_neg<T>(w));
-  const float2 e = exp_expm1_neg(minus_nu * sr);
-  *a = e.x;
-  *b = sqrt_approx(-e.y * (2.0f + e.y)) * sw * x;
+template <typename T, bool NEAR>
+__device__ __forceinline__ void gated_ab(float2 x, float2 r, float2 w, float2 nu, float2& a, float2& b) {
+  const float2 sr = logistic_of(exp_neg<T>(r)), sw = logistic_of(exp_neg<T>(w));
+  float2 q;
+  decay<NEAR>(mul2(nu, sr), a, q);
+  b = mul2(mul2(sqrt_2(mul2(q, add2(a, bcast2(1.0f)))), sw), x);
 }
 
 // 1 - s(v) = e^{-v} s(v) without cancellation, given e = e^{-v} (which may be infinite).
-__device__ __forceinline__ float one_minus_s(float e, float s) { return e > 8.5070592e37f ? 1.0f : e * s; }
+__device__ __forceinline__ float2 one_minus_s(float2 e, float2 s) {
+  const float2 p = mul2(e, s);
+  return make_float2(e.x > 8.5070592e37f ? 1.0f : p.x, e.y > 8.5070592e37f ? 1.0f : p.y);
+}
 
 // ---------------------------------------------------------------- affine maps
 __device__ __forceinline__ bool dropped(float A) { return __float_as_int(A) < 0; }
 
-// v <- A v + H
+// A v + H
 template <bool SEG>
-__device__ __forceinline__ float through(float A, float H, float v) {
-  const float o = fmaf(A, v, H);
-  return SEG && dropped(A) ? H : o;
+__device__ __forceinline__ float2 through(float2 A, float2 H, float2 v) {
+  const float2 o = fma2(A, v, H);
+  if constexpr (!SEG) return o;
+  return make_float2(dropped(A.x) ? H.x : o.x, dropped(A.y) ? H.y : o.y);
 }
 // (A1, H1) then (A2, H2)
 template <bool SEG>
-__device__ __forceinline__ void compose(float& A1, float& H1, float A2, float H2) {
+__device__ __forceinline__ void compose(float2& A1, float2& H1, float2 A2, float2 H2) {
   H1 = through<SEG>(A2, H2, H1);
-  A1 = SEG && dropped(A2) ? A2 : A1 * A2;
+  const float2 A = mul2(A1, A2);
+  A1 = SEG ? make_float2(dropped(A2.x) ? A2.x : A.x, dropped(A2.y) ? A2.y : A.y) : A;
+}
+// A lam, nothing of it at a segment start
+template <bool SEG>
+__device__ __forceinline__ float2 through0(float2 A, float2 lam) {
+  const float2 o = mul2(A, lam);
+  if constexpr (!SEG) return o;
+  return make_float2(dropped(A.x) ? 0.0f : o.x, dropped(A.y) ? 0.0f : o.y);
 }
 
-__device__ __forceinline__ void cluster_barrier() {
+__device__ __forceinline__ void st_cluster(unsigned addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
+__device__ __forceinline__ float4 cat4(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
+
+// The cluster's exchange, one hardware barrier per step. The scan warp's stores to its peers are
+// ordered by its own release and acquire; the other warps only take part.
+__device__ __forceinline__ void cluster_exchange_scan_warp() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void st_cluster(unsigned addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
+__device__ __forceinline__ void cluster_exchange_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_exchange_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+// A cluster's walk: rows of the batch, and in each the steps of its sequence.
+struct GatedWalk {
+  long long bt, step;
+};
 
 // ---------------------------------------------------------------- forward
-template <typename T, int VEC, bool SEG>
-__global__ void __launch_bounds__(kGatedWarps * 32) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
-  using P = Pack<T, VEC>;
-  constexpr int K = kFwdK, NW = kGatedWarps, TILE = K * NW;
-  __shared__ float s_map[2][NW][2 * VEC][32];                 // (A, H) per warp, lane and channel
-  __shared__ float s_cta[2][kGatedMaxCluster][2 * VEC][32];   // and per CTA of the cluster
-  __shared__ float s_carry[2][VEC][32];                       // one CTA: the state leaving its tile
+template <typename T, bool SEG, bool NEAR>
+__device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type* rx, const typename Duo<T>::type* rr,
+                                                 const typename Duo<T>::type* rw, float2 nu, unsigned seg, int live,
+                                                 float2* a, float2* b, float2& A, float2& H) {
+  A = bcast2(1.0f);
+  H = bcast2(0.0f);
+#pragma unroll
+  for (int k = 0; k < kFwdK; ++k) {
+    gated_ab<T, NEAR>(Duo<T>::get(rx[k]), Duo<T>::get(rr[k]), Duo<T>::get(rw[k]), nu, a[k], b[k]);
+    if (SEG && (seg >> k & 1u)) a[k] = bcast2(-0.0f);
+    if (live < kFwdK && k >= live) a[k] = bcast2(1.0f), b[k] = bcast2(0.0f);
+    compose<SEG>(A, H, a[k], b[k]);
+  }
+}
+
+template <typename T, bool SEG, int MODE>
+__global__ void __launch_bounds__(kGatedWarps * 32, 3) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
+  using R = typename Duo<T>::type;
+  constexpr int K = kFwdK, NW = kGatedWarps, TILE = K * NW, S = kFwdStages, NT = 3;
+  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][stage][tensor][token][lane]
+  __shared__ float4 s_map[NW][32];                        // (A, H) of each warp
+  __shared__ float4 s_cta[2][kGatedMaxCluster][32];       // and of each CTA of the cluster
+  __shared__ float2 s_in[NW][32];                         // the state entering each warp's tokens
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
   const unsigned id = blockIdx.x / (unsigned)cs;
-  const int ch = ((int)(id % (unsigned)p.groups) * 32 + lane) * VEC;
-  const bool on = ch < p.D;
-  const long long tiles = (p.L + TILE - 1) / TILE, steps = (tiles + cs - 1) / cs;
-  float nu[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) nu[v] = on ? gated_minus_nu(p.nu_log[ch + v]) : 0.0f;
-  if (cs > 1) cluster_barrier();  // every CTA of the cluster has started before its memory is written
-  int par = 0;
+  const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
+  const long long steps = ((p.L + TILE - 1) / TILE + cs - 1) / cs;
+  R* stage = reinterpret_cast<R*>(s_raw) + (long long)wp * S * NT * K * 32;
+  const float2 nu = make_float2(ch < p.D ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
+  const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
+  if (cs > 1) cluster_exchange_scan_warp();  // every CTA of the cluster has started before its memory is written
 
-  for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
-    float carry[VEC];
+  GatedWalk at{id / (unsigned)p.groups, 0}, ahead = at;
+  auto next = [&](GatedWalk& w) {
+    if (++w.step == steps) w.step = 0, w.bt += p.rows;
+  };
+  auto issue = [&](int slot) {
+    if (ahead.bt < p.B)
+      gated_issue<T, MODE, K, NT>(p, stage + slot * NT * K * 32, ahead.bt, (ahead.step * cs + rank) * TILE + wp * K, ch0, lane);
+    else if (MODE != kModeSingle)
+      copy_commit();  // (an empty group, so that the groups count steps)
+    next(ahead);
+  };
+  auto starts = [&](const GatedWalk& w) {
+    const long long t = (w.step * cs + rank) * TILE + wp * K + lane;
+    return __ballot_sync(0xffffffffu, SEG && lane < K && t < p.L && gated_starts(p.pos, p.pos_bytes, w.bt * p.L + t));
+  };
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = on && p.h0 != nullptr ? p.h0[bt * p.D + ch + v] : 0.0f;
-    if (cs == 1 && wp == NW - 1) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) s_carry[par ^ 1][v][lane] = carry[v];
+  for (int s = 0; s < S - 1; ++s) issue(s);
+  int slot = 0, par = 0;
+  float2 carry = bcast2(0.0f);  // scan warp: the state entering the step
+
+  for (; at.bt < p.B; next(at)) {
+    const long long t0 = (at.step * cs + rank) * TILE + wp * K;
+    const unsigned seg = SEG ? starts(at) : 0u;
+    if (wp == 0 && at.step == 0) carry = load_pair(p.h0, at.bt * p.D + ch, ch, p.D);
+    if constexpr (MODE != kModeSingle) {
+      copy_wait<S - 2>();
+      __syncwarp();
     }
-    typename P::type rx[K], rr[K], rw[K];
-    unsigned seg = 0;  // bit k: token k starts a segment
-    auto fetch = [&](long long step) {
-      const long long t0 = (step * cs + rank) * TILE + wp * K;
-      seg = 0;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const long long t = t0 + k;
-        if (on && t < p.L) {
-          rx[k] = gated_load<T, VEC>(p.x, bt, t, ch);
-          rr[k] = gated_load<T, VEC>(p.r, bt, t, ch);
-          rw[k] = gated_load<T, VEC>(p.w, bt, t, ch);
-        }
-        if (SEG && t < p.L && gated_starts(p.pos, p.pos_bytes, bt * p.L + t)) seg |= 1u << k;
-      }
-    };
-    fetch(0);
-    for (long long step = 0; step < steps; ++step, par ^= 1) {
-      const long long t0 = (step * cs + rank) * TILE + wp * K;
-      float a[K][VEC], b[K][VEC], A[VEC], H[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) A[v] = 1.0f, H[v] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const bool live = on && t0 + k < p.L;
-        float x[VEC], r[VEC], w[VEC];
-        P::get(rx[k], x);
-        P::get(rr[k], r);
-        P::get(rw[k], w);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          gated_ab<T>(x[v], r[v], w[v], nu[v], &a[k][v], &b[k][v]);
-          if (SEG && (seg >> k & 1u)) a[k][v] = -0.0f;
-          if (!live) a[k][v] = 1.0f, b[k][v] = 0.0f;
-          compose<SEG>(A[v], H[v], a[k][v], b[k][v]);
-        }
-      }
-      if (step + 1 < steps) fetch(step + 1);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        s_map[par][wp][2 * v][lane] = A[v];
-        s_map[par][wp][2 * v + 1][lane] = H[v];
-      }
-      __syncthreads();
-      float PA[VEC], PH[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) PA[v] = 1.0f, PH[v] = 0.0f;
-      for (int j = 0; j < wp; ++j) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          compose<SEG>(PA[v], PH[v], s_map[par][j][2 * v][lane], s_map[par][j][2 * v + 1][lane]);
-      }
-      float in[VEC];  // the state entering this CTA's tile
+    float2 a[K], b[K], A, H;
+    {
+      const R* st = stage + slot * NT * K * 32;
+      R rx[K], rr[K], rw[K];
+      gated_read<T, MODE, K>(p, 0, st, at.bt, t0, ch, lane, rx);
+      gated_read<T, MODE, K>(p, 1, st, at.bt, t0, ch, lane, rr);
+      gated_read<T, MODE, K>(p, 2, st, at.bt, t0, ch, lane, rw);
+      const int live = (int)max(0LL, min((long long)K, p.L - t0));
+      if (near) gated_fwd_tokens<T, SEG, true>(rx, rr, rw, nu, seg, live, a, b, A, H);
+      else gated_fwd_tokens<T, SEG, false>(rx, rr, rw, nu, seg, live, a, b, A, H);
+    }
+    __syncwarp();  // the slot before this one has been read by every lane
+    issue(slot == 0 ? S - 1 : slot - 1);
+    slot = slot + 1 == S ? 0 : slot + 1;
+    s_map[wp][lane] = cat4(A, H);
+    __syncthreads();
+    if (wp == 0) {
+      float2 in = carry;  // the state entering this CTA's tile
       if (cs > 1) {
-        if (wp == NW - 1) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            float TA = PA[v], TH = PH[v];
-            compose<SEG>(TA, TH, A[v], H[v]);
-            for (int q = 0; q < cs; ++q) {
-              st_cluster(cluster_smem_addr(&s_cta[par][rank][2 * v][lane], q), TA);
-              st_cluster(cluster_smem_addr(&s_cta[par][rank][2 * v + 1][lane], q), TH);
-            }
-          }
-        }
-        cluster_barrier();
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) in[v] = carry[v];
+        for (int j = 1; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[j][lane]), hi2(s_map[j][lane]));
+        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, H));
+        cluster_exchange_scan_warp();
         for (int q = 0; q < cs; ++q) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            if (q == rank) in[v] = carry[v];
-            carry[v] = through<SEG>(s_cta[par][q][2 * v][lane], s_cta[par][q][2 * v + 1][lane], carry[v]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) in[v] = s_carry[par ^ 1][v][lane];
-      }
-      float h[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) h[v] = through<SEG>(PA[v], PH[v], in[v]);
-      if (p.carry != nullptr && on && t0 % kGatedChunk == 0 && t0 < p.L) {
-        const long long c = (bt * p.chunks + t0 / kGatedChunk) * p.D + ch;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) p.carry[c + v] = h[v];
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = through<SEG>(a[k][v], b[k][v], h[v]);
-        const long long t = t0 + k;
-        if (on && t < p.L) {
-          *reinterpret_cast<typename P::type*>(static_cast<T*>(p.y) + (bt * p.L + t) * p.D + ch) = P::make(h);
-          if (t == p.L - 1 && p.last != nullptr) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) p.last[bt * p.D + ch + v] = h[v];
-          }
+          if (q == rank) in = carry;
+          carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
         }
       }
-      if (cs == 1 && wp == NW - 1) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) s_carry[par][v][lane] = h[v];
+      for (int j = 0; j < NW; ++j) {
+        s_in[j][lane] = in;
+        in = through<SEG>(lo2(s_map[j][lane]), hi2(s_map[j][lane]), in);
       }
+      if (cs == 1) carry = in;
+    } else if (cs > 1) {
+      cluster_exchange_arrive();
     }
+    __syncthreads();
+    if (cs > 1 && wp != 0) cluster_exchange_wait();
+    par ^= 1;
+    float2 h = s_in[wp][lane];
+    if (p.carry != nullptr && t0 % kGatedChunk == 0 && t0 < p.L)
+      store_pair(p.carry, (at.bt * p.chunks + t0 / kGatedChunk) * p.D + ch, ch, p.D, h);
+    const long long i0 = (at.bt * p.L + t0) * p.D + ch;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      h = through<SEG>(a[k], b[k], h);
+      if (t0 + k < p.L) gated_store<T, MODE>(p.y, i0 + (long long)k * p.D, ch, p.D, h);
+    }
+    if (p.last != nullptr && t0 < p.L && t0 + K >= p.L) store_pair(p.last, at.bt * p.D + ch, ch, p.D, h);
   }
+  if constexpr (MODE != kModeSingle) copy_wait<0>();
 }
 
 // ---------------------------------------------------------------- backward
-template <typename T, int VEC, bool SEG>
-__global__ void __launch_bounds__(kGatedWarps * 32) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
-  using P = Pack<T, VEC>;
-  constexpr int K = kBwdK, NW = kGatedWarps, TILE = K * NW;
-  // per warp: A, H (states, forward) and G (adjoints, reverse: out = A in + G)
-  __shared__ float s_map[2][NW][3 * VEC][32];
-  __shared__ float s_cta[2][kGatedMaxCluster][2 * VEC][32];  // (A, G) per CTA of the cluster
-  __shared__ float s_adj[2][VEC][32];                        // one CTA: the adjoint leaving its tile
-  __shared__ double s_nu[NW][VEC][32];
+struct GatedBwdTokens {
+  // c = a or -0; g = sqrt(1 - a^2) s(write); b = g x; bw = b (1 - s(write)); q1 = a w (w = -u >= 0);
+  // q2 = -b a^2 w / (1 - a^2); om = 1 - s(retention)
+  float2 c[kBwdK], g[kBwdK], b[kBwdK], bw[kBwdK], q1[kBwdK], q2[kBwdK], om[kBwdK];
+};
+
+template <typename T, bool SEG, bool NEAR>
+__device__ __forceinline__ void gated_bwd_tokens(const typename Duo<T>::type* rx, const typename Duo<T>::type* rr,
+                                                 const typename Duo<T>::type* rw, float2 nu, unsigned seg, int live,
+                                                 GatedBwdTokens& o, float2& A, float2& H) {
+  A = bcast2(1.0f);
+  H = bcast2(0.0f);
+#pragma unroll
+  for (int k = 0; k < kBwdK; ++k) {
+    const float2 er = exp_neg<T>(Duo<T>::get(rr[k])), ew = exp_neg<T>(Duo<T>::get(rw[k]));
+    const float2 sr = logistic_of(er), sw = logistic_of(ew), w = mul2(nu, sr);
+    float2 a, q;
+    decay<NEAR>(w, a, q);
+    const float2 m = mul2(q, add2(a, bcast2(1.0f)));
+    // (1 - a^2 = 0 only with w = 0, or w too small for float32: the products with m and w are then 0)
+    const float2 rs = make_float2(rsqrt_approx(fmaxf(m.x, 1.17549435e-38f)), rsqrt_approx(fmaxf(m.y, 1.17549435e-38f)));
+    const float2 xs = mul2(Duo<T>::get(rx[k]), sw), beta = mul2(m, rs);
+    o.g[k] = mul2(beta, sw);
+    o.b[k] = mul2(beta, xs);
+    o.bw[k] = mul2(o.b[k], one_minus_s(ew, sw));
+    o.q1[k] = mul2(a, w);
+    o.q2[k] = neg2(mul2(mul2(o.q1[k], a), mul2(xs, rs)));
+    o.om[k] = one_minus_s(er, sr);
+    o.c[k] = a;
+    if (SEG && (seg >> k & 1u)) o.c[k] = bcast2(-0.0f), o.q1[k] = bcast2(-0.0f);
+    if (live < kBwdK && k >= live) o.c[k] = bcast2(1.0f), o.b[k] = bcast2(0.0f);
+    compose<SEG>(A, H, o.c[k], o.b[k]);
+  }
+}
+
+template <typename T, bool SEG, int MODE>
+__global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
+  using R = typename Duo<T>::type;
+  constexpr int K = kBwdK, NW = kGatedWarps, TILE = K * NW, S = kBwdStages, NT = 4;
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  __shared__ float4 s_map[NW][32];                   // (A, H) of each warp: states, forward
+  __shared__ float2 s_adj[NW][32];                   // G: adjoints, in reverse, out = A in + G
+  __shared__ float4 s_cta[2][kGatedMaxCluster][32];  // (A, G) of each CTA of the cluster
+  __shared__ float4 s_in[NW][32];                    // the state and the adjoint entering each warp's tokens
+  __shared__ double2 s_nu[NW][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
   const unsigned id = blockIdx.x / (unsigned)cs;
-  const int ch = ((int)(id % (unsigned)p.groups) * 32 + lane) * VEC;
-  const bool on = ch < p.D;
-  const long long tiles = p.chunks, steps = (tiles + cs - 1) / cs;
-  float nu[VEC];
-  double dnu[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    nu[v] = on ? gated_minus_nu(p.nu_log[ch + v]) : 0.0f;
-    dnu[v] = 0.0;
-  }
-  if (cs > 1) cluster_barrier();
-  int par = 0;
+  const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
+  const long long steps = (p.chunks + cs - 1) / cs;
+  R* stage = reinterpret_cast<R*>(s_raw) + (long long)wp * S * NT * K * 32;
+  const float2 nu = make_float2(ch < p.D ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
+  const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
+  if (cs > 1) cluster_exchange_scan_warp();
 
-  for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
-    float adj[VEC];  // c_{t+1} lam_{t+1} entering the step's last token
+  GatedWalk at{id / (unsigned)p.groups, steps - 1}, ahead = at;
+  auto next = [&](GatedWalk& w) {
+    if (--w.step < 0) w.step = steps - 1, w.bt += p.rows;
+  };
+  auto issue = [&](int slot) {
+    if (ahead.bt < p.B)
+      gated_issue<T, MODE, K, NT>(p, stage + slot * NT * K * 32, ahead.bt, (ahead.step * cs + rank) * TILE + wp * K, ch0, lane);
+    else if (MODE != kModeSingle)
+      copy_commit();
+    next(ahead);
+  };
+  auto starts = [&](const GatedWalk& w) {
+    const long long t = (w.step * cs + rank) * TILE + wp * K + lane;
+    return __ballot_sync(0xffffffffu, SEG && lane < K && t < p.L && gated_starts(p.pos, p.pos_bytes, w.bt * p.L + t));
+  };
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) adj[v] = on && p.grad_last != nullptr ? p.grad_last[bt * p.D + ch + v] : 0.0f;
-    if (cs == 1 && wp == 0) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) s_adj[par ^ 1][v][lane] = adj[v];
+  for (int s = 0; s < S - 1; ++s) issue(s);
+  int slot = 0, par = 0;
+  float2 carry = bcast2(0.0f);  // scan warp: c_{t+1} lam_{t+1} entering the step's last token
+  double dnu_x = 0.0, dnu_y = 0.0;
+
+  for (; at.bt < p.B; next(at)) {
+    const long long tile = at.step * cs + rank, t0 = tile * TILE + wp * K;
+    const unsigned seg = SEG ? starts(at) : 0u;
+    float2 hin = bcast2(0.0f);
+    if (wp == 0) {
+      if (at.step == steps - 1) carry = load_pair(p.grad_last, at.bt * p.D + ch, ch, p.D);
+      if (tile < p.chunks) hin = load_pair(p.carry, (at.bt * p.chunks + tile) * p.D + ch, ch, p.D);
     }
-    typename P::type rx[K], rr[K], rw[K], rd[K];
-    float hc[VEC];
-    unsigned seg = 0;
-    auto fetch = [&](long long step) {
-      const long long tile = step * cs + rank, t0 = tile * TILE + wp * K;
-      seg = 0;
+    if constexpr (MODE != kModeSingle) {
+      copy_wait<S - 2>();
+      __syncwarp();
+    }
+    const R* st = stage + slot * NT * K * 32;
+    const int live = (int)max(0LL, min((long long)K, p.L - t0));
+    GatedBwdTokens o;
+    float2 A, H, G = bcast2(0.0f);
+    R rd[K];
+    {
+      R rx[K], rr[K], rw[K];
+      gated_read<T, MODE, K>(p, 0, st, at.bt, t0, ch, lane, rx);
+      gated_read<T, MODE, K>(p, 1, st, at.bt, t0, ch, lane, rr);
+      gated_read<T, MODE, K>(p, 2, st, at.bt, t0, ch, lane, rw);
+      gated_read<T, MODE, K>(p, 3, st, at.bt, t0, ch, lane, rd);  // (zeros beyond the sequence)
+      if (near) gated_bwd_tokens<T, SEG, true>(rx, rr, rw, nu, seg, live, o, A, H);
+      else gated_bwd_tokens<T, SEG, false>(rx, rr, rw, nu, seg, live, o, A, H);
+    }
 #pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        hc[v] = on && tile < tiles ? p.carry[(bt * p.chunks + tile) * p.D + ch + v] : 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const long long t = t0 + k;
-        if (on && t < p.L) {
-          rx[k] = gated_load<T, VEC>(p.x, bt, t, ch);
-          rr[k] = gated_load<T, VEC>(p.r, bt, t, ch);
-          rw[k] = gated_load<T, VEC>(p.w, bt, t, ch);
-          rd[k] = gated_load<T, VEC>(p.dy, bt, t, ch);
-        }
-        if (SEG && t < p.L && gated_starts(p.pos, p.pos_bytes, bt * p.L + t)) seg |= 1u << k;
-      }
-    };
-    fetch(steps - 1);
-    for (long long step = steps - 1; step >= 0; --step, par ^= 1) {
-      const long long t0 = (step * cs + rank) * TILE + wp * K;
-      // a; g; b = g x; bw = b (1 - s(write)); q1 = -a u; q2 = x s(write) a^2 u / sqrt(1 - a^2);
-      // omr = 1 - s(retention); d = dy
-      float a[K][VEC], g[K][VEC], b[K][VEC], bw[K][VEC], q1[K][VEC], q2[K][VEC], omr[K][VEC], d[K][VEC];
-      float A[VEC], H[VEC], G[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) A[v] = 1.0f, H[v] = 0.0f, G[v] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const bool live = on && t0 + k < p.L;
-        float x[VEC], r[VEC], w[VEC];
-        P::get(rx[k], x);
-        P::get(rr[k], r);
-        P::get(rw[k], w);
-        P::get(rd[k], d[k]);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float er = exp_neg<T>(r[v]), ew = exp_neg<T>(w[v]);
-          const float sr = rcp_approx(1.0f + er), sw = rcp_approx(1.0f + ew);
-          const float u = nu[v] * sr;
-          const float2 e = exp_expm1_neg(u);
-          const float av = e.x, m = -e.y * (2.0f + e.y);
-          const float rs = rsqrt_approx(fmaxf(m, 1.17549435e-38f));
-          const float xs = x[v] * sw;
-          a[k][v] = av;
-          g[k][v] = m * rs * sw;
-          b[k][v] = m * rs * xs;
-          bw[k][v] = b[k][v] * one_minus_s(ew, sw);
-          q1[k][v] = av * -u;  // >= +0, as a
-          q2[k][v] = xs * (av * av) * (u * rs);
-          omr[k][v] = one_minus_s(er, sr);
-          if (SEG && (seg >> k & 1u)) a[k][v] = -0.0f, q1[k][v] = -0.0f;
-          if (!live) a[k][v] = 1.0f, b[k][v] = 0.0f, d[k][v] = 0.0f;
-          compose<SEG>(A[v], H[v], a[k][v], b[k][v]);
-        }
-      }
-#pragma unroll
-      for (int k = K - 1; k >= 0; --k) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) G[v] = through<SEG>(a[k][v], 0.0f, d[k][v] + G[v]);
-      }
-      float h[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) h[v] = hc[v];
-      if (step > 0) fetch(step - 1);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        s_map[par][wp][3 * v][lane] = A[v];
-        s_map[par][wp][3 * v + 1][lane] = H[v];
-        s_map[par][wp][3 * v + 2][lane] = G[v];
-      }
-      __syncthreads();
-      // the state entering this warp's tokens, from the chunk's carry through the warps before
-      for (int j = 0; j < wp; ++j) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          h[v] = through<SEG>(s_map[par][j][3 * v][lane], s_map[par][j][3 * v + 1][lane], h[v]);
-      }
-      // the map of the adjoint through the warps behind
-      float PA[VEC], PG[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) PA[v] = 1.0f, PG[v] = 0.0f;
-      for (int j = NW - 1; j > wp; --j) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          compose<SEG>(PA[v], PG[v], s_map[par][j][3 * v][lane], s_map[par][j][3 * v + 2][lane]);
-      }
-      float c[VEC];
+    for (int k = K - 1; k >= 0; --k) G = through0<SEG>(o.c[k], add2(Duo<T>::get(rd[k]), G));
+    __syncwarp();
+    issue(slot == 0 ? S - 1 : slot - 1);
+    slot = slot + 1 == S ? 0 : slot + 1;
+    s_map[wp][lane] = cat4(A, H);
+    s_adj[wp][lane] = G;
+    __syncthreads();
+    if (wp == 0) {
+      float2 in = carry;  // the adjoint entering this CTA's tile
       if (cs > 1) {
-        if (wp == 0) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            float TA = PA[v], TG = PG[v];
-            compose<SEG>(TA, TG, A[v], G[v]);
-            for (int q = 0; q < cs; ++q) {
-              st_cluster(cluster_smem_addr(&s_cta[par][rank][2 * v][lane], q), TA);
-              st_cluster(cluster_smem_addr(&s_cta[par][rank][2 * v + 1][lane], q), TG);
-            }
-          }
-        }
-        cluster_barrier();
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) c[v] = adj[v];
+        float2 TA = bcast2(1.0f), TG = bcast2(0.0f);
+        for (int j = NW - 1; j >= 0; --j) compose<SEG>(TA, TG, lo2(s_map[j][lane]), s_adj[j][lane]);
+        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(TA, TG));
+        cluster_exchange_scan_warp();
         for (int q = cs - 1; q >= 0; --q) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            if (q == rank) c[v] = adj[v];
-            adj[v] = through<SEG>(s_cta[par][q][2 * v][lane], s_cta[par][q][2 * v + 1][lane], adj[v]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) c[v] = s_adj[par ^ 1][v][lane];
-      }
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) c[v] = through<SEG>(PA[v], PG[v], c[v]);
-      // states forward: q1 <- q1 h_{t-1} + q2 = -du u / lam
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          q1[k][v] = through<SEG>(q1[k][v], q2[k][v], h[v]);
-          h[v] = through<SEG>(a[k][v], b[k][v], h[v]);
-        }
-      }
-      // adjoints in reverse
-      float sum[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) sum[v] = 0.0f;
-#pragma unroll
-      for (int k = K - 1; k >= 0; --k) {
-        const long long t = t0 + k;
-        const bool live = on && t < p.L;
-        float ox[VEC], orr[VEC], ow[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float lam = d[k][v] + c[v];
-          const float du = -lam * q1[k][v];  // du u
-          ox[v] = lam * g[k][v];
-          ow[v] = lam * bw[k][v];
-          orr[v] = du * omr[k][v];
-          if (live) sum[v] += du;
-          c[v] = through<SEG>(a[k][v], 0.0f, lam);
-        }
-        if (live) {
-          const long long i = (bt * p.L + t) * p.D + ch;
-          *reinterpret_cast<typename P::type*>(static_cast<T*>(p.dx) + i) = P::make(ox);
-          *reinterpret_cast<typename P::type*>(static_cast<T*>(p.dr) + i) = P::make(orr);
-          *reinterpret_cast<typename P::type*>(static_cast<T*>(p.dw) + i) = P::make(ow);
+          if (q == rank) in = carry;
+          carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
         }
       }
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) dnu[v] += (double)sum[v];
-      if (wp == 0) {
-        if (cs == 1) {
+      for (int j = 0; j < NW; ++j) {
+        const int i = NW - 1 - j;
+        reinterpret_cast<float2*>(&s_in[j][lane])[0] = hin;
+        hin = through<SEG>(lo2(s_map[j][lane]), hi2(s_map[j][lane]), hin);
+        reinterpret_cast<float2*>(&s_in[i][lane])[1] = in;
+        in = through<SEG>(lo2(s_map[i][lane]), s_adj[i][lane], in);
+      }
+      if (cs == 1) carry = in;
+      if (tile == 0 && p.grad_h0 != nullptr) store_pair(p.grad_h0, at.bt * p.D + ch, ch, p.D, in);
+    } else if (cs > 1) {
+      cluster_exchange_arrive();
+    }
+    __syncthreads();
+    if (cs > 1 && wp != 0) cluster_exchange_wait();
+    par ^= 1;
+    float2 h = lo2(s_in[wp][lane]), c = hi2(s_in[wp][lane]);
+    // states forward: q1 <- q1 h_{t-1} + q2 = -du u / lam
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) s_adj[par][v][lane] = c[v];
-        }
-        if (t0 == 0 && on && p.grad_h0 != nullptr) {
+    for (int k = 0; k < K; ++k) {
+      o.q1[k] = through<SEG>(o.q1[k], o.q2[k], h);
+      h = through<SEG>(o.c[k], o.b[k], h);
+    }
+    // adjoints in reverse
+    float2 sum = bcast2(0.0f);
+    const long long i0 = (at.bt * p.L + t0) * p.D + ch;
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) p.grad_h0[bt * p.D + ch + v] = c[v];
-        }
+    for (int k = K - 1; k >= 0; --k) {
+      const float2 lam = add2(Duo<T>::get(rd[k]), c), du = mul2(neg2(lam), o.q1[k]);
+      c = through0<SEG>(o.c[k], lam);
+      if (k < live) {
+        const long long i = i0 + (long long)k * p.D;
+        gated_store<T, MODE>(p.dx, i, ch, p.D, mul2(lam, o.g[k]));
+        gated_store<T, MODE>(p.dr, i, ch, p.D, mul2(du, o.om[k]));
+        gated_store<T, MODE>(p.dw, i, ch, p.D, mul2(lam, o.bw[k]));
+        sum = add2(sum, du);
       }
     }
+    dnu_x += (double)sum.x;
+    dnu_y += (double)sum.y;
   }
+  if constexpr (MODE != kModeSingle) copy_wait<0>();
   // the CTA's sum of dnu_log per channel, over its warps in order
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) s_nu[wp][v][lane] = dnu[v];
+  s_nu[wp][lane] = make_double2(dnu_x, dnu_y);
   __syncthreads();
-  if (wp == 0 && on) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      double s = 0.0;
-      for (int j = 0; j < NW; ++j) s += s_nu[j][v][lane];
-      p.part[((long long)(id / (unsigned)p.groups) * cs + rank) * p.D + ch + v] = s;
-    }
+  if (wp == 0) {
+    double sx = 0.0, sy = 0.0;
+    for (int j = 0; j < NW; ++j) sx += s_nu[j][lane].x, sy += s_nu[j][lane].y;
+    double* part = p.part + ((long long)(id / (unsigned)p.groups) * cs + rank) * p.D;
+    if (ch < p.D) part[ch] = sx;
+    if (ch + 1 < p.D) part[ch + 1] = sy;
   }
 }
 
@@ -584,16 +627,16 @@ template <typename T>
 __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p) {
   const int d = blockIdx.x * 128 + threadIdx.x;
   if (d >= p.D) return;
-  const float nu = gated_minus_nu(__ldg(p.nu_log + d));
+  const float nu = gated_nu(__ldg(p.nu_log + d));
   for (long long b = blockIdx.y; b < p.B; b += gridDim.y) {
     const float x = Io<T>::load(static_cast<const T*>(p.x) + b * p.sx + d);
     const float r = Io<T>::load(static_cast<const T*>(p.r) + b * p.sr + d);
     const float w = Io<T>::load(static_cast<const T*>(p.w) + b * p.sw + d);
     const float s = p.state[b * p.D + d];
-    float a, c;
-    gated_ab<T>(x, r, w, nu, &a, &c);
+    float2 a, c;
+    gated_ab<T, false>(bcast2(x), bcast2(r), bcast2(w), bcast2(nu), a, c);
     const bool start = p.pos != nullptr && gated_starts(p.pos, p.pos_bytes, b);
-    const float h = start ? c : fmaf(a, s, c);
+    const float h = start ? c.x : fmaf(a.x, s, c.x);
     Io<T>::store(static_cast<T*>(p.y) + b * p.D + d, h);
     p.new_state[b * p.D + d] = h;
   }
@@ -601,18 +644,16 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p
 
 // ---------------------------------------------------------------- host
 struct GatedPlan {
-  int vec, groups, cluster, rows;
+  int groups, cluster, rows;
 };
 
-// Channels two per lane where sizes and strides allow it. The cluster grows (to the portable 8
-// CTAs, no further than the tiles reach) until rows x channel groups x cluster fills the SMs four
-// CTAs each; more rows than a few waves of CTAs need are walked by the same clusters, which
-// bounds the partial sums.
-static GatedPlan gated_plan(long long B, long long L, long long D, bool pairs, int tile) {
+// 64 channels a cluster. The cluster grows (to the portable 8 CTAs, no further than the tiles
+// reach) until rows x channel groups x cluster fills the SMs four CTAs each; more rows than a few
+// waves of CTAs need are walked by the same clusters, which bounds the partial sums.
+static GatedPlan gated_plan(long long B, long long L, long long D, int tile) {
   constexpr long long kFill = 148 * 4, kMost = kFill * 4;
   GatedPlan pl;
-  pl.vec = pairs ? 2 : 1;
-  pl.groups = (int)((D + 32 * pl.vec - 1) / (32 * pl.vec));
+  pl.groups = (int)((D + 63) / 64);
   const long long tiles = (L + tile - 1) / tile;
   pl.cluster = 1;
   while (pl.cluster < kGatedMaxCluster && pl.cluster * 2 <= tiles && B * pl.groups * pl.cluster < kFill) pl.cluster *= 2;
@@ -634,17 +675,33 @@ static bool gated_pos_ok(const void* pos, int bytes) {
   return pos == nullptr || bytes == 1 || bytes == 2 || bytes == 4 || bytes == 8;
 }
 
-static bool gated_pairs(const GatedIn& in, long long B, long long L, int size) {
-  return reinterpret_cast<uintptr_t>(in.p) % (2 * size) == 0 && (B <= 1 || in.sb % 2 == 0) &&
-         (L <= 1 || in.st % 2 == 0);
-}
 static bool gated_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <typename T, int VEC, bool SEG>
+// The widest reads that the inputs' bases, strides and width allow.
+static GatedMode gated_mode(const GatedParams& p, int inputs, int size) {
+  auto fits = [&](int bytes) {
+    bool ok = (long long)p.D * size % bytes == 0;
+    for (int n = 0; n < inputs; ++n)
+      ok = ok && gated_aligned(p.in[n].p, bytes) && (p.B <= 1 || p.in[n].sb * size % bytes == 0) &&
+           (p.L <= 1 || p.in[n].st * size % bytes == 0);
+    return ok;
+  };
+  return fits(16) ? kModeWide : fits(2 * size) ? kModePair : kModeSingle;
+}
+
+template <typename T, bool SEG, int MODE>
 static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_t s) {
+  constexpr int kRow = kGatedWarps * 32 * (int)sizeof(typename Duo<T>::type);
+  const int smem = MODE == kModeSingle ? 0 : kRow * (backward ? kBwdStages * 4 * kBwdK : kFwdStages * 3 * kFwdK);
+  const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
+  if (smem > 0) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.groups * (unsigned)p.rows * (unsigned)p.cluster);
   cfg.blockDim = dim3(kGatedWarps * 32);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -654,24 +711,29 @@ static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_
   cfg.attrs = attr;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
   TimedLaunch tl(backward ? kTimeGatedBwd : kTimeGatedFwd, s);
-  return backward ? cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T, VEC, SEG>, p)
-                  : cudaLaunchKernelEx(&cfg, gated_fwd_kernel<T, VEC, SEG>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <typename T>
-static cudaError_t gated_dispatch(const GatedParams& p, int vec, bool backward, cudaStream_t s) {
-  if (p.pos != nullptr)
-    return vec == 2 ? gated_launch<T, 2, true>(p, backward, s) : gated_launch<T, 1, true>(p, backward, s);
-  return vec == 2 ? gated_launch<T, 2, false>(p, backward, s) : gated_launch<T, 1, false>(p, backward, s);
+template <typename T, bool SEG>
+static cudaError_t gated_modes(const GatedParams& p, GatedMode mode, bool backward, cudaStream_t s) {
+  switch (mode) {
+    case kModeWide: return gated_launch<T, SEG, kModeWide>(p, backward, s);
+    case kModePair: return gated_launch<T, SEG, kModePair>(p, backward, s);
+    default: return gated_launch<T, SEG, kModeSingle>(p, backward, s);
+  }
+}
+
+static cudaError_t gated_dispatch(const GatedParams& p, GatedMode mode, int dtype, bool backward, cudaStream_t s) {
+  if (dtype == SPARC_DTYPE_BF16)
+    return p.pos != nullptr ? gated_modes<__nv_bfloat16, true>(p, mode, backward, s)
+                            : gated_modes<__nv_bfloat16, false>(p, mode, backward, s);
+  return p.pos != nullptr ? gated_modes<float, true>(p, mode, backward, s)
+                          : gated_modes<float, false>(p, mode, backward, s);
 }
 
 static size_t gated_ws_bytes(long long B, long long L, long long D) {
-  size_t rows = 0;  // whichever way the strides let the channels be read
-  for (int pairs = 0; pairs < 2; ++pairs) {
-    const GatedPlan pl = gated_plan(B, L, D, pairs != 0, kGatedChunk);
-    rows = std::max(rows, (size_t)pl.rows * (size_t)pl.cluster);
-  }
-  return rows * (size_t)D * sizeof(double);
+  const GatedPlan pl = gated_plan(B, L, D, kGatedChunk);
+  return (size_t)pl.rows * (size_t)pl.cluster * (size_t)D * sizeof(double);
 }
 
 }  // namespace sparc
@@ -701,9 +763,9 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   if (!gated_pos_ok(a->segment_pos, a->segment_pos_bytes))
     return fail(SPARC_ERR_ARG, "segment_pos_bytes must be 1, 2, 4 or 8");
   GatedParams p = {};
-  p.x = GatedIn{a->x, a->x_batch_stride, a->x_token_stride};
-  p.r = GatedIn{a->retention_gate, a->retention_batch_stride, a->retention_token_stride};
-  p.w = GatedIn{a->write_gate, a->write_batch_stride, a->write_token_stride};
+  p.in[0] = GatedIn{a->x, a->x_batch_stride, a->x_token_stride};
+  p.in[1] = GatedIn{a->retention_gate, a->retention_batch_stride, a->retention_token_stride};
+  p.in[2] = GatedIn{a->write_gate, a->write_batch_stride, a->write_token_stride};
   p.y = a->y;
   p.nu_log = a->nu_log;
   p.h0 = a->h0;
@@ -718,15 +780,13 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
-  const bool pairs = p.D % 2 == 0 && gated_pairs(p.x, p.B, p.L, size) && gated_pairs(p.r, p.B, p.L, size) &&
-                     gated_pairs(p.w, p.B, p.L, size) && gated_aligned(p.y, 2 * size);
-  const GatedPlan pl = gated_plan(p.B, p.L, p.D, pairs, kFwdK * kGatedWarps);
+  const GatedMode mode = gated_aligned(p.y, 2 * size) ? gated_mode(p, 3, size) : kModeSingle;
+  const GatedPlan pl = gated_plan(p.B, p.L, p.D, kFwdK * kGatedWarps);
   p.groups = pl.groups;
   p.cluster = pl.cluster;
   p.rows = pl.rows;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? gated_dispatch<__nv_bfloat16>(p, pl.vec, false, s)
-                                                     : gated_dispatch<float>(p, pl.vec, false, s);
+  const cudaError_t e = gated_dispatch(p, mode, a->dtype, false, s);
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
   return SPARC_OK;
 }
@@ -746,10 +806,10 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
       a->workspace_bytes < gated_ws_bytes(a->batch, a->length, a->channels))
     return fail(SPARC_ERR_WORKSPACE, "workspace missing, too small or not 8-byte aligned");
   GatedParams p = {};
-  p.x = GatedIn{a->x, a->x_batch_stride, a->x_token_stride};
-  p.r = GatedIn{a->retention_gate, a->retention_batch_stride, a->retention_token_stride};
-  p.w = GatedIn{a->write_gate, a->write_batch_stride, a->write_token_stride};
-  p.dy = GatedIn{a->dy, a->dy_batch_stride, a->dy_token_stride};
+  p.in[0] = GatedIn{a->x, a->x_batch_stride, a->x_token_stride};
+  p.in[1] = GatedIn{a->retention_gate, a->retention_batch_stride, a->retention_token_stride};
+  p.in[2] = GatedIn{a->write_gate, a->write_batch_stride, a->write_token_stride};
+  p.in[3] = GatedIn{a->dy, a->dy_batch_stride, a->dy_token_stride};
   p.dx = a->grad_x;
   p.dr = a->grad_retention_gate;
   p.dw = a->grad_write_gate;
@@ -765,22 +825,20 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
   p.D = (int)a->channels;
   p.chunks = sparc_gated_carry_chunks(a->length);
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
-  bool pairs = p.D % 2 == 0;
-  for (const GatedIn* in : {&p.x, &p.r, &p.w, &p.dy}) {
-    if (!gated_aligned(in->p, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
-    pairs = pairs && gated_pairs(*in, p.B, p.L, size);
-  }
+  for (const GatedIn& in : p.in)
+    if (!gated_aligned(in.p, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
+  bool pairs = true;
   for (const void* q : {p.dx, p.dr, p.dw}) {
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
     pairs = pairs && gated_aligned(q, 2 * size);
   }
-  const GatedPlan pl = gated_plan(p.B, p.L, p.D, pairs, kGatedChunk);
+  const GatedMode mode = pairs ? gated_mode(p, 4, size) : kModeSingle;
+  const GatedPlan pl = gated_plan(p.B, p.L, p.D, kGatedChunk);
   p.groups = pl.groups;
   p.cluster = pl.cluster;
   p.rows = pl.rows;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? gated_dispatch<__nv_bfloat16>(p, pl.vec, true, s)
-                                               : gated_dispatch<float>(p, pl.vec, true, s);
+  cudaError_t e = gated_dispatch(p, mode, a->dtype, true, s);
   if (e == cudaSuccess) {
     TimedLaunch tl(kTimeGatedReduce, s);
     gated_reduce_kernel<<<(p.D + 31) / 32, kGatedWarps * 32, 0, s>>>(p.part, a->grad_nu_log, pl.rows * pl.cluster, p.D);
