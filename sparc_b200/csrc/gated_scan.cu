@@ -13,9 +13,9 @@
 // adjacent channels (packed f32x2 arithmetic) and a warp K consecutive tokens; a CTA's eight warps
 // own consecutive spans of K tokens (a tile), and a thread-block cluster's CTAs consecutive tiles;
 // the cluster walks the sequence. A thread turns its K tokens into an affine map (A, H): h_out =
-// A h_in + H in registers; one warp of the CTA runs the state through the warps' maps (and, over
-// distributed shared memory and one cluster barrier, through the maps of the cluster's CTAs) and
-// hands every warp the state entering its tokens, from which they are replayed. The backward does
+// A h_in + H in registers; after one barrier every warp runs the state through the maps of the
+// warps before it (and, over distributed shared memory and one cluster barrier, through those of
+// the cluster's CTAs before its own), and replays its tokens from there. The backward does
 // both directions in one step: the states from the forward's saved chunk carries (float32, one
 // per kGatedChunk tokens, so that the states are not rounded to the activations' type), the
 // adjoints from the step before. The cluster size grows as rows x channels shrink. All orders are
@@ -105,12 +105,11 @@ __device__ __forceinline__ bool gated_starts(const void* pos, int bytes, long lo
 enum GatedMode { kModeWide, kModePair, kModeSingle };
 
 template <int BYTES>
-__device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool valid) {
-  const int n = valid ? BYTES : 0;  // the rest is filled with zeros
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
   if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -118,28 +117,46 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A warp's tokens t0 .. t0 + K - 1 of NT tensors, in stage[tensor][token][lane].
+// A warp's reads of its next tokens: K of them a step, of NT tensors, into stage[tensor][token][lane].
+// Each lane owns pieces of kRows tokens apart, and keeps a pointer per tensor that moves by a
+// constant from step to step. What lies beyond the sequence or the channels is not copied: those
+// values are never used.
 template <typename T, int MODE, int K, int NT>
-__device__ __forceinline__ void gated_issue(const GatedParams& p, typename Duo<T>::type* stage, long long bt,
-                                            long long t0, int ch0, int lane) {
+struct GatedReader {
   using R = typename Duo<T>::type;
-  if constexpr (MODE != kModeSingle) {
-    constexpr int BYTES = MODE == kModeWide ? 16 : (int)sizeof(R);
-    constexpr int ROW = 32 * (int)sizeof(R) / BYTES;  // pieces per token
+  static constexpr int kBytes = MODE == kModeWide ? 16 : (int)sizeof(R);
+  static constexpr int kPieces = 32 * (int)sizeof(R) / kBytes;  // of a token
+  static constexpr int kRows = 32 / kPieces;
+  const T* src[NT];
+  int token, chan;  // this lane's first piece: token of the step, channel
+
+  __device__ __forceinline__ void start(const GatedParams& p, long long bt, long long t0, int ch0, int lane) {
+    if constexpr (MODE == kModeSingle) return;
+    token = lane / kPieces;
+    chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const T* base = static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb;
+    for (int n = 0; n < NT; ++n)
+      src[n] = static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + (t0 + token) * p.in[n].st + chan;
+  }
+  // `left`: tokens of the sequence from the step's first on
+  __device__ __forceinline__ void copy(const GatedParams& p, R* stage, long long left, int lane) {
+    if constexpr (MODE == kModeSingle) return;
+    const int some = chan < p.D ? (int)min(left, (long long)K) : 0;
+    const unsigned dst = smem_addr(stage) + lane * kBytes;
 #pragma unroll
-      for (int c = lane; c < K * ROW; c += 32) {
-        const int k = c / ROW, e = c % ROW * (BYTES / (int)sizeof(T));
-        const bool valid = t0 + k < p.L && ch0 + e < p.D;
-        const T* src = valid ? base + (t0 + k) * p.in[n].st + ch0 + e : static_cast<const T*>(p.in[n].p);
-        copy_async<BYTES>(smem_addr(stage + n * K * 32) + c * BYTES, src, valid);
-      }
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < K / kRows; ++i)
+        if (token + i * kRows < some)
+          copy_async<kBytes>(dst + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * kRows * p.in[n].st);
     copy_commit();
   }
-}
+  __device__ __forceinline__ void move(const GatedParams& p, long long tokens) {
+    if constexpr (MODE == kModeSingle) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) src[n] += tokens * p.in[n].st;
+  }
+};
 
 template <typename T, int MODE, int K>
 __device__ __forceinline__ void gated_read(const GatedParams& p, int n, const typename Duo<T>::type* stage, long long bt,
@@ -158,13 +175,14 @@ __device__ __forceinline__ void gated_read(const GatedParams& p, int n, const ty
   }
 }
 
+// `base`: the same for the whole CTA; `i`: elements from it (below 2^32 bytes, as the widths are limited)
 template <typename T, int MODE>
-__device__ __forceinline__ void gated_store(void* out, long long i, int ch, int D, float2 v) {
-  T* o = static_cast<T*>(out) + i;
+__device__ __forceinline__ void gated_store(T* base, unsigned i, int ch, int D, float2 v) {
+  T* o = reinterpret_cast<T*>(reinterpret_cast<char*>(base) + i * (unsigned)sizeof(T));
   if constexpr (MODE != kModeSingle) {
-    if (ch < D) *reinterpret_cast<typename Duo<T>::type*>(o) = Duo<T>::make(v);
+    *reinterpret_cast<typename Duo<T>::type*>(o) = Duo<T>::make(v);
   } else {
-    if (ch < D) Io<T>::store(o, v.x);
+    Io<T>::store(o, v.x);
     if (ch + 1 < D) Io<T>::store(o + 1, v.y);
   }
 }
@@ -288,13 +306,15 @@ __device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); 
 __device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 cat4(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
 
-// The cluster's exchange, one hardware barrier per step. The scan warp's stores to its peers are
-// ordered by its own release and acquire; the other warps only take part.
-__device__ __forceinline__ void cluster_exchange_scan_warp() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// The cluster's exchange, one hardware barrier per step: only the warp that stored to its peers
+// releases, every warp acquires.
+__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_barrier() {
+  cluster_arrive_release();
+  cluster_wait();
 }
-__device__ __forceinline__ void cluster_exchange_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_exchange_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // A cluster's walk: rows of the batch, and in each the steps of its sequence.
 struct GatedWalk {
@@ -322,9 +342,9 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 3) gated_fwd_kernel(const __
   using R = typename Duo<T>::type;
   constexpr int K = kFwdK, NW = kGatedWarps, TILE = K * NW, S = kFwdStages, NT = 3;
   extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][stage][tensor][token][lane]
-  __shared__ float4 s_map[NW][32];                        // (A, H) of each warp
+  __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
   __shared__ float4 s_cta[2][kGatedMaxCluster][32];       // and of each CTA of the cluster
-  __shared__ float2 s_in[NW][32];                         // the state entering each warp's tokens
+  __shared__ float2 s_out[2][32];                         // one CTA: the state leaving its tile
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
   const unsigned id = blockIdx.x / (unsigned)cs;
@@ -333,17 +353,18 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 3) gated_fwd_kernel(const __
   R* stage = reinterpret_cast<R*>(s_raw) + (long long)wp * S * NT * K * 32;
   const float2 nu = make_float2(ch < p.D ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
-  if (cs > 1) cluster_exchange_scan_warp();  // every CTA of the cluster has started before its memory is written
+  if (cs > 1) cluster_barrier();  // every CTA of the cluster has started before its memory is written
 
   GatedWalk at{id / (unsigned)p.groups, 0}, ahead = at;
   auto next = [&](GatedWalk& w) {
     if (++w.step == steps) w.step = 0, w.bt += p.rows;
   };
-  auto issue = [&](int slot) {
-    if (ahead.bt < p.B)
-      gated_issue<T, MODE, K, NT>(p, stage + slot * NT * K * 32, ahead.bt, (ahead.step * cs + rank) * TILE + wp * K, ch0, lane);
-    else if (MODE != kModeSingle)
-      copy_commit();  // (an empty group, so that the groups count steps)
+  GatedReader<T, MODE, K, NT> reader;
+  auto issue = [&](int slot) {  // (an empty group behind the last step, so that the groups count steps)
+    const long long t0 = (ahead.step * cs + rank) * TILE + wp * K;
+    if (ahead.step == 0) reader.start(p, ahead.bt, t0, ch0, lane);
+    reader.copy(p, stage + slot * NT * K * 32, ahead.bt < p.B ? p.L - t0 : 0, lane);
+    reader.move(p, cs * TILE);
     next(ahead);
   };
   auto starts = [&](const GatedWalk& w) {
@@ -353,65 +374,73 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 3) gated_fwd_kernel(const __
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) issue(s);
   int slot = 0, par = 0;
-  float2 carry = bcast2(0.0f);  // scan warp: the state entering the step
+  float2 carry = bcast2(0.0f);  // the state entering the step
 
   for (; at.bt < p.B; next(at)) {
     const long long t0 = (at.step * cs + rank) * TILE + wp * K;
     const unsigned seg = SEG ? starts(at) : 0u;
-    if (wp == 0 && at.step == 0) carry = load_pair(p.h0, at.bt * p.D + ch, ch, p.D);
+    if (at.step == 0) carry = load_pair(p.h0, at.bt * p.D + ch, ch, p.D);
     if constexpr (MODE != kModeSingle) {
       copy_wait<S - 2>();
       __syncwarp();
     }
     float2 a[K], b[K], A, H;
+    const int live = (int)max(0LL, min((long long)K, p.L - t0));  // tokens of the sequence among these
     {
       const R* st = stage + slot * NT * K * 32;
       R rx[K], rr[K], rw[K];
       gated_read<T, MODE, K>(p, 0, st, at.bt, t0, ch, lane, rx);
       gated_read<T, MODE, K>(p, 1, st, at.bt, t0, ch, lane, rr);
       gated_read<T, MODE, K>(p, 2, st, at.bt, t0, ch, lane, rw);
-      const int live = (int)max(0LL, min((long long)K, p.L - t0));
       if (near) gated_fwd_tokens<T, SEG, true>(rx, rr, rw, nu, seg, live, a, b, A, H);
       else gated_fwd_tokens<T, SEG, false>(rx, rr, rw, nu, seg, live, a, b, A, H);
     }
     __syncwarp();  // the slot before this one has been read by every lane
     issue(slot == 0 ? S - 1 : slot - 1);
     slot = slot + 1 == S ? 0 : slot + 1;
-    s_map[wp][lane] = cat4(A, H);
+    s_map[par][wp][lane] = cat4(A, H);
     __syncthreads();
-    if (wp == 0) {
-      float2 in = carry;  // the state entering this CTA's tile
-      if (cs > 1) {
-        for (int j = 1; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[j][lane]), hi2(s_map[j][lane]));
-        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, H));
-        cluster_exchange_scan_warp();
-        for (int q = 0; q < cs; ++q) {
-          if (q == rank) in = carry;
-          carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
-        }
-      }
+    float2 h;  // the state entering this CTA's tile, then this warp's tokens
+    if (cs > 1) {
+      if (wp == NW - 1) {
+        A = bcast2(1.0f), H = bcast2(0.0f);
 #pragma unroll
-      for (int j = 0; j < NW; ++j) {
-        s_in[j][lane] = in;
-        in = through<SEG>(lo2(s_map[j][lane]), hi2(s_map[j][lane]), in);
+        for (int j = 0; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]));
+        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, H));
+        cluster_arrive_release();
+      } else {
+        cluster_arrive_relaxed();
       }
-      if (cs == 1) carry = in;
-    } else if (cs > 1) {
-      cluster_exchange_arrive();
+      cluster_wait();
+      for (int q = 0; q < rank; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+      h = carry;
+      for (int q = rank; q < cs; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+    } else {
+      h = at.step == 0 ? carry : s_out[par ^ 1][lane];
     }
-    __syncthreads();
-    if (cs > 1 && wp != 0) cluster_exchange_wait();
-    par ^= 1;
-    float2 h = s_in[wp][lane];
+#pragma unroll
+    for (int j = 0; j < NW - 1; ++j)
+      if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
     if (p.carry != nullptr && t0 % kGatedChunk == 0 && t0 < p.L)
       store_pair(p.carry, (at.bt * p.chunks + t0 / kGatedChunk) * p.D + ch, ch, p.D, h);
-    const long long i0 = (at.bt * p.L + t0) * p.D + ch;
+    T* y = static_cast<T*>(p.y) + (at.bt * p.L + (at.step * cs + rank) * TILE) * p.D;
+    const unsigned i0 = (unsigned)(wp * K) * (unsigned)p.D + (unsigned)ch;
+    if (live == K && ch < p.D) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      h = through<SEG>(a[k], b[k], h);
-      if (t0 + k < p.L) gated_store<T, MODE>(p.y, i0 + (long long)k * p.D, ch, p.D, h);
+      for (int k = 0; k < K; ++k) {
+        h = through<SEG>(a[k], b[k], h);
+        gated_store<T, MODE>(y, i0 + (unsigned)(k * p.D), ch, p.D, h);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        h = through<SEG>(a[k], b[k], h);
+        if (k < live && ch < p.D) gated_store<T, MODE>(y, i0 + (unsigned)(k * p.D), ch, p.D, h);
+      }
     }
     if (p.last != nullptr && t0 < p.L && t0 + K >= p.L) store_pair(p.last, at.bt * p.D + ch, ch, p.D, h);
+    if (cs == 1 && wp == NW - 1) s_out[par][lane] = h;
+    par ^= 1;
   }
   if constexpr (MODE != kModeSingle) copy_wait<0>();
 }
@@ -457,10 +486,10 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
   using R = typename Duo<T>::type;
   constexpr int K = kBwdK, NW = kGatedWarps, TILE = K * NW, S = kBwdStages, NT = 4;
   extern __shared__ __align__(16) unsigned char s_raw[];
-  __shared__ float4 s_map[NW][32];                   // (A, H) of each warp: states, forward
-  __shared__ float2 s_adj[NW][32];                   // G: adjoints, in reverse, out = A in + G
+  __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
+  __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
   __shared__ float4 s_cta[2][kGatedMaxCluster][32];  // (A, G) of each CTA of the cluster
-  __shared__ float4 s_in[NW][32];                    // the state and the adjoint entering each warp's tokens
+  __shared__ float2 s_out[2][32];                    // one CTA: the adjoint leaving its tile
   __shared__ double2 s_nu[NW][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
@@ -470,17 +499,18 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
   R* stage = reinterpret_cast<R*>(s_raw) + (long long)wp * S * NT * K * 32;
   const float2 nu = make_float2(ch < p.D ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
-  if (cs > 1) cluster_exchange_scan_warp();
+  if (cs > 1) cluster_barrier();
 
   GatedWalk at{id / (unsigned)p.groups, steps - 1}, ahead = at;
   auto next = [&](GatedWalk& w) {
     if (--w.step < 0) w.step = steps - 1, w.bt += p.rows;
   };
+  GatedReader<T, MODE, K, NT> reader;
   auto issue = [&](int slot) {
-    if (ahead.bt < p.B)
-      gated_issue<T, MODE, K, NT>(p, stage + slot * NT * K * 32, ahead.bt, (ahead.step * cs + rank) * TILE + wp * K, ch0, lane);
-    else if (MODE != kModeSingle)
-      copy_commit();
+    const long long t0 = (ahead.step * cs + rank) * TILE + wp * K;
+    if (ahead.step == steps - 1) reader.start(p, ahead.bt, t0, ch0, lane);
+    reader.copy(p, stage + slot * NT * K * 32, ahead.bt < p.B ? p.L - t0 : 0, lane);
+    reader.move(p, -cs * TILE);
     next(ahead);
   };
   auto starts = [&](const GatedWalk& w) {
@@ -490,17 +520,15 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) issue(s);
   int slot = 0, par = 0;
-  float2 carry = bcast2(0.0f);  // scan warp: c_{t+1} lam_{t+1} entering the step's last token
+  float2 carry = bcast2(0.0f);  // c_{t+1} lam_{t+1} entering the step's last token
   double dnu_x = 0.0, dnu_y = 0.0;
 
   for (; at.bt < p.B; next(at)) {
     const long long tile = at.step * cs + rank, t0 = tile * TILE + wp * K;
     const unsigned seg = SEG ? starts(at) : 0u;
-    float2 hin = bcast2(0.0f);
-    if (wp == 0) {
-      if (at.step == steps - 1) carry = load_pair(p.grad_last, at.bt * p.D + ch, ch, p.D);
-      if (tile < p.chunks) hin = load_pair(p.carry, (at.bt * p.chunks + tile) * p.D + ch, ch, p.D);
-    }
+    if (at.step == steps - 1) carry = load_pair(p.grad_last, at.bt * p.D + ch, ch, p.D);
+    // the state entering this CTA's tile
+    float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (at.bt * p.chunks + tile) * p.D + ch, ch, p.D);
     if constexpr (MODE != kModeSingle) {
       copy_wait<S - 2>();
       __syncwarp();
@@ -515,7 +543,12 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
       gated_read<T, MODE, K>(p, 0, st, at.bt, t0, ch, lane, rx);
       gated_read<T, MODE, K>(p, 1, st, at.bt, t0, ch, lane, rr);
       gated_read<T, MODE, K>(p, 2, st, at.bt, t0, ch, lane, rw);
-      gated_read<T, MODE, K>(p, 3, st, at.bt, t0, ch, lane, rd);  // (zeros beyond the sequence)
+      gated_read<T, MODE, K>(p, 3, st, at.bt, t0, ch, lane, rd);
+      if (live < K) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (k >= live) rd[k] = Duo<T>::make(bcast2(0.0f));
+      }
       if (near) gated_bwd_tokens<T, SEG, true>(rx, rr, rw, nu, seg, live, o, A, H);
       else gated_bwd_tokens<T, SEG, false>(rx, rr, rw, nu, seg, live, o, A, H);
     }
@@ -524,38 +557,37 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
     __syncwarp();
     issue(slot == 0 ? S - 1 : slot - 1);
     slot = slot + 1 == S ? 0 : slot + 1;
-    s_map[wp][lane] = cat4(A, H);
-    s_adj[wp][lane] = G;
+    s_map[par][wp][lane] = cat4(A, H);
+    s_adj[par][wp][lane] = G;
     __syncthreads();
-    if (wp == 0) {
-      float2 in = carry;  // the adjoint entering this CTA's tile
-      if (cs > 1) {
-        float2 TA = bcast2(1.0f), TG = bcast2(0.0f);
-        for (int j = NW - 1; j >= 0; --j) compose<SEG>(TA, TG, lo2(s_map[j][lane]), s_adj[j][lane]);
-        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(TA, TG));
-        cluster_exchange_scan_warp();
-        for (int q = cs - 1; q >= 0; --q) {
-          if (q == rank) in = carry;
-          carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
-        }
-      }
+    float2 c;  // the adjoint entering this CTA's tile, then this warp's tokens
+    if (cs > 1) {
+      if (wp == 0) {
 #pragma unroll
-      for (int j = 0; j < NW; ++j) {
-        const int i = NW - 1 - j;
-        reinterpret_cast<float2*>(&s_in[j][lane])[0] = hin;
-        hin = through<SEG>(lo2(s_map[j][lane]), hi2(s_map[j][lane]), hin);
-        reinterpret_cast<float2*>(&s_in[i][lane])[1] = in;
-        in = through<SEG>(lo2(s_map[i][lane]), s_adj[i][lane], in);
+        for (int j = 0, i = NW - 1; j < NW; ++j, --i) {
+          if (j == 0) A = lo2(s_map[par][i][lane]), G = s_adj[par][i][lane];
+          else compose<SEG>(A, G, lo2(s_map[par][i][lane]), s_adj[par][i][lane]);
+        }
+        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, G));
+        cluster_arrive_release();
+      } else {
+        cluster_arrive_relaxed();
       }
-      if (cs == 1) carry = in;
-      if (tile == 0 && p.grad_h0 != nullptr) store_pair(p.grad_h0, at.bt * p.D + ch, ch, p.D, in);
-    } else if (cs > 1) {
-      cluster_exchange_arrive();
     }
-    __syncthreads();
-    if (cs > 1 && wp != 0) cluster_exchange_wait();
-    par ^= 1;
-    float2 h = lo2(s_in[wp][lane]), c = hi2(s_in[wp][lane]);
+#pragma unroll
+    for (int j = 0; j < NW - 1; ++j)
+      if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
+    if (cs > 1) {
+      cluster_wait();
+      for (int q = cs - 1; q > rank; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+      c = carry;
+      for (int q = rank; q >= 0; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+    } else {
+      c = at.step == steps - 1 ? carry : s_out[par ^ 1][lane];
+    }
+#pragma unroll
+    for (int j = NW - 1; j > 0; --j)
+      if (j > wp) c = through<SEG>(lo2(s_map[par][j][lane]), s_adj[par][j][lane], c);
     // states forward: q1 <- q1 h_{t-1} + q2 = -du u / lam
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -564,21 +596,34 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
     }
     // adjoints in reverse
     float2 sum = bcast2(0.0f);
-    const long long i0 = (at.bt * p.L + t0) * p.D + ch;
-#pragma unroll
-    for (int k = K - 1; k >= 0; --k) {
+    const long long base = (at.bt * p.L + tile * TILE) * p.D;
+    T *dx = static_cast<T*>(p.dx) + base, *dr = static_cast<T*>(p.dr) + base, *dw = static_cast<T*>(p.dw) + base;
+    const unsigned i0 = (unsigned)(wp * K) * (unsigned)p.D + (unsigned)ch;
+    auto token = [&](int k, bool store) {
       const float2 lam = add2(Duo<T>::get(rd[k]), c), du = mul2(neg2(lam), o.q1[k]);
       c = through0<SEG>(o.c[k], lam);
-      if (k < live) {
-        const long long i = i0 + (long long)k * p.D;
-        gated_store<T, MODE>(p.dx, i, ch, p.D, mul2(lam, o.g[k]));
-        gated_store<T, MODE>(p.dr, i, ch, p.D, mul2(du, o.om[k]));
-        gated_store<T, MODE>(p.dw, i, ch, p.D, mul2(lam, o.bw[k]));
+      if (store) {
+        const unsigned i = i0 + (unsigned)(k * p.D);
+        gated_store<T, MODE>(dx, i, ch, p.D, mul2(lam, o.g[k]));
+        gated_store<T, MODE>(dr, i, ch, p.D, mul2(du, o.om[k]));
+        gated_store<T, MODE>(dw, i, ch, p.D, mul2(lam, o.bw[k]));
         sum = add2(sum, du);
       }
+    };
+    if (live == K && ch < p.D) {
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k) token(k, true);
+    } else {
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k) token(k, k < live && ch < p.D);
     }
     dnu_x += (double)sum.x;
     dnu_y += (double)sum.y;
+    if (wp == 0) {
+      if (cs == 1) s_out[par][lane] = c;
+      if (tile == 0 && p.grad_h0 != nullptr) store_pair(p.grad_h0, at.bt * p.D + ch, ch, p.D, c);
+    }
+    par ^= 1;
   }
   if constexpr (MODE != kModeSingle) copy_wait<0>();
   // the CTA's sum of dnu_log per channel, over its warps in order
@@ -666,8 +711,8 @@ static bool gated_valid_dtype(int d) { return d == SPARC_DTYPE_F32 || d == SPARC
 
 static int gated_check_shape(long long B, long long L, long long D) {
   if (B <= 0 || L <= 0 || D <= 0) return fail(SPARC_ERR_SHAPE, "batch, length and channels must be positive");
-  if (D > (1LL << 24) || B > (1LL << 31) || L > (1LL << 40) || (double)B * (double)L * (double)D > 4.0e18)
-    return fail(SPARC_ERR_SHAPE, "shape beyond the launch grid (channels <= 2^24, batch <= 2^31)");
+  if (D > (1LL << 22) || B > (1LL << 31) || L > (1LL << 40) || (double)B * (double)L * (double)D > 4.0e18)
+    return fail(SPARC_ERR_SHAPE, "shape beyond the launch grid (channels <= 2^22, batch <= 2^31)");
   return SPARC_OK;
 }
 
