@@ -34,13 +34,24 @@
 namespace sparc {
 
 constexpr int kGatedChunk = 32;  // tokens per saved carry
-constexpr int kGatedWarps = 8;   // warps per CTA
-constexpr int kFwdK = 8;         // tokens per thread and step, forward
-constexpr int kBwdK = 4;         // tokens per thread and step, backward (a chunk per CTA and step)
 constexpr int kGatedMaxCluster = 8;
-constexpr int kFwdStages = 2, kBwdStages = 3;  // steps of inputs held in shared memory
-static_assert(kBwdK * kGatedWarps == kGatedChunk, "the backward's tile is one chunk");
-static_assert(kGatedChunk % kFwdK == 0, "a carry is some thread's entering state");
+
+// How a CTA cuts its tile: WARPS spans of K tokens, STAGES steps of inputs in shared memory, BLOCKS
+// CTAs per SM that the registers are held to.
+template <int K_, int WARPS_, int STAGES_, int BLOCKS_>
+struct GatedCut {
+  static constexpr int K = K_, WARPS = WARPS_, STAGES = STAGES_, BLOCKS = BLOCKS_, TILE = K * WARPS;
+};
+template <typename T> struct GatedFwdCut;
+template <> struct GatedFwdCut<__nv_bfloat16> : GatedCut<16, 4, 2, 4> {};
+template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2, 2> {};
+template <typename T> struct GatedBwdCut;
+template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 2, 3> {};
+template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2, 2> {};
+constexpr int kFwdTile = 64;  // of either type, so that the plans are
+static_assert(GatedFwdCut<float>::TILE == kFwdTile && GatedFwdCut<__nv_bfloat16>::TILE == kFwdTile);
+// the backward's tile is one chunk
+static_assert(GatedBwdCut<float>::TILE == kGatedChunk && GatedBwdCut<__nv_bfloat16>::TILE == kGatedChunk);
 
 struct GatedIn {
   const void* p;
@@ -60,7 +71,8 @@ struct GatedParams {
   double* part;        // [rows * cluster, D] partial sums of dnu_log
   const void* pos;     // segment positions [B, L] or null
   int pos_bytes;
-  long long B, L, chunks;
+  long long B;
+  int L, chunks;
   int D, groups, cluster, rows;  // rows: clusters per channel group, each walking rows of the batch
 };
 
@@ -118,49 +130,68 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 // A warp's reads of its next tokens: K of them a step, of NT tensors, into stage[tensor][token][lane].
-// Each lane owns pieces of kRows tokens apart, and keeps a pointer per tensor that moves by a
-// constant from step to step. What lies beyond the sequence or the channels is not copied: those
-// values are never used.
+// Each lane owns pieces kRows tokens apart, and keeps a pointer per tensor that moves by a constant
+// from step to step. What lies beyond the sequence or the channels is not copied: those values are
+// never used.
 template <typename T, int MODE, int K, int NT>
 struct GatedReader {
   using R = typename Duo<T>::type;
   static constexpr int kBytes = MODE == kModeWide ? 16 : (int)sizeof(R);
   static constexpr int kPieces = 32 * (int)sizeof(R) / kBytes;  // of a token
   static constexpr int kRows = 32 / kPieces;
-  const T* src[NT];
-  int token, chan;  // this lane's first piece: token of the step, channel
+  const char* src[NT];
+  long long row[NT], move[NT];  // bytes from a piece to the next, from a step to the next
+  unsigned dst;                 // this lane's first piece in a stage
+  int token;                    // and its token of the step (none of this lane's where its channels are beyond D)
 
-  __device__ __forceinline__ void start(const GatedParams& p, long long bt, long long t0, int ch0, int lane) {
+  __device__ __forceinline__ GatedReader(const GatedParams& p, R* stage, int ch0, int lane, int tokens) {
     if constexpr (MODE == kModeSingle) return;
-    token = lane / kPieces;
-    chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
+    const int chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
+    token = chan < p.D ? lane / kPieces : K;
+    dst = smem_addr(stage) + lane * kBytes;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      src[n] = static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + (t0 + token) * p.in[n].st + chan;
+    for (int n = 0; n < NT; ++n) {
+      row[n] = kRows * p.in[n].st * (int)sizeof(T);
+      move[n] = tokens * p.in[n].st * (int)sizeof(T);
+    }
   }
-  // `left`: tokens of the sequence from the step's first on
-  __device__ __forceinline__ void copy(const GatedParams& p, R* stage, long long left, int lane) {
+  __device__ __forceinline__ void start(const GatedParams& p, long long bt, int t0, int ch0, int lane) {
     if constexpr (MODE == kModeSingle) return;
-    const int some = chan < p.D ? (int)min(left, (long long)K) : 0;
-    const unsigned dst = smem_addr(stage) + lane * kBytes;
+    const int chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
+      src[n] = reinterpret_cast<const char*>(static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb +
+                                             (long long)(t0 + lane / kPieces) * p.in[n].st + chan);
+  }
+  // `left`: tokens of the sequence from this step's first on (none: an empty group, so that the groups count steps)
+  __device__ __forceinline__ void copy(int slot, int left) {
+    if constexpr (MODE == kModeSingle) return;
+    const unsigned to = dst + slot * (NT * K * 32 * (int)sizeof(R));
+    if (left >= K) {
+      if (token < K) {
 #pragma unroll
-      for (int i = 0; i < K / kRows; ++i)
-        if (token + i * kRows < some)
-          copy_async<kBytes>(dst + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * kRows * p.in[n].st);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < K / kRows; ++i)
+            copy_async<kBytes>(to + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < K / kRows; ++i)
+          if (token < K && token + i * kRows < left)
+            copy_async<kBytes>(to + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
+    }
     copy_commit();
-  }
-  __device__ __forceinline__ void move(const GatedParams& p, long long tokens) {
-    if constexpr (MODE == kModeSingle) return;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) src[n] += tokens * p.in[n].st;
+    for (int n = 0; n < NT; ++n) src[n] += move[n];
   }
 };
 
 template <typename T, int MODE, int K>
 __device__ __forceinline__ void gated_read(const GatedParams& p, int n, const typename Duo<T>::type* stage, long long bt,
-                                           long long t0, int ch, int lane, typename Duo<T>::type* v) {
+                                           int t0, int ch, int lane, typename Duo<T>::type* v) {
   if constexpr (MODE != kModeSingle) {
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = stage[(n * K + k) * 32 + lane];
@@ -169,16 +200,14 @@ __device__ __forceinline__ void gated_read(const GatedParams& p, int n, const ty
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const bool ok = t0 + k < p.L;
-      const T* q = base + (t0 + k) * p.in[n].st;
+      const T* q = base + (long long)(t0 + k) * p.in[n].st;
       v[k] = Duo<T>::join(ok && ch < p.D ? Duo<T>::bits(q) : 0, ok && ch + 1 < p.D ? Duo<T>::bits(q + 1) : 0);
     }
   }
 }
 
-// `base`: the same for the whole CTA; `i`: elements from it (below 2^32 bytes, as the widths are limited)
 template <typename T, int MODE>
-__device__ __forceinline__ void gated_store(T* base, unsigned i, int ch, int D, float2 v) {
-  T* o = reinterpret_cast<T*>(reinterpret_cast<char*>(base) + i * (unsigned)sizeof(T));
+__device__ __forceinline__ void gated_store(T* o, int ch, int D, float2 v) {
   if constexpr (MODE != kModeSingle) {
     *reinterpret_cast<typename Duo<T>::type*>(o) = Duo<T>::make(v);
   } else {
@@ -214,57 +243,92 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
 }
 __device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }
 
+// The functions below take N tokens' pairs at once, an operation after the other over all of them:
+// a constant of packed arithmetic is a pair of registers that two moves set, which N tokens share.
+
 // e^{-v}. float32: the product with log2 e is carried in two terms (its rounding alone would cost
 // |v| 2^-24 in the result), with v held to +-88 so that both stay finite; 1 / (1 + e^88) flushes
 // to the exact 0 that s(-inf) is.
-template <typename T>
-__device__ __forceinline__ float2 exp_neg(float2 v) {
+template <typename T, int N>
+__device__ __forceinline__ void exp_neg(const float2 (&v)[N], float2 (&e)[N]) {
   if constexpr (sizeof(T) == 2) {
-    return ex2_2(mul2(v, bcast2(-kLog2e)));
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = mul2(v[k], bcast2(-kLog2e));
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = ex2_2(e[k]);
   } else {
     constexpr float kLog2eLo = 1.9259630e-8f;  // log2 e - kLog2e
-    v = make_float2(min_nan(max_nan(v.x, -88.0f), 88.0f), min_nan(max_nan(v.y, -88.0f), 88.0f));
-    const float2 t = mul2(v, bcast2(-kLog2e));
-    const float2 lo = fma2(v, bcast2(-kLog2eLo), fma2(v, bcast2(-kLog2e), neg2(t)));
-    const float2 e = ex2_2(t);
-    return fma2(e, mul2(lo, bcast2(0.6931471805599453f)), e);
+    float2 lo[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float2 c = make_float2(min_nan(max_nan(v[k].x, -88.0f), 88.0f), min_nan(max_nan(v[k].y, -88.0f), 88.0f));
+      const float2 t = mul2(c, bcast2(-kLog2e));
+      lo[k] = mul2(fma2(c, bcast2(-kLog2eLo), fma2(c, bcast2(-kLog2e), neg2(t))), bcast2(0.6931471805599453f));
+      e[k] = t;
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = ex2_2(e[k]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) e[k] = fma2(e[k], lo[k], e[k]);
   }
 }
-__device__ __forceinline__ float2 logistic_of(float2 e) { return rcp_2(add2(e, bcast2(1.0f))); }
+// s = 1 / (1 + e)
+template <int N>
+__device__ __forceinline__ void logistic_of(const float2 (&e)[N], float2 (&s)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = add2(e[k], bcast2(1.0f));
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = rcp_2(s[k]);
+}
 
 // For w = -u >= 0: a = e^{-w} and q = 1 - a. Below 1/2 from the series of q (through w^8 / 8!: the
 // next term is below 2^-26 of the first), which keeps 1 - a^2 = q (1 + a) exact to a few ulp where
 // a is near 1 and holds the decay of long sequences; else the hardware exp2, which keeps a to a few
 // ulp where it is small. NEAR: nu <= 1/2 in every channel of the warp, so w never leaves the series.
 constexpr float kGatedNear = 0.5f;
-template <bool NEAR>
-__device__ __forceinline__ void decay(float2 w, float2& a, float2& q) {
-  float2 s = bcast2(-2.4801587301587302e-5f);        // -1/8!
-  s = fma2(s, w, bcast2(1.9841269841269841e-4f));    // 1/7!
-  s = fma2(s, w, bcast2(-1.3888888888888889e-3f));   // -1/6!
-  s = fma2(s, w, bcast2(8.3333333333333333e-3f));    // 1/5!
-  s = fma2(s, w, bcast2(-4.1666666666666667e-2f));   // -1/4!
-  s = fma2(s, w, bcast2(1.6666666666666667e-1f));    // 1/3!
-  s = fma2(s, w, bcast2(-0.5f));
-  q = fma2(mul2(s, w), w, w);
-  a = sub2(bcast2(1.0f), q);
+template <bool NEAR, int N>
+__device__ __forceinline__ void decay(const float2 (&w)[N], float2 (&a)[N], float2 (&q)[N]) {
+  constexpr float kSeries[6] = {1.9841269841269841e-4f,  -1.3888888888888889e-3f, 8.3333333333333333e-3f,
+                                -4.1666666666666667e-2f, 1.6666666666666667e-1f,  -0.5f};  // 1/7! ... -1/2!
+#pragma unroll
+  for (int k = 0; k < N; ++k) q[k] = bcast2(-2.4801587301587302e-5f);  // -1/8!
+#pragma unroll
+  for (int i = 0; i < 6; ++i)
+#pragma unroll
+    for (int k = 0; k < N; ++k) q[k] = fma2(q[k], w[k], bcast2(kSeries[i]));
+#pragma unroll
+  for (int k = 0; k < N; ++k) q[k] = fma2(mul2(q[k], w[k]), w[k], w[k]);
+#pragma unroll
+  for (int k = 0; k < N; ++k) a[k] = sub2(bcast2(1.0f), q[k]);
   if constexpr (!NEAR) {
-    const float2 e = ex2_2(mul2(w, bcast2(-kLog2e))), f = sub2(bcast2(1.0f), e);
-    const bool nx = w.x < kGatedNear, ny = w.y < kGatedNear;
-    a = make_float2(nx ? a.x : e.x, ny ? a.y : e.y);
-    q = make_float2(nx ? q.x : f.x, ny ? q.y : f.y);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float2 e = ex2_2(mul2(w[k], bcast2(-kLog2e))), f = sub2(bcast2(1.0f), e);
+      const bool nx = w[k].x < kGatedNear, ny = w[k].y < kGatedNear;
+      a[k] = make_float2(nx ? a[k].x : e.x, ny ? a[k].y : e.y);
+      q[k] = make_float2(nx ? q[k].x : f.x, ny ? q[k].y : f.y);
+    }
   }
 }
 
 // nu of a channel, held finite so that nu s(retention) never meets 0 x infinity.
 __device__ __forceinline__ float gated_nu(float nu_log) { return min_nan(expf(nu_log), 3.402823466e38f); }
 
-template <typename T, bool NEAR>
-__device__ __forceinline__ void gated_ab(float2 x, float2 r, float2 w, float2 nu, float2& a, float2& b) {
-  const float2 sr = logistic_of(exp_neg<T>(r)), sw = logistic_of(exp_neg<T>(w));
-  float2 q;
-  decay<NEAR>(mul2(nu, sr), a, q);
-  b = mul2(mul2(sqrt_2(mul2(q, add2(a, bcast2(1.0f)))), sw), x);
+template <typename T, bool NEAR, int N>
+__device__ __forceinline__ void gated_ab(const float2 (&x)[N], const float2 (&r)[N], const float2 (&w)[N], float2 nu,
+                                         float2 (&a)[N], float2 (&b)[N]) {
+  float2 e[N], q[N], sw[N];
+  exp_neg<T>(r, e);
+  logistic_of(e, q);
+  exp_neg<T>(w, e);
+  logistic_of(e, sw);
+#pragma unroll
+  for (int k = 0; k < N; ++k) e[k] = mul2(nu, q[k]);
+  decay<NEAR>(e, a, q);
+#pragma unroll
+  for (int k = 0; k < N; ++k) q[k] = mul2(q[k], add2(a[k], bcast2(1.0f)));
+#pragma unroll
+  for (int k = 0; k < N; ++k) b[k] = mul2(mul2(sqrt_2(q[k]), sw[k]), x[k]);
 }
 
 // 1 - s(v) = e^{-v} s(v) without cancellation, given e = e^{-v} (which may be infinite).
@@ -316,31 +380,34 @@ __device__ __forceinline__ void cluster_barrier() {
   cluster_wait();
 }
 
-// A cluster's walk: rows of the batch, and in each the steps of its sequence.
-struct GatedWalk {
-  long long bt, step;
-};
+// Which of a warp's K tokens from t0 on start a segment, as bits.
+template <int K>
+__device__ __forceinline__ unsigned gated_segments(const GatedParams& p, long long bt, int t0, int lane) {
+  const int t = t0 + lane;
+  return __ballot_sync(0xffffffffu, lane < K && t < p.L && gated_starts(p.pos, p.pos_bytes, bt * p.L + t));
+}
 
 // ---------------------------------------------------------------- forward
-template <typename T, bool SEG, bool NEAR>
-__device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type* rx, const typename Duo<T>::type* rr,
-                                                 const typename Duo<T>::type* rw, float2 nu, unsigned seg, int live,
-                                                 float2* a, float2* b, float2& A, float2& H) {
-  A = bcast2(1.0f);
-  H = bcast2(0.0f);
+template <typename T, bool SEG, bool NEAR, int K>
+__device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
+                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2 (&a)[K],
+                                                 float2 (&b)[K]) {
+  constexpr int N = 4;  // (more tokens at once take too many registers)
 #pragma unroll
-  for (int k = 0; k < kFwdK; ++k) {
-    gated_ab<T, NEAR>(Duo<T>::get(rx[k]), Duo<T>::get(rr[k]), Duo<T>::get(rw[k]), nu, a[k], b[k]);
-    if (SEG && (seg >> k & 1u)) a[k] = bcast2(-0.0f);
-    if (live < kFwdK && k >= live) a[k] = bcast2(1.0f), b[k] = bcast2(0.0f);
-    compose<SEG>(A, H, a[k], b[k]);
+  for (int k0 = 0; k0 < K; k0 += N) {
+    float2 x[N], r[N], w[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = Duo<T>::get(rx[k0 + k]), r[k] = Duo<T>::get(rr[k0 + k]), w[k] = Duo<T>::get(rw[k0 + k]);
+    gated_ab<T, NEAR>(x, r, w, nu, *reinterpret_cast<float2(*)[N]>(a + k0), *reinterpret_cast<float2(*)[N]>(b + k0));
   }
 }
 
 template <typename T, bool SEG, int MODE>
-__global__ void __launch_bounds__(kGatedWarps * 32, 3) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
+__global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BLOCKS)
+    gated_fwd_kernel(const __grid_constant__ GatedParams p) {
   using R = typename Duo<T>::type;
-  constexpr int K = kFwdK, NW = kGatedWarps, TILE = K * NW, S = kFwdStages, NT = 3;
+  using C = GatedFwdCut<T>;
+  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, S = C::STAGES, NT = 3;
   extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][stage][tensor][token][lane]
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
   __shared__ float4 s_cta[2][kGatedMaxCluster][32];       // and of each CTA of the cluster
@@ -349,143 +416,151 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 3) gated_fwd_kernel(const __
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
   const unsigned id = blockIdx.x / (unsigned)cs;
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
-  const long long steps = ((p.L + TILE - 1) / TILE + cs - 1) / cs;
-  R* stage = reinterpret_cast<R*>(s_raw) + (long long)wp * S * NT * K * 32;
-  const float2 nu = make_float2(ch < p.D ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
+  const bool on = ch < p.D;
+  const int stride = cs * TILE;  // tokens from a step to the next
+  R* stage = reinterpret_cast<R*>(s_raw) + wp * S * NT * K * 32;
+  const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
+  GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, stride);
   if (cs > 1) cluster_barrier();  // every CTA of the cluster has started before its memory is written
+  int par = 0;
 
-  GatedWalk at{id / (unsigned)p.groups, 0}, ahead = at;
-  auto next = [&](GatedWalk& w) {
-    if (++w.step == steps) w.step = 0, w.bt += p.rows;
-  };
-  GatedReader<T, MODE, K, NT> reader;
-  auto issue = [&](int slot) {  // (an empty group behind the last step, so that the groups count steps)
-    const long long t0 = (ahead.step * cs + rank) * TILE + wp * K;
-    if (ahead.step == 0) reader.start(p, ahead.bt, t0, ch0, lane);
-    reader.copy(p, stage + slot * NT * K * 32, ahead.bt < p.B ? p.L - t0 : 0, lane);
-    reader.move(p, cs * TILE);
-    next(ahead);
-  };
-  auto starts = [&](const GatedWalk& w) {
-    const long long t = (w.step * cs + rank) * TILE + wp * K + lane;
-    return __ballot_sync(0xffffffffu, SEG && lane < K && t < p.L && gated_starts(p.pos, p.pos_bytes, w.bt * p.L + t));
-  };
+  for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
+    int t0 = rank * TILE + wp * K;  // this warp's first token of the step
+    float2 carry = load_pair(p.h0, bt * p.D + ch, ch, p.D);  // the state entering the step
+    T* y = static_cast<T*>(p.y) + (bt * p.L + t0) * p.D + ch;
+    reader.start(p, bt, t0, ch0, lane);
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) issue(s);
-  int slot = 0, par = 0;
-  float2 carry = bcast2(0.0f);  // the state entering the step
-
-  for (; at.bt < p.B; next(at)) {
-    const long long t0 = (at.step * cs + rank) * TILE + wp * K;
-    const unsigned seg = SEG ? starts(at) : 0u;
-    if (at.step == 0) carry = load_pair(p.h0, at.bt * p.D + ch, ch, p.D);
-    if constexpr (MODE != kModeSingle) {
-      copy_wait<S - 2>();
-      __syncwarp();
-    }
-    float2 a[K], b[K], A, H;
-    const int live = (int)max(0LL, min((long long)K, p.L - t0));  // tokens of the sequence among these
-    {
-      const R* st = stage + slot * NT * K * 32;
-      R rx[K], rr[K], rw[K];
-      gated_read<T, MODE, K>(p, 0, st, at.bt, t0, ch, lane, rx);
-      gated_read<T, MODE, K>(p, 1, st, at.bt, t0, ch, lane, rr);
-      gated_read<T, MODE, K>(p, 2, st, at.bt, t0, ch, lane, rw);
-      if (near) gated_fwd_tokens<T, SEG, true>(rx, rr, rw, nu, seg, live, a, b, A, H);
-      else gated_fwd_tokens<T, SEG, false>(rx, rr, rw, nu, seg, live, a, b, A, H);
-    }
-    __syncwarp();  // the slot before this one has been read by every lane
-    issue(slot == 0 ? S - 1 : slot - 1);
-    slot = slot + 1 == S ? 0 : slot + 1;
-    s_map[par][wp][lane] = cat4(A, H);
-    __syncthreads();
-    float2 h;  // the state entering this CTA's tile, then this warp's tokens
-    if (cs > 1) {
-      if (wp == NW - 1) {
-        A = bcast2(1.0f), H = bcast2(0.0f);
+    for (int s = 0; s < S - 1; ++s) reader.copy(s, p.L - t0 - s * stride);
+    int slot = 0;
+    for (int first = 0; first < p.L; first += stride, t0 += stride, par ^= 1) {
+      const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
+      if constexpr (MODE != kModeSingle) {
+        copy_wait<S - 2>();
+        __syncwarp();
+      }
+      float2 a[K], b[K], A = bcast2(1.0f), H = bcast2(0.0f);
+      {
+        const R* st = stage + slot * NT * K * 32;
+        R rx[K], rr[K], rw[K];
+        gated_read<T, MODE, K>(p, 0, st, bt, t0, ch, lane, rx);
+        gated_read<T, MODE, K>(p, 1, st, bt, t0, ch, lane, rr);
+        gated_read<T, MODE, K>(p, 2, st, bt, t0, ch, lane, rw);
+        if (near) gated_fwd_tokens<T, SEG, true>(rx, rr, rw, nu, a, b);
+        else gated_fwd_tokens<T, SEG, false>(rx, rr, rw, nu, a, b);
+      }
+      const int live = p.L - t0;  // tokens of the sequence from here on
+      if (SEG && seg != 0) {
 #pragma unroll
-        for (int j = 0; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]));
-        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, H));
-        cluster_arrive_release();
+        for (int k = 0; k < K; ++k)
+          if (seg >> k & 1u) a[k] = bcast2(-0.0f);
+      }
+      if (live < K) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (k >= live) a[k] = bcast2(1.0f), b[k] = bcast2(0.0f);
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) compose<SEG>(A, H, a[k], b[k]);
+      __syncwarp();  // the slot before this one has been read by every lane
+      slot = slot == 0 ? S - 1 : slot - 1;
+      reader.copy(slot, live - (S - 1) * stride);
+      slot = slot + 2 >= S ? slot + 2 - S : slot + 2;
+      s_map[par][wp][lane] = cat4(A, H);
+      __syncthreads();
+      float2 h;  // the state entering this CTA's tile, then this warp's tokens
+      if (cs > 1) {
+        if (wp == NW - 1) {
+          A = bcast2(1.0f), H = bcast2(0.0f);
+#pragma unroll
+          for (int j = 0; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]));
+          for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, H));
+          cluster_arrive_release();
+        } else {
+          cluster_arrive_relaxed();
+        }
+        cluster_wait();
+        for (int q = 0; q < rank; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+        h = carry;
+        for (int q = rank; q < cs; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
       } else {
-        cluster_arrive_relaxed();
+        h = first == 0 ? carry : s_out[par ^ 1][lane];
       }
-      cluster_wait();
-      for (int q = 0; q < rank; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
-      h = carry;
-      for (int q = rank; q < cs; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
-    } else {
-      h = at.step == 0 ? carry : s_out[par ^ 1][lane];
+#pragma unroll
+      for (int j = 0; j < NW - 1; ++j)
+        if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
+      if (p.carry != nullptr && wp * K % kGatedChunk == 0 && live > 0)
+        store_pair(p.carry, (bt * p.chunks + t0 / kGatedChunk) * p.D + ch, ch, p.D, h);
+      if (live >= K && on) {
+        T* o = y;
+#pragma unroll
+        for (int k = 0; k < K; ++k, o += p.D) {
+          h = through<SEG>(a[k], b[k], h);
+          gated_store<T, MODE>(o, ch, p.D, h);
+        }
+      } else {
+        T* o = y;
+#pragma unroll
+        for (int k = 0; k < K; ++k, o += p.D) {
+          h = through<SEG>(a[k], b[k], h);
+          if (k < live && on) gated_store<T, MODE>(o, ch, p.D, h);
+        }
+      }
+      y += (long long)stride * p.D;
+      if (live <= K && live > 0 && p.last != nullptr) store_pair(p.last, bt * p.D + ch, ch, p.D, h);
+      if (cs == 1 && wp == NW - 1) s_out[par][lane] = h;
     }
-#pragma unroll
-    for (int j = 0; j < NW - 1; ++j)
-      if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
-    if (p.carry != nullptr && t0 % kGatedChunk == 0 && t0 < p.L)
-      store_pair(p.carry, (at.bt * p.chunks + t0 / kGatedChunk) * p.D + ch, ch, p.D, h);
-    T* y = static_cast<T*>(p.y) + (at.bt * p.L + (at.step * cs + rank) * TILE) * p.D;
-    const unsigned i0 = (unsigned)(wp * K) * (unsigned)p.D + (unsigned)ch;
-    if (live == K && ch < p.D) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        h = through<SEG>(a[k], b[k], h);
-        gated_store<T, MODE>(y, i0 + (unsigned)(k * p.D), ch, p.D, h);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        h = through<SEG>(a[k], b[k], h);
-        if (k < live && ch < p.D) gated_store<T, MODE>(y, i0 + (unsigned)(k * p.D), ch, p.D, h);
-      }
-    }
-    if (p.last != nullptr && t0 < p.L && t0 + K >= p.L) store_pair(p.last, at.bt * p.D + ch, ch, p.D, h);
-    if (cs == 1 && wp == NW - 1) s_out[par][lane] = h;
-    par ^= 1;
   }
   if constexpr (MODE != kModeSingle) copy_wait<0>();
 }
 
 // ---------------------------------------------------------------- backward
-struct GatedBwdTokens {
-  // c = a or -0; g = sqrt(1 - a^2) s(write); b = g x; bw = b (1 - s(write)); q1 = a w (w = -u >= 0);
-  // q2 = -b a^2 w / (1 - a^2); om = 1 - s(retention)
-  float2 c[kBwdK], g[kBwdK], b[kBwdK], bw[kBwdK], q1[kBwdK], q2[kBwdK], om[kBwdK];
-};
-
-template <typename T, bool SEG, bool NEAR>
-__device__ __forceinline__ void gated_bwd_tokens(const typename Duo<T>::type* rx, const typename Duo<T>::type* rr,
-                                                 const typename Duo<T>::type* rw, float2 nu, unsigned seg, int live,
-                                                 GatedBwdTokens& o, float2& A, float2& H) {
-  A = bcast2(1.0f);
-  H = bcast2(0.0f);
+// Of a thread's tokens: c = a or -0; b = g x with g = sqrt(1 - a^2) s(write); q1 = a w (w = -u >= 0);
+// q2 = -b a^2 w / (1 - a^2); and, put by in shared memory until the adjoints are there, g,
+// b (1 - s(write)) and 1 - s(retention).
+template <typename T, bool SEG, bool NEAR, int K>
+__device__ __forceinline__ void gated_bwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
+                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2* put,
+                                                 float2 (&c)[K], float2 (&b)[K], float2 (&q1)[K], float2 (&q2)[K]) {
+  constexpr int N = 4;
 #pragma unroll
-  for (int k = 0; k < kBwdK; ++k) {
-    const float2 er = exp_neg<T>(Duo<T>::get(rr[k])), ew = exp_neg<T>(Duo<T>::get(rw[k]));
-    const float2 sr = logistic_of(er), sw = logistic_of(ew), w = mul2(nu, sr);
-    float2 a, q;
-    decay<NEAR>(w, a, q);
-    const float2 m = mul2(q, add2(a, bcast2(1.0f)));
-    // (1 - a^2 = 0 only with w = 0, or w too small for float32: the products with m and w are then 0)
-    const float2 rs = make_float2(rsqrt_approx(fmaxf(m.x, 1.17549435e-38f)), rsqrt_approx(fmaxf(m.y, 1.17549435e-38f)));
-    const float2 xs = mul2(Duo<T>::get(rx[k]), sw), beta = mul2(m, rs);
-    o.g[k] = mul2(beta, sw);
-    o.b[k] = mul2(beta, xs);
-    o.bw[k] = mul2(o.b[k], one_minus_s(ew, sw));
-    o.q1[k] = mul2(a, w);
-    o.q2[k] = neg2(mul2(mul2(o.q1[k], a), mul2(xs, rs)));
-    o.om[k] = one_minus_s(er, sr);
-    o.c[k] = a;
-    if (SEG && (seg >> k & 1u)) o.c[k] = bcast2(-0.0f), o.q1[k] = bcast2(-0.0f);
-    if (live < kBwdK && k >= live) o.c[k] = bcast2(1.0f), o.b[k] = bcast2(0.0f);
-    compose<SEG>(A, H, o.c[k], o.b[k]);
+  for (int k0 = 0; k0 < K; k0 += N) {
+    float2 v[N], er[N], ew[N], sr[N], sw[N], q[N], a[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = Duo<T>::get(rr[k0 + k]);
+    exp_neg<T>(v, er);
+    logistic_of(er, sr);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = Duo<T>::get(rw[k0 + k]);
+    exp_neg<T>(v, ew);
+    logistic_of(ew, sw);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = mul2(nu, sr[k]);
+    decay<NEAR>(v, a, q);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float2 m = mul2(q[k], add2(a[k], bcast2(1.0f)));
+      // (1 - a^2 = 0 only with w = 0, or w too small for float32: the products with m and w are then 0)
+      const float2 rs = make_float2(rsqrt_approx(fmaxf(m.x, 1.17549435e-38f)), rsqrt_approx(fmaxf(m.y, 1.17549435e-38f)));
+      const float2 xs = mul2(Duo<T>::get(rx[k0 + k]), sw[k]), beta = mul2(m, rs);
+      b[k0 + k] = mul2(beta, xs);
+      put[(k0 + k) * 96] = mul2(beta, sw[k]);
+      put[(k0 + k) * 96 + 32] = mul2(b[k0 + k], one_minus_s(ew[k], sw[k]));
+      put[(k0 + k) * 96 + 64] = one_minus_s(er[k], sr[k]);
+      q1[k0 + k] = mul2(a[k], v[k]);
+      q2[k0 + k] = neg2(mul2(mul2(q1[k0 + k], a[k]), mul2(xs, rs)));
+      c[k0 + k] = a[k];
+    }
   }
 }
 
 template <typename T, bool SEG, int MODE>
-__global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
+__global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BLOCKS)
+    gated_bwd_kernel(const __grid_constant__ GatedParams p) {
   using R = typename Duo<T>::type;
-  constexpr int K = kBwdK, NW = kGatedWarps, TILE = K * NW, S = kBwdStages, NT = 4;
-  extern __shared__ __align__(16) unsigned char s_raw[];
+  using C = GatedBwdCut<T>;
+  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, S = C::STAGES, NT = 4;
+  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][token][3][lane] put by, then the stages
   __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
   __shared__ float4 s_cta[2][kGatedMaxCluster][32];  // (A, G) of each CTA of the cluster
@@ -495,135 +570,130 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
   const unsigned id = blockIdx.x / (unsigned)cs;
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
-  const long long steps = (p.chunks + cs - 1) / cs;
-  R* stage = reinterpret_cast<R*>(s_raw) + (long long)wp * S * NT * K * 32;
-  const float2 nu = make_float2(ch < p.D ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
+  const bool on = ch < p.D;
+  const int stride = cs * TILE, steps = (p.chunks + cs - 1) / cs;
+  float2* put = reinterpret_cast<float2*>(s_raw) + wp * K * 96 + lane;
+  R* stage = reinterpret_cast<R*>(s_raw + NW * K * 96 * sizeof(float2)) + wp * S * NT * K * 32;
+  const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
+  GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, -stride);
   if (cs > 1) cluster_barrier();
-
-  GatedWalk at{id / (unsigned)p.groups, steps - 1}, ahead = at;
-  auto next = [&](GatedWalk& w) {
-    if (--w.step < 0) w.step = steps - 1, w.bt += p.rows;
-  };
-  GatedReader<T, MODE, K, NT> reader;
-  auto issue = [&](int slot) {
-    const long long t0 = (ahead.step * cs + rank) * TILE + wp * K;
-    if (ahead.step == steps - 1) reader.start(p, ahead.bt, t0, ch0, lane);
-    reader.copy(p, stage + slot * NT * K * 32, ahead.bt < p.B ? p.L - t0 : 0, lane);
-    reader.move(p, -cs * TILE);
-    next(ahead);
-  };
-  auto starts = [&](const GatedWalk& w) {
-    const long long t = (w.step * cs + rank) * TILE + wp * K + lane;
-    return __ballot_sync(0xffffffffu, SEG && lane < K && t < p.L && gated_starts(p.pos, p.pos_bytes, w.bt * p.L + t));
-  };
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s) issue(s);
-  int slot = 0, par = 0;
-  float2 carry = bcast2(0.0f);  // c_{t+1} lam_{t+1} entering the step's last token
+  int par = 0;
   double dnu_x = 0.0, dnu_y = 0.0;
 
-  for (; at.bt < p.B; next(at)) {
-    const long long tile = at.step * cs + rank, t0 = tile * TILE + wp * K;
-    const unsigned seg = SEG ? starts(at) : 0u;
-    if (at.step == steps - 1) carry = load_pair(p.grad_last, at.bt * p.D + ch, ch, p.D);
-    // the state entering this CTA's tile
-    float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (at.bt * p.chunks + tile) * p.D + ch, ch, p.D);
-    if constexpr (MODE != kModeSingle) {
-      copy_wait<S - 2>();
-      __syncwarp();
-    }
-    const R* st = stage + slot * NT * K * 32;
-    const int live = (int)max(0LL, min((long long)K, p.L - t0));
-    GatedBwdTokens o;
-    float2 A, H, G = bcast2(0.0f);
-    R rd[K];
-    {
-      R rx[K], rr[K], rw[K];
-      gated_read<T, MODE, K>(p, 0, st, at.bt, t0, ch, lane, rx);
-      gated_read<T, MODE, K>(p, 1, st, at.bt, t0, ch, lane, rr);
-      gated_read<T, MODE, K>(p, 2, st, at.bt, t0, ch, lane, rw);
-      gated_read<T, MODE, K>(p, 3, st, at.bt, t0, ch, lane, rd);
+  for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
+    int tile = (steps - 1) * cs + rank, t0 = tile * TILE + wp * K;
+    float2 carry = load_pair(p.grad_last, bt * p.D + ch, ch, p.D);  // c_{t+1} lam_{t+1} entering the step's last token
+    long long at = (bt * p.L + t0) * p.D + ch;                      // of this thread's first token in the gradients
+    reader.start(p, bt, t0, ch0, lane);
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) reader.copy(s, s < steps ? p.L - t0 + s * stride : 0);
+    int slot = 0;
+    for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, par ^= 1) {
+      const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
+      // the state entering this CTA's tile
+      float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (bt * p.chunks + tile) * p.D + ch, ch, p.D);
+      if constexpr (MODE != kModeSingle) {
+        copy_wait<S - 2>();
+        __syncwarp();
+      }
+      const R* st = stage + slot * NT * K * 32;
+      const int live = p.L - t0;
+      float2 f[K], b[K], q1[K], q2[K], A = bcast2(1.0f), H = bcast2(0.0f), G = bcast2(0.0f);
+      R rd[K];
+      {
+        R rx[K], rr[K], rw[K];
+        gated_read<T, MODE, K>(p, 0, st, bt, t0, ch, lane, rx);
+        gated_read<T, MODE, K>(p, 1, st, bt, t0, ch, lane, rr);
+        gated_read<T, MODE, K>(p, 2, st, bt, t0, ch, lane, rw);
+        gated_read<T, MODE, K>(p, 3, st, bt, t0, ch, lane, rd);
+        if (near) gated_bwd_tokens<T, SEG, true>(rx, rr, rw, nu, put, f, b, q1, q2);
+        else gated_bwd_tokens<T, SEG, false>(rx, rr, rw, nu, put, f, b, q1, q2);
+      }
+      if (SEG && seg != 0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (seg >> k & 1u) f[k] = bcast2(-0.0f), q1[k] = bcast2(-0.0f);
+      }
       if (live < K) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
-          if (k >= live) rd[k] = Duo<T>::make(bcast2(0.0f));
+          if (k >= live) f[k] = bcast2(1.0f), b[k] = bcast2(0.0f), rd[k] = Duo<T>::make(bcast2(0.0f));
       }
-      if (near) gated_bwd_tokens<T, SEG, true>(rx, rr, rw, nu, seg, live, o, A, H);
-      else gated_bwd_tokens<T, SEG, false>(rx, rr, rw, nu, seg, live, o, A, H);
-    }
 #pragma unroll
-    for (int k = K - 1; k >= 0; --k) G = through0<SEG>(o.c[k], add2(Duo<T>::get(rd[k]), G));
-    __syncwarp();
-    issue(slot == 0 ? S - 1 : slot - 1);
-    slot = slot + 1 == S ? 0 : slot + 1;
-    s_map[par][wp][lane] = cat4(A, H);
-    s_adj[par][wp][lane] = G;
-    __syncthreads();
-    float2 c;  // the adjoint entering this CTA's tile, then this warp's tokens
-    if (cs > 1) {
-      if (wp == 0) {
+      for (int k = 0; k < K; ++k) compose<SEG>(A, H, f[k], b[k]);
 #pragma unroll
-        for (int j = 0, i = NW - 1; j < NW; ++j, --i) {
-          if (j == 0) A = lo2(s_map[par][i][lane]), G = s_adj[par][i][lane];
-          else compose<SEG>(A, G, lo2(s_map[par][i][lane]), s_adj[par][i][lane]);
+      for (int k = K - 1; k >= 0; --k) G = through0<SEG>(f[k], add2(Duo<T>::get(rd[k]), G));
+      __syncwarp();
+      slot = slot == 0 ? S - 1 : slot - 1;
+      reader.copy(slot, step >= S - 1 ? live + (S - 1) * stride : 0);
+      slot = slot + 2 >= S ? slot + 2 - S : slot + 2;
+      s_map[par][wp][lane] = cat4(A, H);
+      s_adj[par][wp][lane] = G;
+      __syncthreads();
+      if (cs > 1) {
+        if (wp == 0) {
+#pragma unroll
+          for (int i = NW - 1; i >= 0; --i) {
+            if (i == NW - 1) A = lo2(s_map[par][i][lane]), G = s_adj[par][i][lane];
+            else compose<SEG>(A, G, lo2(s_map[par][i][lane]), s_adj[par][i][lane]);
+          }
+          for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, G));
+          cluster_arrive_release();
+        } else {
+          cluster_arrive_relaxed();
         }
-        for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, G));
-        cluster_arrive_release();
+      }
+#pragma unroll
+      for (int j = 0; j < NW - 1; ++j)
+        if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
+      // states forward: q1 <- q1 h_{t-1} + q2 = -du u / lam
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        q1[k] = through<SEG>(q1[k], q2[k], h);
+        h = through<SEG>(f[k], b[k], h);
+      }
+      float2 c;  // the adjoint entering this CTA's tile, then this warp's tokens
+      if (cs > 1) {
+        cluster_wait();
+        for (int q = cs - 1; q > rank; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+        c = carry;
+        for (int q = rank; q >= 0; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
       } else {
-        cluster_arrive_relaxed();
+        c = step == steps - 1 ? carry : s_out[par ^ 1][lane];
+      }
+#pragma unroll
+      for (int j = NW - 1; j > 0; --j)
+        if (j > wp) c = through<SEG>(lo2(s_map[par][j][lane]), s_adj[par][j][lane], c);
+      // adjoints in reverse
+      float2 sum = bcast2(0.0f);
+      long long i = at + (long long)(K - 1) * p.D;
+      auto token = [&](int k, bool store) {
+        const float2 lam = add2(Duo<T>::get(rd[k]), c), du = mul2(neg2(lam), q1[k]);
+        c = through0<SEG>(f[k], lam);
+        if (store) {
+          gated_store<T, MODE>(static_cast<T*>(p.dx) + i, ch, p.D, mul2(lam, put[k * 96]));
+          gated_store<T, MODE>(static_cast<T*>(p.dw) + i, ch, p.D, mul2(lam, put[k * 96 + 32]));
+          gated_store<T, MODE>(static_cast<T*>(p.dr) + i, ch, p.D, mul2(du, put[k * 96 + 64]));
+          sum = add2(sum, du);
+        }
+        i -= p.D;
+      };
+      if (live >= K && on) {
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) token(k, true);
+      } else {
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) token(k, k < live && on);
+      }
+      at -= (long long)stride * p.D;
+      dnu_x += (double)sum.x;
+      dnu_y += (double)sum.y;
+      if (wp == 0) {
+        if (cs == 1) s_out[par][lane] = c;
+        if (tile == 0 && p.grad_h0 != nullptr) store_pair(p.grad_h0, bt * p.D + ch, ch, p.D, c);
       }
     }
-#pragma unroll
-    for (int j = 0; j < NW - 1; ++j)
-      if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
-    if (cs > 1) {
-      cluster_wait();
-      for (int q = cs - 1; q > rank; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
-      c = carry;
-      for (int q = rank; q >= 0; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
-    } else {
-      c = at.step == steps - 1 ? carry : s_out[par ^ 1][lane];
-    }
-#pragma unroll
-    for (int j = NW - 1; j > 0; --j)
-      if (j > wp) c = through<SEG>(lo2(s_map[par][j][lane]), s_adj[par][j][lane], c);
-    // states forward: q1 <- q1 h_{t-1} + q2 = -du u / lam
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      o.q1[k] = through<SEG>(o.q1[k], o.q2[k], h);
-      h = through<SEG>(o.c[k], o.b[k], h);
-    }
-    // adjoints in reverse
-    float2 sum = bcast2(0.0f);
-    const long long base = (at.bt * p.L + tile * TILE) * p.D;
-    T *dx = static_cast<T*>(p.dx) + base, *dr = static_cast<T*>(p.dr) + base, *dw = static_cast<T*>(p.dw) + base;
-    const unsigned i0 = (unsigned)(wp * K) * (unsigned)p.D + (unsigned)ch;
-    auto token = [&](int k, bool store) {
-      const float2 lam = add2(Duo<T>::get(rd[k]), c), du = mul2(neg2(lam), o.q1[k]);
-      c = through0<SEG>(o.c[k], lam);
-      if (store) {
-        const unsigned i = i0 + (unsigned)(k * p.D);
-        gated_store<T, MODE>(dx, i, ch, p.D, mul2(lam, o.g[k]));
-        gated_store<T, MODE>(dr, i, ch, p.D, mul2(du, o.om[k]));
-        gated_store<T, MODE>(dw, i, ch, p.D, mul2(lam, o.bw[k]));
-        sum = add2(sum, du);
-      }
-    };
-    if (live == K && ch < p.D) {
-#pragma unroll
-      for (int k = K - 1; k >= 0; --k) token(k, true);
-    } else {
-#pragma unroll
-      for (int k = K - 1; k >= 0; --k) token(k, k < live && ch < p.D);
-    }
-    dnu_x += (double)sum.x;
-    dnu_y += (double)sum.y;
-    if (wp == 0) {
-      if (cs == 1) s_out[par][lane] = c;
-      if (tile == 0 && p.grad_h0 != nullptr) store_pair(p.grad_h0, at.bt * p.D + ch, ch, p.D, c);
-    }
-    par ^= 1;
   }
   if constexpr (MODE != kModeSingle) copy_wait<0>();
   // the CTA's sum of dnu_log per channel, over its warps in order
@@ -633,24 +703,25 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) gated_bwd_kernel(const __
     double sx = 0.0, sy = 0.0;
     for (int j = 0; j < NW; ++j) sx += s_nu[j][lane].x, sy += s_nu[j][lane].y;
     double* part = p.part + ((long long)(id / (unsigned)p.groups) * cs + rank) * p.D;
-    if (ch < p.D) part[ch] = sx;
+    if (on) part[ch] = sx;
     if (ch + 1 < p.D) part[ch + 1] = sy;
   }
 }
 
 // dnu_log[d] = the sum of the partial rows, in order: a warp's lanes own 32 channels, the block's
-// warps every kGatedWarps-th row, then warp 0 adds the warps' sums.
-__global__ void __launch_bounds__(kGatedWarps * 32) gated_reduce_kernel(const double* part, float* out, int rows, int D) {
-  __shared__ double s[kGatedWarps][32];
+// warps every kReduceRows-th row, then warp 0 adds the warps' sums.
+constexpr int kReduceRows = 8;
+__global__ void __launch_bounds__(kReduceRows * 32) gated_reduce_kernel(const double* part, float* out, int rows, int D) {
+  __shared__ double s[kReduceRows][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + lane;
   double t = 0.0;
   if (d < D)
-    for (int r = wp; r < rows; r += kGatedWarps) t += part[(long long)r * D + d];
+    for (int r = wp; r < rows; r += kReduceRows) t += part[(long long)r * D + d];
   s[wp][lane] = t;
   __syncthreads();
   if (wp == 0 && d < D) {
-    for (int j = 1; j < kGatedWarps; ++j) t += s[j][lane];
+    for (int j = 1; j < kReduceRows; ++j) t += s[j][lane];
     out[d] = (float)t;
   }
 }
@@ -678,10 +749,11 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p
     const float r = Io<T>::load(static_cast<const T*>(p.r) + b * p.sr + d);
     const float w = Io<T>::load(static_cast<const T*>(p.w) + b * p.sw + d);
     const float s = p.state[b * p.D + d];
-    float2 a, c;
-    gated_ab<T, false>(bcast2(x), bcast2(r), bcast2(w), bcast2(nu), a, c);
+    const float2 x2[1] = {bcast2(x)}, r2[1] = {bcast2(r)}, w2[1] = {bcast2(w)};
+    float2 a[1], c[1];
+    gated_ab<T, false>(x2, r2, w2, bcast2(nu), a, c);
     const bool start = p.pos != nullptr && gated_starts(p.pos, p.pos_bytes, b);
-    const float h = start ? c.x : fmaf(a.x, s, c.x);
+    const float h = start ? c[0].x : fmaf(a[0].x, s, c[0].x);
     Io<T>::store(static_cast<T*>(p.y) + b * p.D + d, h);
     p.new_state[b * p.D + d] = h;
   }
@@ -711,8 +783,8 @@ static bool gated_valid_dtype(int d) { return d == SPARC_DTYPE_F32 || d == SPARC
 
 static int gated_check_shape(long long B, long long L, long long D) {
   if (B <= 0 || L <= 0 || D <= 0) return fail(SPARC_ERR_SHAPE, "batch, length and channels must be positive");
-  if (D > (1LL << 22) || B > (1LL << 31) || L > (1LL << 40) || (double)B * (double)L * (double)D > 4.0e18)
-    return fail(SPARC_ERR_SHAPE, "shape beyond the launch grid (channels <= 2^22, batch <= 2^31)");
+  if (D > (1LL << 22) || B > (1LL << 31) || L > (1LL << 30) || (double)B * (double)L * (double)D > 4.0e18)
+    return fail(SPARC_ERR_SHAPE, "shape beyond the launch grid (channels <= 2^22, length <= 2^30, batch <= 2^31)");
   return SPARC_OK;
 }
 
@@ -736,8 +808,11 @@ static GatedMode gated_mode(const GatedParams& p, int inputs, int size) {
 
 template <typename T, bool SEG, int MODE>
 static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_t s) {
-  constexpr int kRow = kGatedWarps * 32 * (int)sizeof(typename Duo<T>::type);
-  const int smem = MODE == kModeSingle ? 0 : kRow * (backward ? kBwdStages * 4 * kBwdK : kFwdStages * 3 * kFwdK);
+  constexpr int kRow = 32 * (int)sizeof(typename Duo<T>::type);
+  using F = GatedFwdCut<T>;
+  using W = GatedBwdCut<T>;
+  const int staged = MODE == kModeSingle ? 0 : backward ? W::TILE * W::STAGES * 4 * kRow : F::TILE * F::STAGES * 3 * kRow;
+  const int smem = staged + (backward ? W::TILE * 96 * (int)sizeof(float2) : 0);
   const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
   if (smem > 0) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -745,7 +820,7 @@ static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.groups * (unsigned)p.rows * (unsigned)p.cluster);
-  cfg.blockDim = dim3(kGatedWarps * 32);
+  cfg.blockDim = dim3((backward ? W::WARPS : F::WARPS) * 32);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -819,14 +894,14 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   p.pos = a->segment_pos;
   p.pos_bytes = a->segment_pos_bytes;
   p.B = a->batch;
-  p.L = a->length;
+  p.L = (int)a->length;
   p.D = (int)a->channels;
-  p.chunks = sparc_gated_carry_chunks(a->length);
+  p.chunks = (int)sparc_gated_carry_chunks(a->length);
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
   const GatedMode mode = gated_aligned(p.y, 2 * size) ? gated_mode(p, 3, size) : kModeSingle;
-  const GatedPlan pl = gated_plan(p.B, p.L, p.D, kFwdK * kGatedWarps);
+  const GatedPlan pl = gated_plan(p.B, p.L, p.D, kFwdTile);
   p.groups = pl.groups;
   p.cluster = pl.cluster;
   p.rows = pl.rows;
@@ -866,9 +941,9 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
   p.pos = a->segment_pos;
   p.pos_bytes = a->segment_pos_bytes;
   p.B = a->batch;
-  p.L = a->length;
+  p.L = (int)a->length;
   p.D = (int)a->channels;
-  p.chunks = sparc_gated_carry_chunks(a->length);
+  p.chunks = (int)sparc_gated_carry_chunks(a->length);
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const GatedIn& in : p.in)
     if (!gated_aligned(in.p, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
@@ -886,7 +961,7 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
   cudaError_t e = gated_dispatch(p, mode, a->dtype, true, s);
   if (e == cudaSuccess) {
     TimedLaunch tl(kTimeGatedReduce, s);
-    gated_reduce_kernel<<<(p.D + 31) / 32, kGatedWarps * 32, 0, s>>>(p.part, a->grad_nu_log, pl.rows * pl.cluster, p.D);
+    gated_reduce_kernel<<<(p.D + 31) / 32, kReduceRows * 32, 0, s>>>(p.part, a->grad_nu_log, pl.rows * pl.cluster, p.D);
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
