@@ -20,7 +20,8 @@
 // per kGatedChunk tokens, so that the states are not rounded to the activations' type), the
 // adjoints from the step before. The cluster size grows as rows x channels shrink. All orders are
 // fixed: results are bitwise reproducible. Each warp copies its own tokens to shared memory
-// asynchronously, kStages - 1 steps ahead, so nothing but the copies' own completion orders them.
+// asynchronously, a step ahead (into the place whose values it has just taken into registers), so
+// nothing but the copies' own completion orders them.
 //
 // A segment start drops what came before it, infinities and NaN included: its factor is kept as
 // -0 (a_t >= +0, so the sign marks it through products), and composing with it selects instead of
@@ -36,18 +37,17 @@ namespace sparc {
 constexpr int kGatedChunk = 32;  // tokens per saved carry
 constexpr int kGatedMaxCluster = 8;
 
-// How a CTA cuts its tile: WARPS spans of K tokens, STAGES steps of inputs in shared memory, BLOCKS
-// CTAs per SM that the registers are held to.
-template <int K_, int WARPS_, int STAGES_, int BLOCKS_>
+// How a CTA cuts its tile: WARPS spans of K tokens; BLOCKS CTAs per SM that the registers are held to.
+template <int K_, int WARPS_, int BLOCKS_>
 struct GatedCut {
-  static constexpr int K = K_, WARPS = WARPS_, STAGES = STAGES_, BLOCKS = BLOCKS_, TILE = K * WARPS;
+  static constexpr int K = K_, WARPS = WARPS_, BLOCKS = BLOCKS_, TILE = K * WARPS;
 };
 template <typename T> struct GatedFwdCut;
-template <> struct GatedFwdCut<__nv_bfloat16> : GatedCut<16, 4, 2, 4> {};
-template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2, 2> {};
+template <> struct GatedFwdCut<__nv_bfloat16> : GatedCut<16, 4, 4> {};
+template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2> {};
 template <typename T> struct GatedBwdCut;
-template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 2, 3> {};
-template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2, 2> {};
+template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 3> {};
+template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2> {};
 constexpr int kFwdTile = 64;  // of either type, so that the plans are
 static_assert(GatedFwdCut<float>::TILE == kFwdTile && GatedFwdCut<__nv_bfloat16>::TILE == kFwdTile);
 // the backward's tile is one chunk
@@ -123,11 +123,7 @@ __device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A warp's reads of its next tokens: K of them a step, of NT tensors, into stage[tensor][token][lane].
 // Each lane owns pieces kRows tokens apart, and keeps a pointer per tensor that moves by a constant
@@ -163,17 +159,16 @@ struct GatedReader {
       src[n] = reinterpret_cast<const char*>(static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb +
                                              (long long)(t0 + lane / kPieces) * p.in[n].st + chan);
   }
-  // `left`: tokens of the sequence from this step's first on (none: an empty group, so that the groups count steps)
-  __device__ __forceinline__ void copy(int slot, int left) {
+  // `left`: tokens of the sequence from this step's first on
+  __device__ __forceinline__ void copy(int left) {
     if constexpr (MODE == kModeSingle) return;
-    const unsigned to = dst + slot * (NT * K * 32 * (int)sizeof(R));
     if (left >= K) {
       if (token < K) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < K / kRows; ++i)
-            copy_async<kBytes>(to + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
+            copy_async<kBytes>(dst + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
       }
     } else {
 #pragma unroll
@@ -181,9 +176,8 @@ struct GatedReader {
 #pragma unroll
         for (int i = 0; i < K / kRows; ++i)
           if (token < K && token + i * kRows < left)
-            copy_async<kBytes>(to + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
+            copy_async<kBytes>(dst + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
     }
-    copy_commit();
 #pragma unroll
     for (int n = 0; n < NT; ++n) src[n] += move[n];
   }
@@ -407,8 +401,8 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
     gated_fwd_kernel(const __grid_constant__ GatedParams p) {
   using R = typename Duo<T>::type;
   using C = GatedFwdCut<T>;
-  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, S = C::STAGES, NT = 3;
-  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][stage][tensor][token][lane]
+  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 3;
+  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][tensor][token][lane]
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
   __shared__ float4 s_cta[2][kGatedMaxCluster][32];       // and of each CTA of the cluster
   __shared__ float2 s_out[2][32];                         // one CTA: the state leaving its tile
@@ -418,7 +412,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
   const bool on = ch < p.D;
   const int stride = cs * TILE;  // tokens from a step to the next
-  R* stage = reinterpret_cast<R*>(s_raw) + wp * S * NT * K * 32;
+  R* stage = reinterpret_cast<R*>(s_raw) + wp * NT * K * 32;
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, stride);
@@ -430,26 +424,25 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
     float2 carry = load_pair(p.h0, bt * p.D + ch, ch, p.D);  // the state entering the step
     T* y = static_cast<T*>(p.y) + (bt * p.L + t0) * p.D + ch;
     reader.start(p, bt, t0, ch0, lane);
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) reader.copy(s, p.L - t0 - s * stride);
-    int slot = 0;
+    reader.copy(p.L - t0);
     for (int first = 0; first < p.L; first += stride, t0 += stride, par ^= 1) {
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
       if constexpr (MODE != kModeSingle) {
-        copy_wait<S - 2>();
+        copy_wait();
         __syncwarp();
       }
       float2 a[K], b[K], A = bcast2(1.0f), H = bcast2(0.0f);
+      const int live = p.L - t0;  // tokens of the sequence from here on
       {
-        const R* st = stage + slot * NT * K * 32;
         R rx[K], rr[K], rw[K];
-        gated_read<T, MODE, K>(p, 0, st, bt, t0, ch, lane, rx);
-        gated_read<T, MODE, K>(p, 1, st, bt, t0, ch, lane, rr);
-        gated_read<T, MODE, K>(p, 2, st, bt, t0, ch, lane, rw);
+        gated_read<T, MODE, K>(p, 0, stage, bt, t0, ch, lane, rx);
+        gated_read<T, MODE, K>(p, 1, stage, bt, t0, ch, lane, rr);
+        gated_read<T, MODE, K>(p, 2, stage, bt, t0, ch, lane, rw);
+        __syncwarp();  // every lane has read its values
+        reader.copy(live - stride);
         if (near) gated_fwd_tokens<T, SEG, true>(rx, rr, rw, nu, a, b);
         else gated_fwd_tokens<T, SEG, false>(rx, rr, rw, nu, a, b);
       }
-      const int live = p.L - t0;  // tokens of the sequence from here on
       if (SEG && seg != 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -462,10 +455,6 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) compose<SEG>(A, H, a[k], b[k]);
-      __syncwarp();  // the slot before this one has been read by every lane
-      slot = slot == 0 ? S - 1 : slot - 1;
-      reader.copy(slot, live - (S - 1) * stride);
-      slot = slot + 2 >= S ? slot + 2 - S : slot + 2;
       s_map[par][wp][lane] = cat4(A, H);
       __syncthreads();
       float2 h;  // the state entering this CTA's tile, then this warp's tokens
@@ -511,7 +500,6 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
       if (cs == 1 && wp == NW - 1) s_out[par][lane] = h;
     }
   }
-  if constexpr (MODE != kModeSingle) copy_wait<0>();
 }
 
 // ---------------------------------------------------------------- backward
@@ -559,8 +547,8 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     gated_bwd_kernel(const __grid_constant__ GatedParams p) {
   using R = typename Duo<T>::type;
   using C = GatedBwdCut<T>;
-  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, S = C::STAGES, NT = 4;
-  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][token][3][lane] put by, then the stages
+  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 4;
+  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][token][3][lane] put by, then the inputs
   __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
   __shared__ float4 s_cta[2][kGatedMaxCluster][32];  // (A, G) of each CTA of the cluster
@@ -573,7 +561,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const bool on = ch < p.D;
   const int stride = cs * TILE, steps = (p.chunks + cs - 1) / cs;
   float2* put = reinterpret_cast<float2*>(s_raw) + wp * K * 96 + lane;
-  R* stage = reinterpret_cast<R*>(s_raw + NW * K * 96 * sizeof(float2)) + wp * S * NT * K * 32;
+  R* stage = reinterpret_cast<R*>(s_raw + NW * K * 96 * sizeof(float2)) + wp * NT * K * 32;
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, -stride);
@@ -586,27 +574,26 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     float2 carry = load_pair(p.grad_last, bt * p.D + ch, ch, p.D);  // c_{t+1} lam_{t+1} entering the step's last token
     long long at = (bt * p.L + t0) * p.D + ch;                      // of this thread's first token in the gradients
     reader.start(p, bt, t0, ch0, lane);
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) reader.copy(s, s < steps ? p.L - t0 + s * stride : 0);
-    int slot = 0;
+    reader.copy(p.L - t0);
     for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, par ^= 1) {
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
       // the state entering this CTA's tile
       float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (bt * p.chunks + tile) * p.D + ch, ch, p.D);
       if constexpr (MODE != kModeSingle) {
-        copy_wait<S - 2>();
+        copy_wait();
         __syncwarp();
       }
-      const R* st = stage + slot * NT * K * 32;
       const int live = p.L - t0;
       float2 f[K], b[K], q1[K], q2[K], A = bcast2(1.0f), H = bcast2(0.0f), G = bcast2(0.0f);
       R rd[K];
       {
         R rx[K], rr[K], rw[K];
-        gated_read<T, MODE, K>(p, 0, st, bt, t0, ch, lane, rx);
-        gated_read<T, MODE, K>(p, 1, st, bt, t0, ch, lane, rr);
-        gated_read<T, MODE, K>(p, 2, st, bt, t0, ch, lane, rw);
-        gated_read<T, MODE, K>(p, 3, st, bt, t0, ch, lane, rd);
+        gated_read<T, MODE, K>(p, 0, stage, bt, t0, ch, lane, rx);
+        gated_read<T, MODE, K>(p, 1, stage, bt, t0, ch, lane, rr);
+        gated_read<T, MODE, K>(p, 2, stage, bt, t0, ch, lane, rw);
+        gated_read<T, MODE, K>(p, 3, stage, bt, t0, ch, lane, rd);
+        __syncwarp();
+        reader.copy(step > 0 ? live + stride : 0);
         if (near) gated_bwd_tokens<T, SEG, true>(rx, rr, rw, nu, put, f, b, q1, q2);
         else gated_bwd_tokens<T, SEG, false>(rx, rr, rw, nu, put, f, b, q1, q2);
       }
@@ -624,10 +611,6 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       for (int k = 0; k < K; ++k) compose<SEG>(A, H, f[k], b[k]);
 #pragma unroll
       for (int k = K - 1; k >= 0; --k) G = through0<SEG>(f[k], add2(Duo<T>::get(rd[k]), G));
-      __syncwarp();
-      slot = slot == 0 ? S - 1 : slot - 1;
-      reader.copy(slot, step >= S - 1 ? live + (S - 1) * stride : 0);
-      slot = slot + 2 >= S ? slot + 2 - S : slot + 2;
       s_map[par][wp][lane] = cat4(A, H);
       s_adj[par][wp][lane] = G;
       __syncthreads();
@@ -695,7 +678,6 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       }
     }
   }
-  if constexpr (MODE != kModeSingle) copy_wait<0>();
   // the CTA's sum of dnu_log per channel, over its warps in order
   s_nu[wp][lane] = make_double2(dnu_x, dnu_y);
   __syncthreads();
@@ -811,7 +793,7 @@ static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_
   constexpr int kRow = 32 * (int)sizeof(typename Duo<T>::type);
   using F = GatedFwdCut<T>;
   using W = GatedBwdCut<T>;
-  const int staged = MODE == kModeSingle ? 0 : backward ? W::TILE * W::STAGES * 4 * kRow : F::TILE * F::STAGES * 3 * kRow;
+  const int staged = MODE == kModeSingle ? 0 : backward ? W::TILE * 4 * kRow : F::TILE * 3 * kRow;
   const int smem = staged + (backward ? W::TILE * 96 * (int)sizeof(float2) : 0);
   const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
   if (smem > 0) {
