@@ -413,6 +413,9 @@ typedef struct SparcGatedFwdArgs {
   long long length;
   long long channels;
   int dtype;
+  unsigned max_spin;                   /* bound of the waits within a cluster (0 = default) */
+  unsigned* status;                    /* device word, or'ed with SPARC_STATUS_TIMEOUT if such a
+                                          wait ran out (the launch still completes), or NULL */
 } SparcGatedFwdArgs;
 
 typedef struct SparcGatedBwdArgs {
@@ -444,6 +447,8 @@ typedef struct SparcGatedBwdArgs {
   long long length;
   long long channels;
   int dtype;
+  unsigned max_spin;
+  unsigned* status;
 } SparcGatedBwdArgs;
 
 /* One token of it: x and the gates [batch, channels] (dtype, row strides in elements), state

@@ -14,8 +14,8 @@
 // own consecutive spans of K tokens (a tile), and a thread-block cluster's CTAs consecutive tiles;
 // the cluster walks the sequence. A thread turns its K tokens into an affine map (A, H): h_out =
 // A h_in + H in registers; after one barrier every warp runs the state through the maps of the
-// warps before it (and, over distributed shared memory and one cluster barrier, through those of
-// the cluster's CTAs before its own), and replays its tokens from there. The backward does
+// warps before it (and, over distributed shared memory, through those of the cluster's CTAs before
+// its own), and replays its tokens from there. The backward does
 // both directions in one step: the states from the forward's saved chunk carries (float32, one
 // per kGatedChunk tokens, so that the states are not rounded to the activations' type), the
 // adjoints from the step before. The cluster size grows as rows x channels shrink. All orders are
@@ -36,6 +36,7 @@ namespace sparc {
 
 constexpr int kGatedChunk = 32;  // tokens per saved carry
 constexpr int kGatedMaxCluster = 8;
+constexpr unsigned kGatedSpin = 1u << 22;  // default bound of a wait's polls (each may sleep in hardware)
 
 // How a CTA cuts its tile: WARPS spans of K tokens; BLOCKS CTAs per SM that the registers are held to.
 template <int K_, int WARPS_, int BLOCKS_>
@@ -74,6 +75,8 @@ struct GatedParams {
   long long B;
   int L, chunks;
   int D, groups, cluster, rows;  // rows: clusters per channel group, each walking rows of the batch
+  unsigned max_spin;             // polls of a wait for the cluster's maps
+  unsigned* status;              // or'ed with kStatusTimeout where one ran out, or null
 };
 
 // ---------------------------------------------------------------- two adjacent channels
@@ -356,22 +359,40 @@ __device__ __forceinline__ float2 through0(float2 A, float2 lam) {
   return make_float2(dropped(A.x) ? 0.0f : o.x, dropped(A.y) ? 0.0f : o.y);
 }
 
-__device__ __forceinline__ void st_cluster(unsigned addr, float4 v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-               : "memory");
-}
 __device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float4 cat4(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
 
-// The cluster's exchange, one hardware barrier per step: only the warp that stored to its peers
-// releases, every warp acquires.
-__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_barrier() {
-  cluster_arrive_release();
-  cluster_wait();
+// The cluster's exchange, once a step: a warp of every CTA pushes the CTA's map to every CTA by
+// asynchronous stores that count down the receiver's mbarrier, and every warp waits for its own
+// CTA's. (A cluster barrier that releases the maps would wait for the warp's outputs on their way
+// to global memory too.) Buffers and barriers are of two parities: a CTA pushes step n + 2 after it
+// has step n + 1 from every CTA, which each pushed once all its warps were through with step n.
+struct GatedExchange {
+  float4 map[2][kGatedMaxCluster][32];
+  unsigned long long bar[2];
+};
+
+__device__ __forceinline__ void exchange_init(GatedExchange& x) {
+  if (threadIdx.x == 0) {
+    mbar_init(&x.bar[0], 1);
+    mbar_init(&x.bar[1], 1);
+    mbar_init_fence();
+  }
+  // every CTA of the cluster has started, and its barriers stand, before anything is pushed
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void exchange_push(GatedExchange& x, unsigned n, int cs, int rank, int lane, float4 v) {
+  const int par = n & 1;
+  if (lane == 0) mbar_arrive_expect_tx(&x.bar[par], (unsigned)cs * 32u * 16u);
+  for (int q = 0; q < cs; ++q)
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                     cluster_smem_addr(&x.map[par][rank][lane], q)),
+                 "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(cluster_smem_addr(&x.bar[par], q))
+                 : "memory");
+}
+__device__ __forceinline__ void exchange_wait(const GatedParams& p, GatedExchange& x, unsigned n) {
+  if (!mbar_wait_cluster(&x.bar[n & 1], n >> 1 & 1u, p.max_spin) && p.status != nullptr) atomicOr(p.status, kStatusTimeout);
 }
 
 // Which of a warp's K tokens from t0 on start a segment, as bits.
@@ -404,7 +425,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 3;
   extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][tensor][token][lane]
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
-  __shared__ float4 s_cta[2][kGatedMaxCluster][32];       // and of each CTA of the cluster
+  __shared__ GatedExchange s_cta;                         // and of each CTA of the cluster
   __shared__ float2 s_out[2][32];                         // one CTA: the state leaving its tile
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
@@ -416,8 +437,8 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, stride);
-  if (cs > 1) cluster_barrier();  // every CTA of the cluster has started before its memory is written
-  int par = 0;
+  if (cs > 1) exchange_init(s_cta);
+  unsigned n = 0;  // steps so far
 
   for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
     int t0 = rank * TILE + wp * K;  // this warp's first token of the step
@@ -425,7 +446,8 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
     T* y = static_cast<T*>(p.y) + (bt * p.L + t0) * p.D + ch;
     reader.start(p, bt, t0, ch0, lane);
     reader.copy(p.L - t0);
-    for (int first = 0; first < p.L; first += stride, t0 += stride, par ^= 1) {
+    for (int first = 0; first < p.L; first += stride, t0 += stride, ++n) {
+      const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
       if constexpr (MODE != kModeSingle) {
         copy_wait();
@@ -463,15 +485,12 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
           A = bcast2(1.0f), H = bcast2(0.0f);
 #pragma unroll
           for (int j = 0; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]));
-          for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, H));
-          cluster_arrive_release();
-        } else {
-          cluster_arrive_relaxed();
+          exchange_push(s_cta, n, cs, rank, lane, cat4(A, H));
         }
-        cluster_wait();
-        for (int q = 0; q < rank; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+        exchange_wait(p, s_cta, n);
+        for (int q = 0; q < rank; ++q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
         h = carry;
-        for (int q = rank; q < cs; ++q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+        for (int q = rank; q < cs; ++q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
       } else {
         h = first == 0 ? carry : s_out[par ^ 1][lane];
       }
@@ -500,6 +519,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
       if (cs == 1 && wp == NW - 1) s_out[par][lane] = h;
     }
   }
+  if (cs > 1) cluster_sync_relaxed();  // no CTA leaves while a peer may still push to it
 }
 
 // ---------------------------------------------------------------- backward
@@ -551,7 +571,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][token][3][lane] put by, then the inputs
   __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
-  __shared__ float4 s_cta[2][kGatedMaxCluster][32];  // (A, G) of each CTA of the cluster
+  __shared__ GatedExchange s_cta;                    // (A, G) of each CTA of the cluster
   __shared__ float2 s_out[2][32];                    // one CTA: the adjoint leaving its tile
   __shared__ double2 s_nu[NW][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
@@ -565,8 +585,8 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, -stride);
-  if (cs > 1) cluster_barrier();
-  int par = 0;
+  if (cs > 1) exchange_init(s_cta);
+  unsigned n = 0;  // steps so far
   double dnu_x = 0.0, dnu_y = 0.0;
 
   for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
@@ -575,7 +595,8 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     long long at = (bt * p.L + t0) * p.D + ch;                      // of this thread's first token in the gradients
     reader.start(p, bt, t0, ch0, lane);
     reader.copy(p.L - t0);
-    for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, par ^= 1) {
+    for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, ++n) {
+      const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
       // the state entering this CTA's tile
       float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (bt * p.chunks + tile) * p.D + ch, ch, p.D);
@@ -621,10 +642,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
             if (i == NW - 1) A = lo2(s_map[par][i][lane]), G = s_adj[par][i][lane];
             else compose<SEG>(A, G, lo2(s_map[par][i][lane]), s_adj[par][i][lane]);
           }
-          for (int q = 0; q < cs; ++q) st_cluster(cluster_smem_addr(&s_cta[par][rank][lane], q), cat4(A, G));
-          cluster_arrive_release();
-        } else {
-          cluster_arrive_relaxed();
+          exchange_push(s_cta, n, cs, rank, lane, cat4(A, G));
         }
       }
 #pragma unroll
@@ -638,10 +656,10 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       }
       float2 c;  // the adjoint entering this CTA's tile, then this warp's tokens
       if (cs > 1) {
-        cluster_wait();
-        for (int q = cs - 1; q > rank; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+        exchange_wait(p, s_cta, n);
+        for (int q = cs - 1; q > rank; --q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
         c = carry;
-        for (int q = rank; q >= 0; --q) carry = through<SEG>(lo2(s_cta[par][q][lane]), hi2(s_cta[par][q][lane]), carry);
+        for (int q = rank; q >= 0; --q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
       } else {
         c = step == steps - 1 ? carry : s_out[par ^ 1][lane];
       }
@@ -678,6 +696,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       }
     }
   }
+  if (cs > 1) cluster_sync_relaxed();
   // the CTA's sum of dnu_log per channel, over its warps in order
   s_nu[wp][lane] = make_double2(dnu_x, dnu_y);
   __syncthreads();
@@ -879,6 +898,8 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   p.L = (int)a->length;
   p.D = (int)a->channels;
   p.chunks = (int)sparc_gated_carry_chunks(a->length);
+  p.max_spin = a->max_spin != 0 ? a->max_spin : kGatedSpin;
+  p.status = a->status;
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
@@ -926,6 +947,8 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
   p.L = (int)a->length;
   p.D = (int)a->channels;
   p.chunks = (int)sparc_gated_carry_chunks(a->length);
+  p.max_spin = a->max_spin != 0 ? a->max_spin : kGatedSpin;
+  p.status = a->status;
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const GatedIn& in : p.in)
     if (!gated_aligned(in.p, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
