@@ -49,8 +49,6 @@ template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2> {};
 template <typename T> struct GatedBwdCut;
 template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 3> {};
 template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2> {};
-constexpr int kFwdTile = 64;  // of either type, so that the plans are
-static_assert(GatedFwdCut<float>::TILE == kFwdTile && GatedFwdCut<__nv_bfloat16>::TILE == kFwdTile);
 // the backward's tile is one chunk
 static_assert(GatedBwdCut<float>::TILE == kGatedChunk && GatedBwdCut<__nv_bfloat16>::TILE == kGatedChunk);
 
@@ -311,27 +309,110 @@ __device__ __forceinline__ void decay(const float2 (&w)[N], float2 (&a)[N], floa
 // nu of a channel, held finite so that nu s(retention) never meets 0 x infinity.
 __device__ __forceinline__ float gated_nu(float nu_log) { return min_nan(expf(nu_log), 3.402823466e38f); }
 
-template <typename T, bool NEAR, int N>
-__device__ __forceinline__ void gated_ab(const float2 (&x)[N], const float2 (&r)[N], const float2 (&w)[N], float2 nu,
-                                         float2 (&a)[N], float2 (&b)[N]) {
-  float2 e[N], q[N], sw[N];
-  exp_neg<T>(r, e);
-  logistic_of(e, q);
-  exp_neg<T>(w, e);
-  logistic_of(e, sw);
-#pragma unroll
-  for (int k = 0; k < N; ++k) e[k] = mul2(nu, q[k]);
-  decay<NEAR>(e, a, q);
-#pragma unroll
-  for (int k = 0; k < N; ++k) q[k] = mul2(q[k], add2(a[k], bcast2(1.0f)));
-#pragma unroll
-  for (int k = 0; k < N; ++k) b[k] = mul2(mul2(sqrt_2(q[k]), sw[k]), x[k]);
-}
-
 // 1 - s(v) = e^{-v} s(v) without cancellation, given e = e^{-v} (which may be infinite).
 __device__ __forceinline__ float2 one_minus_s(float2 e, float2 s) {
   const float2 p = mul2(e, s);
   return make_float2(e.x > 8.5070592e37f ? 1.0f : p.x, e.y > 8.5070592e37f ? 1.0f : p.y);
+}
+
+template <int DEG, int N>
+__device__ __forceinline__ void polynomial(const float (&c)[DEG + 1], const float2 (&x)[N], float2 (&y)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) y[k] = fma2(bcast2(c[DEG]), x[k], bcast2(c[DEG - 1]));
+#pragma unroll
+  for (int i = DEG - 2; i >= 0; --i)
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] = fma2(y[k], x[k], bcast2(c[i]));
+}
+
+// What N tokens' gates give: a, beta = sqrt(1 - a^2), sw = s(write), and for the backward u = log a,
+// kappa = -u a^2 / (1 - a^2), and 1 - s of the gates.
+//
+// In the bfloat16 kernels the special functions' units would bound the forward (five of their
+// operations a channel and token take 16 a clock and SM: as long as the bytes), so with nu <= 1/2
+// throughout the warp one of them goes: from rho = (1 + e^{-retention})^(-1/2) follow s(retention) =
+// rho^2 and beta = sqrt(nu) rho S(w), w = nu rho^2 = -u, where S(w) = sqrt((1 - e^{-2w}) / w) is smooth. S,
+// (1 - e^{-w}) / w and w / (e^{2w} - 1) are interpolated on [0, 1/2] by polynomials through the
+// Chebyshev points (relative errors 3e-9, 2e-9 and 2e-8).
+template <bool BWD, int N>
+struct GatedGates {
+  float2 a[N], beta[N], sw[N], u[BWD ? N : 1], kappa[BWD ? N : 1], om_r[BWD ? N : 1], om_w[BWD ? N : 1];
+};
+template <typename T, bool NEAR, bool BWD, int N>
+__device__ __forceinline__ void gated_gates(const float2 (&r)[N], const float2 (&w)[N], float2 nu, float2 root_nu,
+                                            GatedGates<BWD, N>& o) {
+  float2 e[N], u[N];
+  if constexpr (NEAR && sizeof(T) == 2) {
+    constexpr float kDecay[6] = {1.0f, -0.499999819f, 0.166662419f, -0.0416300728f, 0.00818961363f, -0.00112340422f};
+    constexpr float kRoot[6] = {1.41421356f, -0.707106332f, 0.294617291f, -0.0882973305f, 0.0190368337f, -0.00264261144f};
+    float2 rho[N], y[N], v[N];
+    exp_neg<T>(r, e);
+#pragma unroll
+    for (int k = 0; k < N; ++k) rho[k] = add2(e[k], bcast2(1.0f));
+#pragma unroll
+    for (int k = 0; k < N; ++k) rho[k] = make_float2(rsqrt_approx(rho[k].x), rsqrt_approx(rho[k].y));
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] = mul2(rho[k], rho[k]);
+    if constexpr (BWD) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) o.om_r[k] = one_minus_s(e[k], y[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = mul2(nu, y[k]), u[k] = mul2(make_float2(-nu.x, -nu.y), y[k]);
+    polynomial<5>(kDecay, v, y);
+#pragma unroll
+    for (int k = 0; k < N; ++k) o.a[k] = fma2(u[k], y[k], bcast2(1.0f));
+    polynomial<5>(kRoot, v, y);
+#pragma unroll
+    for (int k = 0; k < N; ++k) o.beta[k] = mul2(y[k], mul2(rho[k], root_nu));
+    if constexpr (BWD) {
+      constexpr float kRatio[6] = {0.499999993f, -0.499998992f, 0.166643005f, 0.000204218905f, -0.0119145593f, 0.00147940113f};
+      polynomial<5>(kRatio, v, o.kappa);
+#pragma unroll
+      for (int k = 0; k < N; ++k) o.u[k] = u[k];
+    }
+  } else {
+    float2 s[N], q[N];
+    exp_neg<T>(r, e);
+    logistic_of(e, s);
+    if constexpr (BWD) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) o.om_r[k] = one_minus_s(e[k], s[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) u[k] = mul2(nu, s[k]);
+    decay<NEAR>(u, o.a, q);
+#pragma unroll
+    for (int k = 0; k < N; ++k) q[k] = mul2(q[k], add2(o.a[k], bcast2(1.0f)));  // 1 - a^2
+    if constexpr (BWD) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        // (1 - a^2 = 0 only with u = 0, or u too small for float32: the products with it and u are then 0)
+        const float2 rs = make_float2(rsqrt_approx(fmaxf(q[k].x, 1.17549435e-38f)), rsqrt_approx(fmaxf(q[k].y, 1.17549435e-38f)));
+        o.beta[k] = mul2(q[k], rs);
+        o.kappa[k] = mul2(mul2(mul2(mul2(u[k], o.a[k]), o.a[k]), rs), rs);
+        o.u[k] = make_float2(-u[k].x, -u[k].y);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) o.beta[k] = sqrt_2(q[k]);
+    }
+  }
+  exp_neg<T>(w, e);
+  logistic_of(e, o.sw);
+  if constexpr (BWD) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) o.om_w[k] = one_minus_s(e[k], o.sw[k]);
+  }
+}
+
+template <typename T, bool NEAR, int N>
+__device__ __forceinline__ void gated_ab(const float2 (&x)[N], const float2 (&r)[N], const float2 (&w)[N], float2 nu,
+                                         float2 root_nu, float2 (&a)[N], float2 (&b)[N]) {
+  GatedGates<false, N> g;
+  gated_gates<T, NEAR, false, N>(r, w, nu, root_nu, g);
+#pragma unroll
+  for (int k = 0; k < N; ++k) a[k] = g.a[k], b[k] = mul2(mul2(g.beta[k], g.sw[k]), x[k]);
 }
 
 // ---------------------------------------------------------------- affine maps
@@ -391,6 +472,16 @@ __device__ __forceinline__ void exchange_push(GatedExchange& x, unsigned n, int 
                  "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(cluster_smem_addr(&x.bar[par], q))
                  : "memory");
 }
+// v through the maps of CTAs q0, q0 + d, ... up to before q1; they are read two ahead of their use
+template <bool SEG>
+__device__ __forceinline__ float2 exchange_through(const GatedExchange& x, int par, int q0, int q1, int d, int lane, float2 v) {
+  for (; q0 != q1 && q0 + d != q1; q0 += 2 * d) {
+    const float4 m = x.map[par][q0][lane], n = x.map[par][q0 + d][lane];
+    v = through<SEG>(lo2(n), hi2(n), through<SEG>(lo2(m), hi2(m), v));
+  }
+  if (q0 != q1) v = through<SEG>(lo2(x.map[par][q0][lane]), hi2(x.map[par][q0][lane]), v);
+  return v;
+}
 __device__ __forceinline__ void exchange_wait(const GatedParams& p, GatedExchange& x, unsigned n) {
   if (!mbar_wait_cluster(&x.bar[n & 1], n >> 1 & 1u, p.max_spin) && p.status != nullptr) atomicOr(p.status, kStatusTimeout);
 }
@@ -403,17 +494,17 @@ __device__ __forceinline__ unsigned gated_segments(const GatedParams& p, long lo
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, bool SEG, bool NEAR, int K>
+template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
-                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2 (&a)[K],
-                                                 float2 (&b)[K]) {
+                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu,
+                                                 float2 (&a)[K], float2 (&b)[K]) {
   constexpr int N = 4;  // (more tokens at once take too many registers)
 #pragma unroll
   for (int k0 = 0; k0 < K; k0 += N) {
     float2 x[N], r[N], w[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) x[k] = Duo<T>::get(rx[k0 + k]), r[k] = Duo<T>::get(rr[k0 + k]), w[k] = Duo<T>::get(rw[k0 + k]);
-    gated_ab<T, NEAR>(x, r, w, nu, *reinterpret_cast<float2(*)[N]>(a + k0), *reinterpret_cast<float2(*)[N]>(b + k0));
+    gated_ab<T, NEAR>(x, r, w, nu, root_nu, *reinterpret_cast<float2(*)[N]>(a + k0), *reinterpret_cast<float2(*)[N]>(b + k0));
   }
 }
 
@@ -435,6 +526,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const int stride = cs * TILE;  // tokens from a step to the next
   R* stage = reinterpret_cast<R*>(s_raw) + wp * NT * K * 32;
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
+  const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, stride);
   if (cs > 1) exchange_init(s_cta);
@@ -443,7 +535,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
     int t0 = rank * TILE + wp * K;  // this warp's first token of the step
     float2 carry = load_pair(p.h0, bt * p.D + ch, ch, p.D);  // the state entering the step
-    T* y = static_cast<T*>(p.y) + (bt * p.L + t0) * p.D + ch;
+    T* y = static_cast<T*>(p.y) + (bt * p.L + rank * TILE) * p.D;  // of the CTA's first token and channel
     reader.start(p, bt, t0, ch0, lane);
     reader.copy(p.L - t0);
     for (int first = 0; first < p.L; first += stride, t0 += stride, ++n) {
@@ -462,8 +554,8 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
         gated_read<T, MODE, K>(p, 2, stage, bt, t0, ch, lane, rw);
         __syncwarp();  // every lane has read its values
         reader.copy(live - stride);
-        if (near) gated_fwd_tokens<T, SEG, true>(rx, rr, rw, nu, a, b);
-        else gated_fwd_tokens<T, SEG, false>(rx, rr, rw, nu, a, b);
+        if (near) gated_fwd_tokens<T, true>(rx, rr, rw, nu, root_nu, a, b);
+        else gated_fwd_tokens<T, false>(rx, rr, rw, nu, root_nu, a, b);
       }
       if (SEG && seg != 0) {
 #pragma unroll
@@ -488,9 +580,8 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
           exchange_push(s_cta, n, cs, rank, lane, cat4(A, H));
         }
         exchange_wait(p, s_cta, n);
-        for (int q = 0; q < rank; ++q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
-        h = carry;
-        for (int q = rank; q < cs; ++q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
+        h = exchange_through<SEG>(s_cta, par, 0, rank, 1, lane, carry);
+        carry = exchange_through<SEG>(s_cta, par, rank, cs, 1, lane, h);
       } else {
         h = first == 0 ? carry : s_out[par ^ 1][lane];
       }
@@ -499,19 +590,18 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
         if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
       if (p.carry != nullptr && wp * K % kGatedChunk == 0 && live > 0)
         store_pair(p.carry, (bt * p.chunks + t0 / kGatedChunk) * p.D + ch, ch, p.D, h);
+      unsigned i = (unsigned)(wp * K) * (unsigned)p.D + (unsigned)ch;
       if (live >= K && on) {
-        T* o = y;
 #pragma unroll
-        for (int k = 0; k < K; ++k, o += p.D) {
+        for (int k = 0; k < K; ++k, i += (unsigned)p.D) {
           h = through<SEG>(a[k], b[k], h);
-          gated_store<T, MODE>(o, ch, p.D, h);
+          gated_store<T, MODE>(y + i, ch, p.D, h);
         }
       } else {
-        T* o = y;
 #pragma unroll
-        for (int k = 0; k < K; ++k, o += p.D) {
+        for (int k = 0; k < K; ++k, i += (unsigned)p.D) {
           h = through<SEG>(a[k], b[k], h);
-          if (k < live && on) gated_store<T, MODE>(o, ch, p.D, h);
+          if (k < live && on) gated_store<T, MODE>(y + i, ch, p.D, h);
         }
       }
       y += (long long)stride * p.D;
@@ -523,41 +613,31 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
 }
 
 // ---------------------------------------------------------------- backward
-// Of a thread's tokens: c = a or -0; b = g x with g = sqrt(1 - a^2) s(write); q1 = a w (w = -u >= 0);
-// q2 = -b a^2 w / (1 - a^2); and, put by in shared memory until the adjoints are there, g,
-// b (1 - s(write)) and 1 - s(retention).
-template <typename T, bool SEG, bool NEAR, int K>
+// Of a thread's tokens: f = a (-0 later where a segment starts); b = g x with g = sqrt(1 - a^2) s(write);
+// q1 = a u and q2 = b kappa, so that q1 h_{t-1} + q2 = u du / lam; and, put by in shared memory until
+// the adjoints are there, g, b (1 - s(write)) and 1 - s(retention).
+template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_bwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
-                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2* put,
-                                                 float2 (&c)[K], float2 (&b)[K], float2 (&q1)[K], float2 (&q2)[K]) {
+                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu, float2* put,
+                                                 float2 (&f)[K], float2 (&b)[K], float2 (&q1)[K], float2 (&q2)[K]) {
   constexpr int N = 4;
 #pragma unroll
   for (int k0 = 0; k0 < K; k0 += N) {
-    float2 v[N], er[N], ew[N], sr[N], sw[N], q[N], a[N];
+    float2 r[N], w[N];
+    GatedGates<true, N> o;
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = Duo<T>::get(rr[k0 + k]);
-    exp_neg<T>(v, er);
-    logistic_of(er, sr);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = Duo<T>::get(rw[k0 + k]);
-    exp_neg<T>(v, ew);
-    logistic_of(ew, sw);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = mul2(nu, sr[k]);
-    decay<NEAR>(v, a, q);
+    for (int k = 0; k < N; ++k) r[k] = Duo<T>::get(rr[k0 + k]), w[k] = Duo<T>::get(rw[k0 + k]);
+    gated_gates<T, NEAR, true, N>(r, w, nu, root_nu, o);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const float2 m = mul2(q[k], add2(a[k], bcast2(1.0f)));
-      // (1 - a^2 = 0 only with w = 0, or w too small for float32: the products with m and w are then 0)
-      const float2 rs = make_float2(rsqrt_approx(fmaxf(m.x, 1.17549435e-38f)), rsqrt_approx(fmaxf(m.y, 1.17549435e-38f)));
-      const float2 xs = mul2(Duo<T>::get(rx[k0 + k]), sw[k]), beta = mul2(m, rs);
-      b[k0 + k] = mul2(beta, xs);
-      put[(k0 + k) * 96] = mul2(beta, sw[k]);
-      put[(k0 + k) * 96 + 32] = mul2(b[k0 + k], one_minus_s(ew[k], sw[k]));
-      put[(k0 + k) * 96 + 64] = one_minus_s(er[k], sr[k]);
-      q1[k0 + k] = mul2(a[k], v[k]);
-      q2[k0 + k] = neg2(mul2(mul2(q1[k0 + k], a[k]), mul2(xs, rs)));
-      c[k0 + k] = a[k];
+      const float2 g = mul2(o.beta[k], o.sw[k]), bk = mul2(g, Duo<T>::get(rx[k0 + k]));
+      put[(k0 + k) * 96] = g;
+      put[(k0 + k) * 96 + 32] = mul2(bk, o.om_w[k]);
+      put[(k0 + k) * 96 + 64] = o.om_r[k];
+      f[k0 + k] = o.a[k];
+      b[k0 + k] = bk;
+      q1[k0 + k] = mul2(o.a[k], o.u[k]);
+      q2[k0 + k] = mul2(bk, o.kappa[k]);
     }
   }
 }
@@ -583,6 +663,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   float2* put = reinterpret_cast<float2*>(s_raw) + wp * K * 96 + lane;
   R* stage = reinterpret_cast<R*>(s_raw + NW * K * 96 * sizeof(float2)) + wp * NT * K * 32;
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
+  const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, -stride);
   if (cs > 1) exchange_init(s_cta);
@@ -592,7 +673,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
     int tile = (steps - 1) * cs + rank, t0 = tile * TILE + wp * K;
     float2 carry = load_pair(p.grad_last, bt * p.D + ch, ch, p.D);  // c_{t+1} lam_{t+1} entering the step's last token
-    long long at = (bt * p.L + t0) * p.D + ch;                      // of this thread's first token in the gradients
+    long long base = (bt * p.L + (long long)tile * TILE) * p.D;     // of the CTA's first token and channel in the gradients
     reader.start(p, bt, t0, ch0, lane);
     reader.copy(p.L - t0);
     for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, ++n) {
@@ -615,13 +696,13 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
         gated_read<T, MODE, K>(p, 3, stage, bt, t0, ch, lane, rd);
         __syncwarp();
         reader.copy(step > 0 ? live + stride : 0);
-        if (near) gated_bwd_tokens<T, SEG, true>(rx, rr, rw, nu, put, f, b, q1, q2);
-        else gated_bwd_tokens<T, SEG, false>(rx, rr, rw, nu, put, f, b, q1, q2);
+        if (near) gated_bwd_tokens<T, true>(rx, rr, rw, nu, root_nu, put, f, b, q1, q2);
+        else gated_bwd_tokens<T, false>(rx, rr, rw, nu, root_nu, put, f, b, q1, q2);
       }
       if (SEG && seg != 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
-          if (seg >> k & 1u) f[k] = bcast2(-0.0f), q1[k] = bcast2(-0.0f);
+          if (seg >> k & 1u) f[k] = bcast2(-0.0f);
       }
       if (live < K) {
 #pragma unroll
@@ -648,18 +729,18 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
 #pragma unroll
       for (int j = 0; j < NW - 1; ++j)
         if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
-      // states forward: q1 <- q1 h_{t-1} + q2 = -du u / lam
+      // states forward: q1 <- q1 h_{t-1} + q2 (nothing of h_{t-1} at a segment start)
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        q1[k] = through<SEG>(q1[k], q2[k], h);
+        const float2 v = fma2(q1[k], h, q2[k]);
+        q1[k] = SEG ? make_float2(dropped(f[k].x) ? q2[k].x : v.x, dropped(f[k].y) ? q2[k].y : v.y) : v;
         h = through<SEG>(f[k], b[k], h);
       }
       float2 c;  // the adjoint entering this CTA's tile, then this warp's tokens
       if (cs > 1) {
         exchange_wait(p, s_cta, n);
-        for (int q = cs - 1; q > rank; --q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
-        c = carry;
-        for (int q = rank; q >= 0; --q) carry = through<SEG>(lo2(s_cta.map[par][q][lane]), hi2(s_cta.map[par][q][lane]), carry);
+        c = exchange_through<SEG>(s_cta, par, cs - 1, rank, -1, lane, carry);
+        carry = exchange_through<SEG>(s_cta, par, rank, -1, -1, lane, c);
       } else {
         c = step == steps - 1 ? carry : s_out[par ^ 1][lane];
       }
@@ -668,17 +749,18 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
         if (j > wp) c = through<SEG>(lo2(s_map[par][j][lane]), s_adj[par][j][lane], c);
       // adjoints in reverse
       float2 sum = bcast2(0.0f);
-      long long i = at + (long long)(K - 1) * p.D;
+      T *dx = static_cast<T*>(p.dx) + base, *dr = static_cast<T*>(p.dr) + base, *dw = static_cast<T*>(p.dw) + base;
+      unsigned i = (unsigned)(wp * K + K - 1) * (unsigned)p.D + (unsigned)ch;
       auto token = [&](int k, bool store) {
-        const float2 lam = add2(Duo<T>::get(rd[k]), c), du = mul2(neg2(lam), q1[k]);
+        const float2 lam = add2(Duo<T>::get(rd[k]), c), du = mul2(lam, q1[k]);
         c = through0<SEG>(f[k], lam);
         if (store) {
-          gated_store<T, MODE>(static_cast<T*>(p.dx) + i, ch, p.D, mul2(lam, put[k * 96]));
-          gated_store<T, MODE>(static_cast<T*>(p.dw) + i, ch, p.D, mul2(lam, put[k * 96 + 32]));
-          gated_store<T, MODE>(static_cast<T*>(p.dr) + i, ch, p.D, mul2(du, put[k * 96 + 64]));
+          gated_store<T, MODE>(dx + i, ch, p.D, mul2(lam, put[k * 96]));
+          gated_store<T, MODE>(dw + i, ch, p.D, mul2(lam, put[k * 96 + 32]));
+          gated_store<T, MODE>(dr + i, ch, p.D, mul2(du, put[k * 96 + 64]));
           sum = add2(sum, du);
         }
-        i -= p.D;
+        i -= (unsigned)p.D;
       };
       if (live >= K && on) {
 #pragma unroll
@@ -687,7 +769,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) token(k, k < live && on);
       }
-      at -= (long long)stride * p.D;
+      base -= (long long)stride * p.D;
       dnu_x += (double)sum.x;
       dnu_y += (double)sum.y;
       if (wp == 0) {
@@ -740,23 +822,31 @@ struct GatedStepParams {
   int D;
 };
 
-template <typename T>
+// A warp owns the 64 channels that a warp of the scan owns (two a lane), so that its arithmetic and
+// its results are those of a scan of one token.
+template <typename T, int MODE>
 __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p) {
-  const int d = blockIdx.x * 128 + threadIdx.x;
-  if (d >= p.D) return;
-  const float nu = gated_nu(__ldg(p.nu_log + d));
+  const int ch = (int)(blockIdx.x * 128 + threadIdx.x) * 2;
+  const bool on = ch < p.D, both = ch + 1 < p.D;
+  const float2 nu = make_float2(on ? gated_nu(__ldg(p.nu_log + ch)) : 0.0f, both ? gated_nu(__ldg(p.nu_log + ch + 1)) : 0.0f);
+  const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
+  const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
+  if (!on) return;
+  auto load = [&](const void* base, long long i) {
+    const T* q = static_cast<const T*>(base) + i + ch;
+    if constexpr (MODE != kModeSingle) return Duo<T>::get(__ldg(reinterpret_cast<const typename Duo<T>::type*>(q)));
+    return make_float2(Io<T>::load(q), both ? Io<T>::load(q + 1) : 0.0f);
+  };
   for (long long b = blockIdx.y; b < p.B; b += gridDim.y) {
-    const float x = Io<T>::load(static_cast<const T*>(p.x) + b * p.sx + d);
-    const float r = Io<T>::load(static_cast<const T*>(p.r) + b * p.sr + d);
-    const float w = Io<T>::load(static_cast<const T*>(p.w) + b * p.sw + d);
-    const float s = p.state[b * p.D + d];
-    const float2 x2[1] = {bcast2(x)}, r2[1] = {bcast2(r)}, w2[1] = {bcast2(w)};
-    float2 a[1], c[1];
-    gated_ab<T, false>(x2, r2, w2, bcast2(nu), a, c);
+    const float2 x[1] = {load(p.x, b * p.sx)}, r[1] = {load(p.r, b * p.sr)}, w[1] = {load(p.w, b * p.sw)};
+    const float2 s = load_pair(p.state, b * p.D + ch, ch, p.D);
     const bool start = p.pos != nullptr && gated_starts(p.pos, p.pos_bytes, b);
-    const float h = start ? c[0].x : fmaf(a[0].x, s, c[0].x);
-    Io<T>::store(static_cast<T*>(p.y) + b * p.D + d, h);
-    p.new_state[b * p.D + d] = h;
+    float2 a[1], c[1];
+    if (near) gated_ab<T, true>(x, r, w, nu, root_nu, a, c);
+    else gated_ab<T, false>(x, r, w, nu, root_nu, a, c);
+    const float2 h = start ? c[0] : fma2(a[0], s, c[0]);
+    gated_store<T, MODE>(static_cast<T*>(p.y) + b * p.D + ch, ch, p.D, h);
+    store_pair(p.new_state, b * p.D + ch, ch, p.D, h);
   }
 }
 
@@ -904,7 +994,7 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
   const GatedMode mode = gated_aligned(p.y, 2 * size) ? gated_mode(p, 3, size) : kModeSingle;
-  const GatedPlan pl = gated_plan(p.B, p.L, p.D, kFwdTile);
+  const GatedPlan pl = gated_plan(p.B, p.L, p.D, a->dtype == SPARC_DTYPE_BF16 ? GatedFwdCut<__nv_bfloat16>::TILE : GatedFwdCut<float>::TILE);
   p.groups = pl.groups;
   p.cluster = pl.cluster;
   p.rows = pl.rows;
@@ -998,13 +1088,22 @@ int sparc_gated_step(const SparcGatedStepArgs* a, void* stream) {
   p.new_state = a->new_state;
   p.B = a->batch;
   p.D = (int)a->channels;
-  const dim3 grid((unsigned)((p.D + 127) / 128), (unsigned)std::min<long long>(p.B, 32768));
+  const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
+  for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
+    if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
+  bool pairs = p.D % 2 == 0 && gated_aligned(p.x, 2 * size) && gated_aligned(p.r, 2 * size) &&
+               gated_aligned(p.w, 2 * size) && gated_aligned(p.y, 2 * size);
+  if (p.B > 1) pairs = pairs && p.sx % 2 == 0 && p.sr % 2 == 0 && p.sw % 2 == 0;
+  const dim3 grid((unsigned)((p.D + 255) / 256), (unsigned)std::min<long long>(p.B, 32768));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   TimedLaunch tl(kTimeGatedStep, s);
-  if (a->dtype == SPARC_DTYPE_BF16)
-    gated_step_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  else
-    gated_step_kernel<float><<<grid, 128, 0, s>>>(p);
+  if (a->dtype == SPARC_DTYPE_BF16) {
+    if (pairs) gated_step_kernel<__nv_bfloat16, kModePair><<<grid, 128, 0, s>>>(p);
+    else gated_step_kernel<__nv_bfloat16, kModeSingle><<<grid, 128, 0, s>>>(p);
+  } else {
+    if (pairs) gated_step_kernel<float, kModePair><<<grid, 128, 0, s>>>(p);
+    else gated_step_kernel<float, kModeSingle><<<grid, 128, 0, s>>>(p);
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
   return SPARC_OK;
