@@ -4,10 +4,13 @@
 //
 // Both directions read every activation once: a row lives in the registers of one warp, or of one
 // CTA where it is wider, as NV vectors of VEC elements a thread (16 bytes where width, strides and
-// bases allow it, else single elements). The statistics are exact two-step ones: each warp's mean,
+// bases allow it, else single elements). CTAs walk the rows; of the 16-byte vectors each thread keeps
+// its share of the next kLnRing rows on the way into shared memory by asynchronous copies that only
+// it waits for (two rows in registers leave HBM a third idle), of single elements the next row in
+// registers. The statistics are exact two-step ones: each warp's mean,
 // then its squared deviations about that mean, joined over the warps with one barrier by
 //   mean = sum n_i mean_i / n,  M = sum M_i + n_i (mean_i - mean)^2,
-// so no sum of squares about zero cancels. CTAs walk the rows; in the backward a thread keeps the
+// so no sum of squares about zero cancels. In the backward a thread keeps the
 // sums of dw and db of its own columns in registers, each CTA writes one row of partial sums, and
 // a second kernel adds those rows in a fixed order (bitwise reproducible). Rows wider than the
 // registers hold go to kernels that read them again from cache.
@@ -79,141 +82,217 @@ __device__ __forceinline__ float warp_sum(float v) {
 constexpr int kLnRows = 8;
 template <int WARPS> constexpr int kLnThreads = WARPS == 1 ? 32 * kLnRows : 32 * WARPS;
 
-// Column of element e of vector j of thread i of a row: (j * 32 * WARPS + i) * VEC + e.
+// A thread's share of a row: element e of its vector j is column (j * 32 WARPS + i) VEC + e, i the
+// thread's number among the row's.
+template <typename T, int VEC, int NV, int WARPS>
+struct LnRow {
+  using V = LnVec<T, VEC>;
+  static constexpr int kStep = 32 * WARPS * VEC;  // columns from a vector to the next
+  // `f` <- the row's values, zeros beyond it
+  static __device__ __forceinline__ void get(const typename V::type (&raw)[NV], int c0, int W, float (&f)[NV * VEC]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      V::get(raw[j], f + j * VEC);
+      if (c0 + j * kStep >= W) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[j * VEC + e] = 0.0f;
+      }
+    }
+  }
+  static __device__ __forceinline__ void put(void* base, long long row, int c0, int W, const float (&f)[NV * VEC]) {
+    T* q = static_cast<T*>(base) + row + c0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (c0 + j * kStep < W) *reinterpret_cast<typename V::type*>(q + j * kStep) = V::make(f + j * VEC);
+  }
+  // float32 parameters of the same columns (zeros beyond the row, or where there are none)
+  static __device__ __forceinline__ void params(const float* w, int c0, int W, float (&f)[NV * VEC]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = c0 + j * kStep + e;
+        f[j * VEC + e] = w != nullptr && c < W ? __ldg(w + c) : 0.0f;
+      }
+  }
+};
+
+// A thread's share of the next rows of NT tensors: up to kLnRing of them in shared memory, slot by
+// slot, as far as kLnRingBytes a CTA go, or (single elements) one in registers. Rows are asked for in
+// order, one for each that is taken.
+constexpr int kLnRing = 4, kLnRingBytes = 96 * 1024;
+template <typename T, int VEC, int NV, int WARPS, int NT>
+struct LnAhead {
+  using Row = LnRow<T, VEC, NV, WARPS>;
+  using R = typename LnVec<T, VEC>::type;
+  static constexpr bool kRing = VEC > 1;
+  static constexpr int kRowBytes = NT * NV * 16 * kLnThreads<WARPS>;
+  static constexpr int kDepth = kRing ? std::min(kLnRing, kLnRingBytes / kRowBytes) : 1;
+  static constexpr int kBytes = kRing ? kDepth * kRowBytes : 0;
+  static_assert(kDepth >= 1);
+  R raw[kRing ? 1 : NT][NV];
+  R* mine;  // [slot][tensor][vector][thread]
+  int slot;
+
+  __device__ __forceinline__ explicit LnAhead(unsigned char* ring) : mine(reinterpret_cast<R*>(ring) + threadIdx.x), slot(0) {}
+  // tensor n's row at `q` (this thread's first column); none where not `valid`
+  __device__ __forceinline__ void ask(int n, const T* q, bool valid, int c0, int W) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (valid && c0 + j * Row::kStep < W) {
+        if constexpr (kRing)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           smem_addr(mine + ((slot * NT + n) * NV + j) * kLnThreads<WARPS>)),
+                       "l"(q + j * Row::kStep)
+                       : "memory");
+        else
+          raw[n][j] = __ldg(reinterpret_cast<const R*>(q + j * Row::kStep));
+      }
+  }
+  __device__ __forceinline__ void asked() {  // the row's tensors are complete
+    if constexpr (kRing) {
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      slot = slot + 1 == kDepth ? 0 : slot + 1;
+    }
+  }
+  // with kDepth rows asked for and not taken, the first of them has come (its slot is the next one asked for)
+  __device__ __forceinline__ void wait() {
+    if constexpr (kRing) asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+  }
+  __device__ __forceinline__ void take(int n, int c0, int W, float (&f)[NV * VEC]) {
+    if constexpr (kRing) {
+      R v[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) v[j] = mine[((slot * NT + n) * NV + j) * kLnThreads<WARPS>];
+      Row::get(v, c0, W, f);
+    } else {
+      Row::get(raw[n], c0, W, f);
+    }
+  }
+};
+
+// Elements of a row that warp k of its WARPS holds.
+template <int VEC, int NV, int WARPS>
+__device__ __forceinline__ int ln_count(int k, int W) {
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) n += max(0, min(32 * VEC, W - (j * 32 * WARPS + k * 32) * VEC));
+  return n;
+}
+
 template <typename T, int VEC, int NV, int WARPS>
 __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_fwd_kernel(const LnParams p) {
-  using V = LnVec<T, VEC>;
-  __shared__ float2 s_stat[2][WARPS];
+  using Row = LnRow<T, VEC, NV, WARPS>;
+  constexpr int E = NV * VEC;
+  __shared__ float4 s_stat[2][WARPS];  // mean, squared deviations, count
   const int i = WARPS == 1 ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = i * VEC;
   const long long first = WARPS == 1 ? (long long)blockIdx.x * kLnRows + wp : blockIdx.x;
   const long long step = WARPS == 1 ? (long long)gridDim.x * kLnRows : gridDim.x;
   const float inv_w = 1.0f / (float)p.W;
-  // this warp's elements of a row
-  int count = 0;
+  const float count = (float)ln_count<VEC, NV, WARPS>(WARPS == 1 ? 0 : wp, p.W);
+  const float inv_count = count > 0.0f ? 1.0f / count : 0.0f;
+  extern __shared__ __align__(16) unsigned char s_ring[];
+  using Ahead = LnAhead<T, VEC, NV, WARPS, 1>;
+  Ahead ahead(s_ring);
+  auto ask = [&](long long r) {
+    ahead.ask(0, static_cast<const T*>(p.x) + r * p.sx + c0, r < p.R, c0, p.W);
+    ahead.asked();
+  };
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c0 = (j * 32 * WARPS + (i - lane)) * VEC;
-    count += max(0, min(32 * VEC, p.W - c0));
-  }
-  const float inv_count = count > 0 ? 1.0f / (float)count : 0.0f;
+  for (int k = 0; k < Ahead::kDepth; ++k) ask(first + k * step);
+  float w[E], b[E];
+  Row::params(p.w, c0, p.W, w);
+  Row::params(p.b, c0, p.W, b);
   int par = 0;
   for (long long r = first; r < p.R; r += step, par ^= 1) {
-    float x[NV][VEC];
-    float sum = 0.0f;
-    typename V::type raw[NV];
+    float x[E], sum = 0.0f, m2 = 0.0f;
+    ahead.wait();
+    ahead.take(0, c0, p.W, x);
+    ask(r + Ahead::kDepth * step);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-      if (c < p.W) raw[j] = __ldg(reinterpret_cast<const typename V::type*>(static_cast<const T*>(p.x) + r * p.sx + c));
-    }
+    for (int k = 0; k < E; ++k) sum += x[k];
+    float mean = warp_sum(sum) * inv_count;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-      V::get(raw[j], x[j]);
+    for (int j = 0; j < NV; ++j)
+      if (c0 + j * Row::kStep < p.W) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum += c < p.W ? x[j][e] : 0.0f;
-    }
-    float mean = warp_sum(sum) * inv_count, m2 = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = x[j][e] - mean;
-        m2 += c < p.W ? d * d : 0.0f;
+        for (int e = 0; e < VEC; ++e) {
+          const float d = x[j * VEC + e] - mean;
+          m2 = fmaf(d, d, m2);
+        }
       }
-    }
     m2 = warp_sum(m2);
     if constexpr (WARPS > 1) {
-      if (lane == 0) s_stat[par][wp] = make_float2(mean, m2);
+      if (lane == 0) s_stat[par][wp] = make_float4(mean, m2, count, 0.0f);
       __syncthreads();
       float all = 0.0f;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) all = fmaf(s_stat[par][k].z, s_stat[par][k].x, all);
+      mean = all * inv_w;
       m2 = 0.0f;
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) {
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) n += max(0, min(32 * VEC, p.W - (j * 32 * WARPS + k * 32) * VEC));
-        all = fmaf((float)n, s_stat[par][k].x, all);
-      }
-      mean = all * inv_w;
-#pragma unroll
-      for (int k = 0; k < WARPS; ++k) {
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) n += max(0, min(32 * VEC, p.W - (j * 32 * WARPS + k * 32) * VEC));
-        const float d = s_stat[par][k].x - mean;
-        m2 += n > 0 ? fmaf((float)n * d, d, s_stat[par][k].y) : 0.0f;
+        const float4 q = s_stat[par][k];
+        const float d = q.x - mean;
+        m2 += q.z > 0.0f ? fmaf(q.z * d, d, q.y) : 0.0f;
       }
     }
     const float rstd = 1.0f / sqrtf(fmaf(m2, inv_w, p.eps));
     if (i == 0 && p.mean != nullptr) p.mean[r] = mean, p.rstd[r] = rstd;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-      if (c < p.W) {
-        float y[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float n = (x[j][e] - mean) * rstd;
-          y[e] = p.b != nullptr ? fmaf(n, __ldg(p.w + c + e), __ldg(p.b + c + e)) : n * __ldg(p.w + c + e);
-        }
-        *reinterpret_cast<typename V::type*>(static_cast<T*>(p.out) + r * p.W + c) = V::make(y);
-      }
+    for (int k = 0; k < E; ++k) {
+      const float n = (x[k] - mean) * rstd;
+      x[k] = p.b != nullptr ? fmaf(n, w[k], b[k]) : n * w[k];
     }
+    Row::put(p.out, r * p.W, c0, p.W, x);
   }
 }
 
 template <typename T, int VEC, int NV, int WARPS>
 __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_bwd_kernel(const LnParams p) {
-  using V = LnVec<T, VEC>;
+  using Row = LnRow<T, VEC, NV, WARPS>;
   constexpr int E = NV * VEC;
   __shared__ float2 s_sum[2][WARPS];
-  extern __shared__ float s_part[];  // WARPS == 1: [kLnRows][2][W]
   const int i = WARPS == 1 ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = i * VEC;
   const long long first = WARPS == 1 ? (long long)blockIdx.x * kLnRows + wp : blockIdx.x;
   const long long step = WARPS == 1 ? (long long)gridDim.x * kLnRows : gridDim.x;
   const float inv_w = 1.0f / (float)p.W;
+  extern __shared__ __align__(16) unsigned char s_ring[];
+  using Ahead = LnAhead<T, VEC, NV, WARPS, 2>;
+  Ahead ahead(s_ring);
+  auto ask = [&](long long r) {
+    ahead.ask(0, static_cast<const T*>(p.x) + r * p.sx + c0, r < p.R, c0, p.W);
+    ahead.ask(1, static_cast<const T*>(p.dy) + r * p.sdy + c0, r < p.R, c0, p.W);
+    ahead.asked();
+  };
+#pragma unroll
+  for (int k = 0; k < Ahead::kDepth; ++k) ask(first + k * step);
+  float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
+  if (first < p.R) next_mean = __ldg(p.mean + first), next_rstd = __ldg(p.rstd + first);
   float w[E], dw[E], db[E];
+  Row::params(p.w, c0, p.W, w);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * 32 * WARPS + i) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[j * VEC + e] = c < p.W ? __ldg(p.w + c + e) : 0.0f;
-      dw[j * VEC + e] = db[j * VEC + e] = 0.0f;
-    }
-  }
+  for (int k = 0; k < E; ++k) dw[k] = db[k] = 0.0f;
   int par = 0;
   for (long long r = first; r < p.R; r += step, par ^= 1) {
-    typename V::type rx[NV], rd[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-      if (c < p.W) {
-        rx[j] = __ldg(reinterpret_cast<const typename V::type*>(static_cast<const T*>(p.x) + r * p.sx + c));
-        rd[j] = __ldg(reinterpret_cast<const typename V::type*>(static_cast<const T*>(p.dy) + r * p.sdy + c));
-      }
-    }
-    const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
     float n[E], d[E], s1 = 0.0f, s2 = 0.0f;
+    ahead.wait();
+    ahead.take(0, c0, p.W, n);
+    ahead.take(1, c0, p.W, d);
+    ask(r + Ahead::kDepth * step);
+    mean = next_mean;
+    rstd = next_rstd;
+    if (r + step < p.R) next_mean = __ldg(p.mean + r + step), next_rstd = __ldg(p.rstd + r + step);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const bool on = (j * 32 * WARPS + i) * VEC < p.W;
-      V::get(rx[j], n + j * VEC);
-      V::get(rd[j], d + j * VEC);
-#pragma unroll
-      for (int k = j * VEC; k < (j + 1) * VEC; ++k) {
-        n[k] = on ? (n[k] - mean) * rstd : 0.0f;
-        d[k] = on ? d[k] : 0.0f;
-        dw[k] = fmaf(d[k], n[k], dw[k]);
-        db[k] += d[k];
-        d[k] *= w[k];
-        s1 += d[k];
-        s2 = fmaf(d[k], n[k], s2);
-      }
+    for (int k = 0; k < E; ++k) {
+      n[k] = (n[k] - mean) * rstd;  // (beyond the row d = 0, so n does not matter)
+      dw[k] = fmaf(d[k], n[k], dw[k]);
+      db[k] += d[k];
+      d[k] *= w[k];
+      s1 += d[k];
+      s2 = fmaf(d[k], n[k], s2);
     }
     s1 = warp_sum(s1);
     s2 = warp_sum(s2);
@@ -224,42 +303,37 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_bwd_kernel(const LnParam
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) s1 += s_sum[par][k].x, s2 += s_sum[par][k].y;
     }
-    s1 *= inv_w;
-    s2 *= inv_w;
+    s1 *= inv_w * rstd;
+    s2 *= inv_w * rstd;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-      if (c < p.W) {
-        float o[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = rstd * (d[j * VEC + e] - s1 - n[j * VEC + e] * s2);
-        *reinterpret_cast<typename V::type*>(static_cast<T*>(p.out) + r * p.W + c) = V::make(o);
-      }
-    }
+    for (int k = 0; k < E; ++k) d[k] = fmaf(rstd, d[k], fmaf(-n[k], s2, -s1));
+    Row::put(p.out, r * p.W, c0, p.W, d);
   }
   if (p.part == nullptr) return;
   float* part = p.part + (long long)blockIdx.x * 2 * p.W;
   if constexpr (WARPS > 1) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * WARPS + i) * VEC;
-      if (c < p.W) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) part[c + e] = dw[j * VEC + e], part[p.W + c + e] = db[j * VEC + e];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 + lane) * VEC;
-      if (c < p.W) {
+    for (int j = 0; j < NV; ++j)
+      if (c0 + j * Row::kStep < p.W) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          s_part[wp * 2 * p.W + c + e] = dw[j * VEC + e];
-          s_part[wp * 2 * p.W + p.W + c + e] = db[j * VEC + e];
+          const int c = c0 + j * Row::kStep + e;
+          part[c] = dw[j * VEC + e], part[p.W + c] = db[j * VEC + e];
         }
       }
-    }
+  } else {
+    float* s_part = reinterpret_cast<float*>(s_ring);  // [kLnRows][2][W], once every warp is through with its rows
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (c0 + j * Row::kStep < p.W) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int c = c0 + j * Row::kStep + e;
+          s_part[wp * 2 * p.W + c] = dw[j * VEC + e];
+          s_part[wp * 2 * p.W + p.W + c] = db[j * VEC + e];
+        }
+      }
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * p.W; c += kLnThreads<WARPS>) {
       float s = 0.0f;
@@ -349,29 +423,39 @@ __global__ void __launch_bounds__(256) ln_wide_cols_kernel(const LnParams p) {
   p.part[(long long)blockIdx.x * 2 * p.W + p.W + c] = db;
 }
 
-// dw, db from the partial rows: a block owns 32 of the 2 W columns, its warps every 8th row, in
-// float64 and in order.
-__global__ void __launch_bounds__(256) ln_reduce_kernel(const float* part, float* dw, float* db, int rows, int W) {
-  __shared__ double s[8][32];
+// dw, db from the partial rows: a block owns 32 of the 2 W columns, its 32 warps every 32nd row, in
+// float64 and in order. (The rows are read four at a time: the kernel is a chain of loads.)
+__global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, float* dw, float* db, int rows, int W) {
+  __shared__ double s[32][33];
+  pdl_wait();
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
-  const long long c = (long long)blockIdx.x * 32 + lane;
+  const long long c = (long long)blockIdx.x * 32 + lane, n = 2LL * W;
   double t = 0.0;
-  if (c < 2LL * W)
-    for (int r = wp; r < rows; r += 8) t += (double)part[(long long)r * 2 * W + c];
+  if (c < n)
+    for (int r = wp; r < rows; r += 128) {
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = r + 32 * u < rows ? part[(r + 32 * u) * n + c] : 0.0f;
+      t += ((double)v[0] + (double)v[1]) + ((double)v[2] + (double)v[3]);
+    }
   s[wp][lane] = t;
   __syncthreads();
-  if (wp == 0 && c < 2LL * W) {
-    for (int k = 1; k < 8; ++k) t += s[k][lane];
-    if (c < W) {
-      if (dw != nullptr) dw[c] = (float)t;
+  t = s[lane][wp];  // column wp of the block, row lane of its sums
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const long long out = (long long)blockIdx.x * 32 + wp;
+  if (lane == 0 && out < n) {
+    if (out < W) {
+      if (dw != nullptr) dw[out] = (float)t;
     } else if (db != nullptr) {
-      db[c - W] = (float)t;
+      db[out - W] = (float)t;
     }
   }
 }
 
 // ---------------------------------------------------------------- host
-constexpr int kLnMaxGrid = 148 * 8;  // the most CTAs that walk the rows, and rows of partial sums
+constexpr int kLnSms = 148;
+constexpr int kLnSumGrid = kLnSms * 8;  // the most CTAs that walk the rows
 
 struct LnPlan {
   int vec, nv, warps;  // warps == 0: the wide kernels
@@ -380,18 +464,12 @@ struct LnPlan {
 // The narrowest of the instances that holds a row; vectors where `vectors` (16-byte aligned rows).
 static LnPlan ln_plan(int W, bool vectors, int size) {
   const int vec = vectors ? 16 / size : 1;
-  const int small = vec == 8 ? 1 : vec == 4 ? 2 : 4, big = vec == 8 ? 2 : vec == 4 ? 4 : 16;
-  for (int warps : {1, 4, 8, 16})
-    for (int nv : {small, big})
-      if ((long long)32 * warps * vec * nv >= W) return LnPlan{vec, nv, warps};
+  if (W <= 256) return LnPlan{vec, 8 / vec, 1};
+  if (W <= 512) return LnPlan{vec, 16 / vec, 1};
+  if (W <= 1024) return LnPlan{vec, 8 / vec, 4};
+  for (int warps : {4, 8, 16})
+    if (W <= 32 * 16 * warps) return LnPlan{vec, 16 / vec, warps};
   return LnPlan{1, 0, 0};
-}
-
-static int ln_rows_per_cta(const LnPlan& pl) { return pl.warps == 1 ? kLnRows : 1; }
-
-static int ln_grid(long long R, const LnPlan& pl) {
-  const int per = ln_rows_per_cta(pl);
-  return (int)std::min<long long>((R + per - 1) / per, kLnMaxGrid);
 }
 
 static int ln_check_shape(long long R, long long W) {
@@ -402,49 +480,63 @@ static int ln_check_shape(long long R, long long W) {
 }
 
 static size_t ln_ws_bytes(long long R, long long W) {
-  return (size_t)std::min<long long>(R, kLnMaxGrid) * 2 * (size_t)W * sizeof(float);
+  return (size_t)std::min<long long>(R, kLnSumGrid) * 2 * (size_t)W * sizeof(float);
 }
 
+// CTAs that walk the rows: as many as are resident at once, and in the backward write a row of partial
+// sums each (kLnSumGrid of them at most).
 template <typename T, int VEC, int NV, int WARPS>
-static cudaError_t ln_launch(const LnParams& p, int grid, bool backward, cudaStream_t s) {
-  TimedLaunch tl(backward ? kTimeLnBwd : kTimeLnFwd, s);
-  if (backward) {
-    const size_t smem = WARPS == 1 ? (size_t)kLnRows * 2 * p.W * sizeof(float) : 0;
-    ln_bwd_kernel<T, VEC, NV, WARPS><<<grid, kLnThreads<WARPS>, smem, s>>>(p);
-  } else {
-    ln_fwd_kernel<T, VEC, NV, WARPS><<<grid, kLnThreads<WARPS>, 0, s>>>(p);
+static cudaError_t ln_launch(const LnParams& p, int* grid, bool backward, cudaStream_t s) {
+  const auto kernel = backward ? ln_bwd_kernel<T, VEC, NV, WARPS> : ln_fwd_kernel<T, VEC, NV, WARPS>;
+  const int ring = backward ? LnAhead<T, VEC, NV, WARPS, 2>::kBytes : LnAhead<T, VEC, NV, WARPS, 1>::kBytes;
+  // (one warp a row: the warps' sums meet in the same memory)
+  const int smem = backward && WARPS == 1 ? std::max(ring, kLnRows * 2 * 32 * VEC * NV * (int)sizeof(float)) : ring;
+  cudaError_t e = cudaSuccess;
+  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  static int resident[2] = {0, 0};
+  int per_sm = __atomic_load_n(&resident[backward], __ATOMIC_RELAXED);
+  if (per_sm == 0) {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kLnThreads<WARPS>, smem);
+    if (e != cudaSuccess) return e;
+    per_sm = std::max(1, std::min(per_sm, kLnSumGrid / kLnSms));
+    __atomic_store_n(&resident[backward], per_sm, __ATOMIC_RELAXED);
   }
+  const int rows = WARPS == 1 ? kLnRows : 1;
+  *grid = (int)std::min<long long>((p.R + rows - 1) / rows, (long long)per_sm * kLnSms);
+  TimedLaunch tl(backward ? kTimeLnBwd : kTimeLnFwd, s);
+  kernel<<<*grid, kLnThreads<WARPS>, smem, s>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T, int VEC, int NV>
-static cudaError_t ln_warps(const LnParams& p, const LnPlan& pl, int grid, bool backward, cudaStream_t s) {
-  switch (pl.warps) {
-    case 1: return ln_launch<T, VEC, NV, 1>(p, grid, backward, s);
-    case 4: return ln_launch<T, VEC, NV, 4>(p, grid, backward, s);
-    case 8: return ln_launch<T, VEC, NV, 8>(p, grid, backward, s);
-    default: return ln_launch<T, VEC, NV, 16>(p, grid, backward, s);
+static cudaError_t ln_warps(const LnParams& p, const LnPlan& pl, int* grid, bool backward, cudaStream_t s) {
+  if (pl.warps == 1) return ln_launch<T, VEC, NV, 1>(p, grid, backward, s);
+  if constexpr (VEC * NV == 16) {
+    if (pl.warps == 8) return ln_launch<T, VEC, NV, 8>(p, grid, backward, s);
+    if (pl.warps == 16) return ln_launch<T, VEC, NV, 16>(p, grid, backward, s);
   }
+  return ln_launch<T, VEC, NV, 4>(p, grid, backward, s);
 }
 
 template <typename T>
-static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, bool backward, cudaStream_t s) {
+static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, bool backward, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  const int grid = ln_grid(p.R, pl);
   if (pl.warps == 0) {
+    *grid = (int)std::min<long long>(p.R, kLnSumGrid);
     TimedLaunch tl(backward ? kTimeLnBwd : kTimeLnFwd, s);
     if (!backward) {
-      ln_wide_fwd_kernel<T><<<grid, kLnWide, 0, s>>>(p);
+      ln_wide_fwd_kernel<T><<<*grid, kLnWide, 0, s>>>(p);
     } else {
-      ln_wide_bwd_kernel<T><<<grid, kLnWide, 0, s>>>(p);
+      ln_wide_bwd_kernel<T><<<*grid, kLnWide, 0, s>>>(p);
       const cudaError_t e = cudaGetLastError();
       if (e != cudaSuccess) return e;
-      if (p.part != nullptr) ln_wide_cols_kernel<T><<<dim3(grid, (p.W + 255) / 256), 256, 0, s>>>(p);
+      if (p.part != nullptr) ln_wide_cols_kernel<T><<<dim3(*grid, (p.W + 255) / 256), 256, 0, s>>>(p);
     }
     return cudaGetLastError();
   }
   if (pl.vec == 1) {
-    return pl.nv == 4 ? ln_warps<T, 1, 4>(p, pl, grid, backward, s) : ln_warps<T, 1, 16>(p, pl, grid, backward, s);
+    return pl.nv == 8 ? ln_warps<T, 1, 8>(p, pl, grid, backward, s) : ln_warps<T, 1, 16>(p, pl, grid, backward, s);
   }
   if constexpr (V == 8) {
     return pl.nv == 1 ? ln_warps<T, 8, 1>(p, pl, grid, backward, s) : ln_warps<T, 8, 2>(p, pl, grid, backward, s);
@@ -493,8 +585,9 @@ int sparc_layer_norm_forward(const SparcLayerNormFwdArgs* a, void* stream) {
   const bool vectors = p.W * size % 16 == 0 && ln_aligned(a->x, p.sx, p.R, size) && ln_aligned(a->y, p.W, p.R, size);
   const LnPlan pl = ln_plan(p.W, vectors, size);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, false, s)
-                                                     : ln_dispatch<float>(p, pl, false, s);
+  int grid = 0;
+  const cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, &grid, false, s)
+                                                     : ln_dispatch<float>(p, pl, &grid, false, s);
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
   return SPARC_OK;
 }
@@ -529,12 +622,21 @@ int sparc_layer_norm_backward(const SparcLayerNormBwdArgs* a, void* stream) {
                        ln_aligned(a->dy, p.sdy, p.R, size) && ln_aligned(a->dx, p.W, p.R, size);
   const LnPlan pl = ln_plan(p.W, vectors, size);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, true, s)
-                                               : ln_dispatch<float>(p, pl, true, s);
+  int grid = 0;
+  cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, &grid, true, s)
+                                               : ln_dispatch<float>(p, pl, &grid, true, s);
   if (e == cudaSuccess && sums) {
     TimedLaunch tl(kTimeLnReduce, s);
-    ln_reduce_kernel<<<(2 * p.W + 31) / 32, 256, 0, s>>>(p.part, a->grad_weight, a->grad_bias, ln_grid(p.R, pl), p.W);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((2 * p.W + 31) / 32));
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, ln_reduce_kernel, (const float*)p.part, a->grad_weight, a->grad_bias, grid, p.W);
   }
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
   return SPARC_OK;
