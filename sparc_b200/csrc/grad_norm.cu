@@ -9,7 +9,7 @@
 // scales its chunks, the last read first, so that it meets what the caches still hold. Where
 // nothing is to be clipped and the gradients are updated in place nothing is written.
 //
-// Squares are summed in float32 over groups of a thread's eight elements and then in float64. A
+// Squares are summed in float32 over a thread's 16 or 32 elements at a time and then in float64. A
 // group whose sum leaves [2^-100, 2^120] is summed again in float64, so neither a square that
 // overflows nor one that underflows is lost: the norm is right for every finite float32 input.
 #include <algorithm>
@@ -25,7 +25,8 @@ namespace sparc {
 constexpr int kClipTensors = 256;   // tensors per launch
 constexpr int kClipChunk = 8192;    // elements per chunk
 constexpr int kClipThreads = 256;
-constexpr int kClipGrid = 148 * 4;  // the most CTAs, and partial sums per launch
+constexpr int kClipGrid = 148 * 8;  // the most CTAs, and partial sums per launch
+constexpr int kClipVecs = 4;        // 16-byte vectors a thread has on the way at once
 
 struct ClipTensors {
   const void* in[kClipTensors];
@@ -53,27 +54,99 @@ __device__ __forceinline__ int clip_find(const ClipTensors& t, unsigned chunk) {
   return lo;
 }
 
-template <int N>
-__device__ __forceinline__ void clip_add(const float (&v)[N], double& sum) {
-  float s = 0.0f;
+// 16 bytes of gradients: four float32 or eight bfloat16.
+template <typename T> struct ClipVec;
+template <> struct ClipVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(uint4 v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 scaled(uint4 v, float k) {
+    return make_uint4(__float_as_uint(__uint_as_float(v.x) * k), __float_as_uint(__uint_as_float(v.y) * k),
+                      __float_as_uint(__uint_as_float(v.z) * k), __float_as_uint(__uint_as_float(v.w) * k));
+  }
+};
+template <> struct ClipVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(uint4 v, float (&f)[8]) {
+    const unsigned u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int k = 0; k < N; ++k) s = fmaf(v[k], v[k], s);
-  if (s >= 7.8886090522101181e-31f && s <= 1.3292279957849159e36f) {
-    sum += (double)s;
-  } else {  // (also zeros, infinities and NaN)
+    for (int k = 0; k < 4; ++k) f[2 * k] = __uint_as_float(u[k] << 16), f[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ unsigned scaled(unsigned u, float k) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(u << 16) * k, __uint_as_float(u & 0xffff0000u) * k);
+    return *reinterpret_cast<const unsigned*>(&b);
+  }
+  static __device__ __forceinline__ uint4 scaled(uint4 v, float k) {
+    return make_uint4(scaled(v.x, k), scaled(v.y, k), scaled(v.z, k), scaled(v.w, k));
+  }
+};
+
+// The squares of n elements from `g` on.
+template <typename T>
+__device__ __forceinline__ void clip_squares(const T* g, int n, bool wide, double& sum) {
+  using V = ClipVec<T>;
+  int done = 0;
+  if (wide) {
+    const uint4* gv = reinterpret_cast<const uint4*>(g);
+    const int vecs = n / V::N;
+    for (int k = threadIdx.x; k < vecs; k += kClipVecs * kClipThreads) {
+      uint4 v[kClipVecs];
 #pragma unroll
-    for (int k = 0; k < N; ++k) sum = fma((double)v[k], (double)v[k], sum);
+      for (int u = 0; u < kClipVecs; ++u)
+        v[u] = k + u * kClipThreads < vecs ? __ldg(gv + k + u * kClipThreads) : make_uint4(0u, 0u, 0u, 0u);
+      // sums of four squares, added in pairs: at most seven roundings
+      constexpr int kParts = kClipVecs * V::N / 4;
+      float f[kClipVecs][V::N], s[kParts];
+#pragma unroll
+      for (int u = 0; u < kClipVecs; ++u) V::get(v[u], f[u]);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) {
+        const float* e = &f[q * 4 / V::N][q * 4 % V::N];
+        s[q] = fmaf(e[3], e[3], fmaf(e[2], e[2], fmaf(e[1], e[1], e[0] * e[0])));
+      }
+#pragma unroll
+      for (int d = 1; d < kParts; d *= 2)
+#pragma unroll
+        for (int q = 0; q + d < kParts; q += 2 * d) s[q] += s[q + d];
+      if (s[0] >= 7.8886090522101181e-31f && s[0] <= 1.3292279957849159e36f) {
+        sum += (double)s[0];
+      } else {  // (also zeros, infinities and NaN)
+#pragma unroll
+        for (int u = 0; u < kClipVecs; ++u)
+#pragma unroll
+          for (int e = 0; e < V::N; ++e) sum = fma((double)f[u][e], (double)f[u][e], sum);
+      }
+    }
+    done = vecs * V::N;
+  }
+  for (int k = done + threadIdx.x; k < n; k += kClipThreads) {
+    const double v = (double)to_float(g[k]);
+    sum = fma(v, v, sum);
   }
 }
 
-__device__ __forceinline__ void clip_unpack(uint4 v, float* f) {
-  const unsigned u[4] = {v.x, v.y, v.z, v.w};
+// out = g k for n elements.
+template <typename T>
+__device__ __forceinline__ void clip_scale(const T* g, T* o, int n, bool wide, float k0) {
+  using V = ClipVec<T>;
+  int done = 0;
+  if (wide) {
+    const uint4* gv = reinterpret_cast<const uint4*>(g);
+    uint4* ov = reinterpret_cast<uint4*>(o);
+    const int vecs = n / V::N;
+    for (int k = threadIdx.x; k < vecs; k += kClipVecs * kClipThreads) {
+      uint4 v[kClipVecs];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) f[2 * k] = __uint_as_float(u[k] << 16), f[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-}
-__device__ __forceinline__ unsigned clip_pack(float a, float b) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const unsigned*>(&v);
+      for (int u = 0; u < kClipVecs; ++u)
+        if (k + u * kClipThreads < vecs) v[u] = gv[k + u * kClipThreads];
+#pragma unroll
+      for (int u = 0; u < kClipVecs; ++u)
+        if (k + u * kClipThreads < vecs) ov[k + u * kClipThreads] = V::scaled(v[u], k0);
+    }
+    done = vecs * V::N;
+  }
+  for (int k = done + threadIdx.x; k < n; k += kClipThreads) Io<T>::store(o + k, to_float(g[k]) * k0);
 }
 
 // The sum over the block in a fixed order; every thread gets it.
@@ -97,38 +170,8 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_co
     const long long e0 = (long long)(c - t.first[i]) * kClipChunk;
     const int n = (int)min((long long)kClipChunk, t.count[i] - e0);
     const bool wide = reinterpret_cast<unsigned long long>(t.in[i]) % 16 == 0;
-    int done = 0;
-    if (t.bf16[i]) {
-      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(t.in[i]) + e0;
-      if (wide) {
-        const uint4* gv = reinterpret_cast<const uint4*>(g);
-        for (int k = threadIdx.x; k < n / 8; k += kClipThreads) {
-          float v[8];
-          clip_unpack(__ldg(gv + k), v);
-          clip_add(v, sum);
-        }
-        done = n / 8 * 8;
-      }
-      for (int k = done + threadIdx.x; k < n; k += kClipThreads) {
-        const float v[1] = {__bfloat162float(g[k])};
-        clip_add(v, sum);
-      }
-    } else {
-      const float* g = static_cast<const float*>(t.in[i]) + e0;
-      if (wide) {
-        const float4* gv = reinterpret_cast<const float4*>(g);
-        for (int k = threadIdx.x; k < n / 8; k += kClipThreads) {
-          const float4 a = __ldg(gv + 2 * k), b = __ldg(gv + 2 * k + 1);
-          const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-          clip_add(v, sum);
-        }
-        done = n / 8 * 8;
-      }
-      for (int k = done + threadIdx.x; k < n; k += kClipThreads) {
-        const float v[1] = {g[k]};
-        clip_add(v, sum);
-      }
-    }
+    if (t.bf16[i]) clip_squares(static_cast<const __nv_bfloat16*>(t.in[i]) + e0, n, wide, sum);
+    else clip_squares(static_cast<const float*>(t.in[i]) + e0, n, wide, sum);
   }
   sum = clip_block_sum(sum, s);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -164,32 +207,10 @@ __global__ void __launch_bounds__(kClipThreads) grad_clip_kernel(const __grid_co
     const bool same = t.in[i] == t.out[i];
     if (!(same && k0 == 1.0f)) {
       const bool wide = (reinterpret_cast<unsigned long long>(t.in[i]) | reinterpret_cast<unsigned long long>(t.out[i])) % 16 == 0;
-      int done = 0;
-      if (t.bf16[i]) {
-        const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(t.in[i]) + e0;
-        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(t.out[i]) + e0;
-        if (wide) {
-          for (int k = threadIdx.x; k < n / 8; k += kClipThreads) {
-            float v[8];
-            clip_unpack(reinterpret_cast<const uint4*>(g)[k], v);
-            reinterpret_cast<uint4*>(o)[k] = make_uint4(clip_pack(v[0] * k0, v[1] * k0), clip_pack(v[2] * k0, v[3] * k0),
-                                                        clip_pack(v[4] * k0, v[5] * k0), clip_pack(v[6] * k0, v[7] * k0));
-          }
-          done = n / 8 * 8;
-        }
-        for (int k = done + threadIdx.x; k < n; k += kClipThreads) o[k] = __float2bfloat16_rn(__bfloat162float(g[k]) * k0);
-      } else {
-        const float* g = static_cast<const float*>(t.in[i]) + e0;
-        float* o = static_cast<float*>(t.out[i]) + e0;
-        if (wide) {
-          for (int k = threadIdx.x; k < n / 4; k += kClipThreads) {
-            const float4 a = reinterpret_cast<const float4*>(g)[k];
-            reinterpret_cast<float4*>(o)[k] = make_float4(a.x * k0, a.y * k0, a.z * k0, a.w * k0);
-          }
-          done = n / 4 * 4;
-        }
-        for (int k = done + threadIdx.x; k < n; k += kClipThreads) o[k] = g[k] * k0;
-      }
+      if (t.bf16[i])
+        clip_scale(static_cast<const __nv_bfloat16*>(t.in[i]) + e0, static_cast<__nv_bfloat16*>(t.out[i]) + e0, n, wide, k0);
+      else
+        clip_scale(static_cast<const float*>(t.in[i]) + e0, static_cast<float*>(t.out[i]) + e0, n, wide, k0);
     }
     if (c < gridDim.x) break;
   }

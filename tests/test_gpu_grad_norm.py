@@ -1,7 +1,7 @@
 """The global gradient norm and clipping by it on the GPU (sparc_b200.grad_norm, clip_grads,
 clip_grad_norm_) against float64.
 
-Tolerances, U = 2^-24: a group of eight squares is summed in float32 (at most 9 U, all terms
+Tolerances, U = 2^-24: a thread's group of squares is summed in float32 (at most 9 U, all terms
 positive), everything else in float64, so the norm is off by 5 U and its own rounding by U; the
 factor by as much and its rounding, the product by half a step of the gradient's type."""
 import pytest
