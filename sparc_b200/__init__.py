@@ -19,7 +19,7 @@ from .grads import clip_grad_norm_, clip_grads, grad_norm
 from .norm import LayerNorm, layer_norm
 from .scan import (sparc_chunk_scan, sparc_scan, sparc_scan_precomputed_decay, sparc_scan_with_last,
                    sparc_tiled_serial_scan, sparc_training_scan_dispatch)
-from . import _lib
+from . import _lib, torch_ops
 
 
 def library_path() -> str:
@@ -28,7 +28,8 @@ def library_path() -> str:
 
 def check_status(clear: bool = True) -> None:
     """Raise if any kernel launch on a cached workspace recorded a bounded wait that ran out (a
-    tile kernel's wait on its TMA copies, or the real scan's lookback). The tensor-core product
+    tile kernel's wait on its TMA copies, the real scan's lookback, or the gated scan's exchange
+    within a cluster). The tensor-core product
     and the multi-GPU exchanges keep their own status words (gemm.gemm_status, the reducers'
     timed_out()).
 
@@ -38,6 +39,12 @@ def check_status(clear: bool = True) -> None:
         if st:
             if clear:
                 _lib.clear_status(ws)
+            raise RuntimeError(f"sparc_b200: a bounded wait in a kernel timed out (status {st:#x})")
+    for word in torch_ops.wait_status():
+        st = int(word.item())
+        if st:
+            if clear:
+                word.zero_()
             raise RuntimeError(f"sparc_b200: a bounded wait in a kernel timed out (status {st:#x})")
 
 

@@ -73,7 +73,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-TORCH_SRC = os.path.join(PKG, "csrc_torch", "torch_ops.cpp")
+TORCH_SRCS = [os.path.join(PKG, "csrc_torch", n) for n in ("torch_ops.cpp", "train_ops.cpp")]
 TORCH_LIB = os.path.join(PKG, "libsparc_b200_torch.so")
 
 
@@ -82,7 +82,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     (torch.ops.sparc_b200.*), with PyTorch's extension builder into _build/torch_ops and copy it
     in-tree. Its C-ABI symbols stay undefined: they resolve against libsparc_b200.so, which the
     loader (sparc_b200.torch_ops) opens with global visibility first."""
-    deps = [TORCH_SRC, os.path.join(INCLUDE, "sparc_b200.h")]
+    deps = [*TORCH_SRCS, os.path.join(INCLUDE, "sparc_b200.h")]
     if not force and os.path.exists(TORCH_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_LIB) for d in deps):
         return TORCH_LIB
     import ctypes
@@ -93,7 +93,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     ctypes.CDLL(build(), mode=ctypes.RTLD_GLOBAL)
     bdir = os.path.join(BUILD, "torch_ops")
     os.makedirs(bdir, exist_ok=True)
-    path = ce.load(name="sparc_b200_torch_ops", sources=[TORCH_SRC], extra_include_paths=[INCLUDE],
+    path = ce.load(name="sparc_b200_torch_ops", sources=TORCH_SRCS, extra_include_paths=[INCLUDE],
                    extra_cflags=["-O2"], build_directory=bdir, is_python_module=False, with_cuda=True,
                    verbose=verbose)
     built = os.path.join(bdir, "sparc_b200_torch_ops.so")

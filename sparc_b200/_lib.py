@@ -6,7 +6,6 @@ There is no fallback: if the library or a CUDA device is missing, every entry po
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -326,15 +325,6 @@ def ptr(t):
 
 def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def on_device(device: torch.device):
-    """A context in which `device` is CUDA's current device (a launch has to go to a stream of the
-    current device); nothing to do, and nothing done, where it already is."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-_SAME_DEVICE = contextlib.nullcontext()
 
 
 class _Workspaces:

@@ -8,7 +8,11 @@ library's host-only queries, symbolic lengths included), so that torch.compile /
 trace calls to them, and autograd formulas for ``mixer_forward`` (through ``mixer_backward``)
 and ``real_scan_forward`` (through ``real_scan_backward``): their first output is
 differentiable with respect to the activations and parameters; the saved carries, controls,
-states and last states are marked non-differentiable."""
+states and last states are marked non-differentiable.
+
+The operators of csrc_torch/train_ops.cpp (``gated_scan``, ``gated_scan_step``, ``layer_norm``,
+``grad_clip``) carry their own checks and autograd in C++ and are what `gated.py`, `norm.py` and
+`grads.py` call; they have no fake kernels."""
 from __future__ import annotations
 
 import ctypes
@@ -44,6 +48,23 @@ def load():
         _loaded = True
     _register_python_kernels()
     return torch.ops.sparc_b200
+
+
+_operators = {}
+
+
+def op(name: str):
+    """One operator of the library (its only overload, loaded on first use)."""
+    f = _operators.get(name)
+    if f is None:
+        f = _operators[name] = getattr(load(), name).default
+    return f
+
+
+def wait_status():
+    """The devices' status words of the operators' bounded waits (zero, or the bits of those that
+    ran out), as far as such operators have run."""
+    return op("wait_status")() if _operators else []
 
 
 _python_kernels = False

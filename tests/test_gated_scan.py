@@ -16,10 +16,15 @@ FAKE = 0x100000
 
 @pytest.fixture(scope="module")
 def L():
+    return _lib.load_library()
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
     from sparc_b200 import _build
 
     _build.build()
-    return _lib.load_library()
+    _build.build_torch_ops()
 
 
 def _message(L):

@@ -17,10 +17,15 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 @pytest.fixture(scope="module")
 def L():
+    return _lib.load_library()
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
     from sparc_b200 import _build
 
     _build.build()
-    return _lib.load_library()
+    _build.build_torch_ops()
 
 
 def _message(L):
