@@ -796,6 +796,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
 constexpr int kReduceRows = 8;
 __global__ void __launch_bounds__(kReduceRows * 32) gated_reduce_kernel(const double* part, float* out, int rows, int D) {
   __shared__ double s[kReduceRows][32];
+  pdl_wait();
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + lane;
   double t = 0.0;
@@ -1056,8 +1057,16 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
   cudaError_t e = gated_dispatch(p, mode, a->dtype, true, s);
   if (e == cudaSuccess) {
     TimedLaunch tl(kTimeGatedReduce, s);
-    gated_reduce_kernel<<<(p.D + 31) / 32, kReduceRows * 32, 0, s>>>(p.part, a->grad_nu_log, pl.rows * pl.cluster, p.D);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((p.D + 31) / 32));
+    cfg.blockDim = dim3(kReduceRows * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, gated_reduce_kernel, (const double*)p.part, a->grad_nu_log, pl.rows * pl.cluster, p.D);
   }
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
   return SPARC_OK;

@@ -35,6 +35,7 @@ struct ClipTensors {
   unsigned first[kClipTensors + 1];  // chunks before tensor i
   unsigned char bf16[kClipTensors];
   int n;
+  int single;  // every tensor is one chunk: chunk i is tensor i, with no search
 };
 
 struct ClipScale {
@@ -45,6 +46,7 @@ struct ClipScale {
 };
 
 __device__ __forceinline__ int clip_find(const ClipTensors& t, unsigned chunk) {
+  if (t.single) return (int)chunk;
   int lo = 0, hi = t.n;  // first[lo] <= chunk < first[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -185,6 +187,7 @@ __device__ __forceinline__ double clip_norm(const ClipScale& c, double* s) {
 
 __global__ void __launch_bounds__(kClipThreads) grad_norm_finish_kernel(const ClipScale c) {
   __shared__ double s[kClipThreads / 32];
+  pdl_wait();
   const double norm = clip_norm(c, s);
   if (threadIdx.x == 0) *c.norm = (float)norm;
 }
@@ -192,6 +195,7 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_finish_kernel(const Cl
 __global__ void __launch_bounds__(kClipThreads) grad_clip_kernel(const __grid_constant__ ClipTensors t,
                                                                  const __grid_constant__ ClipScale sc) {
   __shared__ double s[kClipThreads / 32];
+  pdl_wait();
   const double norm = clip_norm(sc, s);
   if (sc.norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *sc.norm = (float)norm;
   const double limit = norm + (double)sc.eps;
@@ -214,6 +218,21 @@ __global__ void __launch_bounds__(kClipThreads) grad_clip_kernel(const __grid_co
     }
     if (c < gridDim.x) break;
   }
+}
+
+// A launch that may start while the kernel before it drains (it waits for that kernel's sums itself).
+template <typename... P>
+static cudaError_t clip_launch(void (*kernel)(P...), unsigned grid, cudaStream_t s, const P&... params) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kClipThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, params...);
 }
 
 static int clip_launches(int tensors) { return std::max(1, (tensors + kClipTensors - 1) / kClipTensors); }
@@ -296,6 +315,7 @@ int sparc_grad_clip(const SparcGradClipArgs* a, void* stream) {
       t->first[t->n + 1] = t->first[t->n] + (unsigned)chunks;
       ++t->n;
     }
+    t->single = t->first[t->n] == (unsigned)t->n;
     return i;
   };
   cudaError_t e = cudaSuccess;
@@ -311,16 +331,14 @@ int sparc_grad_clip(const SparcGradClipArgs* a, void* stream) {
   }
   if (e == cudaSuccess && (a->out == nullptr || sc.parts == 0)) {
     TimedLaunch tl(kTimeGradClip, s);
-    grad_norm_finish_kernel<<<1, kClipThreads, 0, s>>>(sc);
-    e = cudaGetLastError();
+    e = clip_launch(grad_norm_finish_kernel, 1, s, sc);
   } else {
     for (int i = 0; i < a->tensors && e == cudaSuccess;) {
       i = fill(&t, i);
       if (t.n == 0) break;
       TimedLaunch tl(kTimeGradClip, s);
-      grad_clip_kernel<<<std::min<unsigned>(t.first[t.n], kClipGrid), kClipThreads, 0, s>>>(t, sc);
+      e = clip_launch(grad_clip_kernel, std::min<unsigned>(t.first[t.n], kClipGrid), s, t, sc);
       sc.norm = nullptr;
-      e = cudaGetLastError();
     }
   }
   if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
