@@ -333,7 +333,7 @@ __device__ __forceinline__ void polynomial(const float (&c)[DEG + 1], const floa
 // throughout the warp one of them goes: from rho = (1 + e^{-retention})^(-1/2) follow s(retention) =
 // rho^2 and beta = sqrt(nu) rho S(w), w = nu rho^2 = -u, where S(w) = sqrt((1 - e^{-2w}) / w) is smooth. S,
 // (1 - e^{-w}) / w and w / (e^{2w} - 1) are interpolated on [0, 1/2] by polynomials through the
-// Chebyshev points (relative errors 3e-9, 2e-9 and 2e-8).
+// Chebyshev points (relative errors 1.4e-7, 8e-8 and 2e-8).
 template <bool BWD, int N>
 struct GatedGates {
   float2 a[N], beta[N], sw[N], u[BWD ? N : 1], kappa[BWD ? N : 1], om_r[BWD ? N : 1], om_w[BWD ? N : 1];
@@ -343,8 +343,8 @@ __device__ __forceinline__ void gated_gates(const float2 (&r)[N], const float2 (
                                             GatedGates<BWD, N>& o) {
   float2 e[N], u[N];
   if constexpr (NEAR && sizeof(T) == 2) {
-    constexpr float kDecay[6] = {1.0f, -0.499999819f, 0.166662419f, -0.0416300728f, 0.00818961363f, -0.00112340422f};
-    constexpr float kRoot[6] = {1.41421356f, -0.707106332f, 0.294617291f, -0.0882973305f, 0.0190368337f, -0.00264261144f};
+    constexpr float kDecay[5] = {0.999999929f, -0.499992883f, 0.166551928f, -0.0410132105f, 0.00678286256f};
+    constexpr float kRoot[5] = {1.41421339f, -0.70709001f, 0.2943573f, -0.0868460191f, 0.0157274518f};
     float2 rho[N], y[N], v[N];
     exp_neg<T>(r, e);
 #pragma unroll
@@ -359,10 +359,10 @@ __device__ __forceinline__ void gated_gates(const float2 (&r)[N], const float2 (
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = mul2(nu, y[k]), u[k] = mul2(make_float2(-nu.x, -nu.y), y[k]);
-    polynomial<5>(kDecay, v, y);
+    polynomial<4>(kDecay, v, y);
 #pragma unroll
     for (int k = 0; k < N; ++k) o.a[k] = fma2(u[k], y[k], bcast2(1.0f));
-    polynomial<5>(kRoot, v, y);
+    polynomial<4>(kRoot, v, y);
 #pragma unroll
     for (int k = 0; k < N; ++k) o.beta[k] = mul2(y[k], mul2(rho[k], root_nu));
     if constexpr (BWD) {
@@ -856,16 +856,25 @@ struct GatedPlan {
   int groups, cluster, rows;
 };
 
-// 64 channels a cluster. The cluster grows (to the portable 8 CTAs, no further than the tiles
-// reach) until rows x channel groups x cluster fills the SMs four CTAs each; more rows than a few
-// waves of CTAs need are walked by the same clusters, which bounds the partial sums.
-static GatedPlan gated_plan(long long B, long long L, long long D, int tile) {
-  constexpr long long kFill = 148 * 4, kMost = kFill * 4;
+// 64 channels a cluster. A CTA's throughput does not depend on how many others share its sequence,
+// but their exchange costs (B=8 T=16384 D=2048 bf16, 256 rows x groups, backward: one CTA each 932 us,
+// clusters of eight 1017 us), and an SM with one CTA waits most of the time (one row of the same,
+// forward: clusters of one to eight 419, 249, 133, 95 us). So the cluster grows (to the portable 8
+// CTAs, no further than the tiles reach) until half the CTAs that are resident at once are there. More
+// rows than a few waves of CTAs need are walked by the same clusters, which bounds the partial sums.
+static GatedPlan gated_plan(long long B, long long L, long long D, bool backward, int dtype) {
+  constexpr long long kSms = 148, kMost = kSms * 16;
+  using bf16 = __nv_bfloat16;
+  const bool half = dtype == SPARC_DTYPE_BF16;
+  const int blocks = backward ? (half ? GatedBwdCut<bf16>::BLOCKS : GatedBwdCut<float>::BLOCKS)
+                              : (half ? GatedFwdCut<bf16>::BLOCKS : GatedFwdCut<float>::BLOCKS);
+  const int tile = backward ? kGatedChunk : half ? GatedFwdCut<bf16>::TILE : GatedFwdCut<float>::TILE;
   GatedPlan pl;
   pl.groups = (int)((D + 63) / 64);
   const long long tiles = (L + tile - 1) / tile;
   pl.cluster = 1;
-  while (pl.cluster < kGatedMaxCluster && pl.cluster * 2 <= tiles && B * pl.groups * pl.cluster < kFill) pl.cluster *= 2;
+  while (pl.cluster < kGatedMaxCluster && pl.cluster * 2 <= tiles && B * pl.groups * pl.cluster * 2 < kSms * blocks)
+    pl.cluster *= 2;
   const long long rows = std::max(1LL, kMost / ((long long)pl.groups * pl.cluster));
   pl.rows = (int)std::min(B, rows);
   return pl;
@@ -944,8 +953,12 @@ static cudaError_t gated_dispatch(const GatedParams& p, GatedMode mode, int dtyp
 }
 
 static size_t gated_ws_bytes(long long B, long long L, long long D) {
-  const GatedPlan pl = gated_plan(B, L, D, kGatedChunk);
-  return (size_t)pl.rows * (size_t)pl.cluster * (size_t)D * sizeof(double);
+  size_t rows = 0;  // of either type
+  for (int dtype : {SPARC_DTYPE_F32, SPARC_DTYPE_BF16}) {
+    const GatedPlan pl = gated_plan(B, L, D, true, dtype);
+    rows = std::max(rows, (size_t)pl.rows * (size_t)pl.cluster);
+  }
+  return rows * (size_t)D * sizeof(double);
 }
 
 }  // namespace sparc
@@ -995,7 +1008,7 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
   const GatedMode mode = gated_aligned(p.y, 2 * size) ? gated_mode(p, 3, size) : kModeSingle;
-  const GatedPlan pl = gated_plan(p.B, p.L, p.D, a->dtype == SPARC_DTYPE_BF16 ? GatedFwdCut<__nv_bfloat16>::TILE : GatedFwdCut<float>::TILE);
+  const GatedPlan pl = gated_plan(p.B, p.L, p.D, false, a->dtype);
   p.groups = pl.groups;
   p.cluster = pl.cluster;
   p.rows = pl.rows;
@@ -1049,7 +1062,7 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
     pairs = pairs && gated_aligned(q, 2 * size);
   }
   const GatedMode mode = pairs ? gated_mode(p, 4, size) : kModeSingle;
-  const GatedPlan pl = gated_plan(p.B, p.L, p.D, kGatedChunk);
+  const GatedPlan pl = gated_plan(p.B, p.L, p.D, true, a->dtype);
   p.groups = pl.groups;
   p.cluster = pl.cluster;
   p.rows = pl.rows;
