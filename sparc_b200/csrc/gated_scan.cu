@@ -35,7 +35,7 @@
 namespace sparc {
 
 constexpr int kGatedChunk = 32;  // tokens per saved carry
-constexpr int kGatedMaxCluster = 8;
+constexpr int kGatedMaxCluster = 16;  // (above 8 a kernel has to allow it)
 constexpr unsigned kGatedSpin = 1u << 22;  // default bound of a wait's polls (each may sleep in hardware)
 
 // How a CTA cuts its tile: WARPS spans of K tokens; BLOCKS CTAs per SM that the registers are held to.
@@ -83,8 +83,6 @@ template <> struct Duo<float> {
   using type = float2;
   static __device__ __forceinline__ float2 get(float2 v) { return v; }
   static __device__ __forceinline__ float2 make(float2 v) { return v; }
-  static __device__ __forceinline__ float2 join(float a, float b) { return make_float2(a, b); }
-  static __device__ __forceinline__ float bits(const float* p) { return __ldg(p); }
 };
 template <> struct Duo<__nv_bfloat16> {
   using type = unsigned;
@@ -94,12 +92,6 @@ template <> struct Duo<__nv_bfloat16> {
   static __device__ __forceinline__ unsigned make(float2 v) {
     const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
     return *reinterpret_cast<const unsigned*>(&b);
-  }
-  static __device__ __forceinline__ unsigned join(unsigned short a, unsigned short b) {
-    return (unsigned)a | (unsigned)b << 16;
-  }
-  static __device__ __forceinline__ unsigned short bits(const __nv_bfloat16* p) {
-    return __ldg(reinterpret_cast<const unsigned short*>(p));
   }
 };
 
@@ -112,9 +104,10 @@ __device__ __forceinline__ bool gated_starts(const void* pos, int bytes, long lo
   }
 }
 
-// How a warp reads its tokens: pieces of 16 bytes or of one pair of channels, copied to shared
-// memory ahead of their use, or single channels read where they are used (odd widths, strides or
-// bases, which no asynchronous copy of two bytes exists for).
+// How a warp reads its tokens, copied to shared memory ahead of their use: in pieces of 16 bytes, of
+// one pair of channels, or (odd widths, strides or bases) of four bytes. A bfloat16 token may then
+// begin in the middle of such a word: the words that hold its channels are copied as they lie, and a
+// lane joins its pair from two of them.
 enum GatedMode { kModeWide, kModePair, kModeSingle };
 
 template <int BYTES>
@@ -127,25 +120,28 @@ __device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A warp's reads of its next tokens: K of them a step, of NT tensors, into stage[tensor][token][lane].
+// What lies beyond the sequence or the channels is not copied: those values are never used.
 // Each lane owns pieces kRows tokens apart, and keeps a pointer per tensor that moves by a constant
-// from step to step. What lies beyond the sequence or the channels is not copied: those values are
-// never used.
+// from step to step (with single elements the warp's pointers are of the tokens' first channel).
 template <typename T, int MODE, int K, int NT>
 struct GatedReader {
   using R = typename Duo<T>::type;
   static constexpr int kBytes = MODE == kModeWide ? 16 : (int)sizeof(R);
   static constexpr int kPieces = 32 * (int)sizeof(R) / kBytes;  // of a token
-  static constexpr int kRows = 32 / kPieces;
+  static constexpr int kRows = MODE == kModeSingle ? 1 : 32 / kPieces;
+  static constexpr int kStride = MODE == kModeSingle && sizeof(T) == 2 ? 34 : 32;  // R from a token to the next
   const char* src[NT];
   long long row[NT], move[NT];  // bytes from a piece to the next, from a step to the next
-  unsigned dst;                 // this lane's first piece in a stage
-  int token;                    // and its token of the step (none of this lane's where its channels are beyond D)
+  R* stage;
+  unsigned dst;  // this lane's first piece in the stage
+  int token;     // and its token of the step (none of this lane's where its channels are beyond D)
+  int chans;     // single elements: channels of the token, up to 64
 
-  __device__ __forceinline__ GatedReader(const GatedParams& p, R* stage, int ch0, int lane, int tokens) {
-    if constexpr (MODE == kModeSingle) return;
+  __device__ __forceinline__ GatedReader(const GatedParams& p, R* stage_, int ch0, int lane, int tokens) : stage(stage_) {
     const int chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
     token = chan < p.D ? lane / kPieces : K;
-    dst = smem_addr(stage) + lane * kBytes;
+    chans = min(64, p.D - ch0);
+    dst = smem_addr(stage) + lane * (MODE == kModeSingle ? 4 : kBytes);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       row[n] = kRows * p.in[n].st * (int)sizeof(T);
@@ -153,17 +149,38 @@ struct GatedReader {
     }
   }
   __device__ __forceinline__ void start(const GatedParams& p, long long bt, int t0, int ch0, int lane) {
-    if constexpr (MODE == kModeSingle) return;
-    const int chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
+    const int chan = MODE == kModeSingle ? ch0 : ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
+    const int t = MODE == kModeSingle ? t0 : t0 + lane / kPieces;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      src[n] = reinterpret_cast<const char*>(static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb +
-                                             (long long)(t0 + lane / kPieces) * p.in[n].st + chan);
+      src[n] = reinterpret_cast<const char*>(static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + (long long)t * p.in[n].st + chan);
   }
+  // whether a bfloat16 token at `a` begins in the middle of a word
+  static __device__ __forceinline__ int odd(const char* a) { return (int)(reinterpret_cast<unsigned long long>(a) >> 1 & 1u); }
+
   // `left`: tokens of the sequence from this step's first on
-  __device__ __forceinline__ void copy(int left) {
-    if constexpr (MODE == kModeSingle) return;
-    if (left >= K) {
+  __device__ __forceinline__ void copy(int left, int lane) {
+    if constexpr (MODE == kModeSingle) {
+      // (rolled: these are many small copies, and code that runs once is paid for in instruction fetches)
+      const int some = min(K, left);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const char* a = src[n];
+        unsigned to = dst + n * K * kStride * (int)sizeof(R);
+#pragma unroll 1
+        for (int k = 0; k < some; ++k, a += row[n], to += kStride * (int)sizeof(R)) {
+          if constexpr (sizeof(T) == 2) {
+            const int o = odd(a);
+            const char* w = a - 2 * o + 4 * lane;
+            if (2 * lane - o < chans) copy_async<4>(to, w);
+            if (lane == 0 && 64 - o < chans) copy_async<4>(to + 128, w + 128);
+          } else {
+            if (lane < chans) copy_async<4>(to, a + 4 * lane);
+            if (lane + 32 < chans) copy_async<4>(to + 128, a + 128 + 4 * lane);
+          }
+        }
+      }
+    } else if (left >= K) {
       if (token < K) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -182,24 +199,20 @@ struct GatedReader {
 #pragma unroll
     for (int n = 0; n < NT; ++n) src[n] += move[n];
   }
-};
-
-template <typename T, int MODE, int K>
-__device__ __forceinline__ void gated_read(const GatedParams& p, int n, const typename Duo<T>::type* stage, long long bt,
-                                           int t0, int ch, int lane, typename Duo<T>::type* v) {
-  if constexpr (MODE != kModeSingle) {
+  // tokens k0 .. k0 + N - 1 of tensor n of the step that was copied last, once it has come
+  template <int N>
+  __device__ __forceinline__ void read(int n, int k0, int lane, R (&v)[N]) const {
+    const R* q = stage + (n * K + k0) * kStride + lane;
+    const int first = MODE == kModeSingle ? odd(src[n] - move[n]) + k0 * odd(reinterpret_cast<const char*>(row[n])) : 0;
+    const int next = MODE == kModeSingle ? odd(reinterpret_cast<const char*>(row[n])) : 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = stage[(n * K + k) * 32 + lane];
-  } else {
-    const T* base = static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + ch;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const bool ok = t0 + k < p.L;
-      const T* q = base + (long long)(t0 + k) * p.in[n].st;
-      v[k] = Duo<T>::join(ok && ch < p.D ? Duo<T>::bits(q) : 0, ok && ch + 1 < p.D ? Duo<T>::bits(q + 1) : 0);
+    for (int k = 0; k < N; ++k) {
+      v[k] = q[k * kStride];
+      if constexpr (MODE == kModeSingle && sizeof(T) == 2)
+        if (first + k * next & 1) v[k] = __funnelshift_r(v[k], q[k * kStride + 1], 16);
     }
   }
-}
+};
 
 template <typename T, int MODE>
 __device__ __forceinline__ void gated_store(T* o, int ch, int D, float2 v) {
@@ -449,12 +462,16 @@ __device__ __forceinline__ float4 cat4(float2 a, float2 b) { return make_float4(
 // CTA's. (A cluster barrier that releases the maps would wait for the warp's outputs on their way
 // to global memory too.) Buffers and barriers are of two parities: a CTA pushes step n + 2 after it
 // has step n + 1 from every CTA, which each pushed once all its warps were through with step n.
+__host__ __device__ constexpr int gated_map_bytes(int cs) { return cs > 1 ? 2 * cs * 32 * 16 : 0; }
+
 struct GatedExchange {
-  float4 map[2][kGatedMaxCluster][32];
-  unsigned long long bar[2];
+  float4* map;              // [2][CTAs of the cluster][32], at the same place in every CTA
+  unsigned long long* bar;  // [2]
+  int cs;
+  __device__ __forceinline__ float4* at(int par, int rank) const { return map + (par * cs + rank) * 32; }
 };
 
-__device__ __forceinline__ void exchange_init(GatedExchange& x) {
+__device__ __forceinline__ void exchange_init(const GatedExchange& x) {
   if (threadIdx.x == 0) {
     mbar_init(&x.bar[0], 1);
     mbar_init(&x.bar[1], 1);
@@ -463,12 +480,12 @@ __device__ __forceinline__ void exchange_init(GatedExchange& x) {
   // every CTA of the cluster has started, and its barriers stand, before anything is pushed
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void exchange_push(GatedExchange& x, unsigned n, int cs, int rank, int lane, float4 v) {
+__device__ __forceinline__ void exchange_push(const GatedExchange& x, unsigned n, int rank, int lane, float4 v) {
   const int par = n & 1;
-  if (lane == 0) mbar_arrive_expect_tx(&x.bar[par], (unsigned)cs * 32u * 16u);
-  for (int q = 0; q < cs; ++q)
+  if (lane == 0) mbar_arrive_expect_tx(&x.bar[par], (unsigned)x.cs * 32u * 16u);
+  for (int q = 0; q < x.cs; ++q)
     asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
-                     cluster_smem_addr(&x.map[par][rank][lane], q)),
+                     cluster_smem_addr(x.at(par, rank) + lane, q)),
                  "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(cluster_smem_addr(&x.bar[par], q))
                  : "memory");
 }
@@ -476,13 +493,13 @@ __device__ __forceinline__ void exchange_push(GatedExchange& x, unsigned n, int 
 template <bool SEG>
 __device__ __forceinline__ float2 exchange_through(const GatedExchange& x, int par, int q0, int q1, int d, int lane, float2 v) {
   for (; q0 != q1 && q0 + d != q1; q0 += 2 * d) {
-    const float4 m = x.map[par][q0][lane], n = x.map[par][q0 + d][lane];
+    const float4 m = x.at(par, q0)[lane], n = x.at(par, q0 + d)[lane];
     v = through<SEG>(lo2(n), hi2(n), through<SEG>(lo2(m), hi2(m), v));
   }
-  if (q0 != q1) v = through<SEG>(lo2(x.map[par][q0][lane]), hi2(x.map[par][q0][lane]), v);
+  if (q0 != q1) v = through<SEG>(lo2(x.at(par, q0)[lane]), hi2(x.at(par, q0)[lane]), v);
   return v;
 }
-__device__ __forceinline__ void exchange_wait(const GatedParams& p, GatedExchange& x, unsigned n) {
+__device__ __forceinline__ void exchange_wait(const GatedParams& p, const GatedExchange& x, unsigned n) {
   if (!mbar_wait_cluster(&x.bar[n & 1], n >> 1 & 1u, p.max_spin) && p.status != nullptr) atomicOr(p.status, kStatusTimeout);
 }
 
@@ -494,11 +511,14 @@ __device__ __forceinline__ unsigned gated_segments(const GatedParams& p, long lo
 }
 
 // ---------------------------------------------------------------- forward
+// A thread's tokens go through the gates four at a time (more take too many registers).
+constexpr int kGatedGroup = 4;
+
 template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
                                                  const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu,
                                                  float2 (&a)[K], float2 (&b)[K]) {
-  constexpr int N = 4;  // (more tokens at once take too many registers)
+  constexpr int N = kGatedGroup;
 #pragma unroll
   for (int k0 = 0; k0 < K; k0 += N) {
     float2 x[N], r[N], w[N];
@@ -514,9 +534,9 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   using R = typename Duo<T>::type;
   using C = GatedFwdCut<T>;
   constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 3;
-  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][tensor][token][lane]
+  extern __shared__ __align__(16) unsigned char s_raw[];  // the cluster's maps, then [warp][tensor][token][lane]
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
-  __shared__ GatedExchange s_cta;                         // and of each CTA of the cluster
+  __shared__ unsigned long long s_bar[2];
   __shared__ float2 s_out[2][32];                         // one CTA: the state leaving its tile
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
@@ -524,12 +544,13 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
   const bool on = ch < p.D;
   const int stride = cs * TILE;  // tokens from a step to the next
-  R* stage = reinterpret_cast<R*>(s_raw) + wp * NT * K * 32;
+  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, H) of each CTA
+  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * NT * K * GatedReader<T, MODE, K, NT>::kStride;
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, stride);
-  if (cs > 1) exchange_init(s_cta);
+  if (cs > 1) exchange_init(peers);
   unsigned n = 0;  // steps so far
 
   for (long long bt = id / (unsigned)p.groups; bt < p.B; bt += p.rows) {
@@ -537,23 +558,22 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
     float2 carry = load_pair(p.h0, bt * p.D + ch, ch, p.D);  // the state entering the step
     T* y = static_cast<T*>(p.y) + (bt * p.L + rank * TILE) * p.D;  // of the CTA's first token and channel
     reader.start(p, bt, t0, ch0, lane);
-    reader.copy(p.L - t0);
+    reader.copy(p.L - t0, lane);
     for (int first = 0; first < p.L; first += stride, t0 += stride, ++n) {
       const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
-      if constexpr (MODE != kModeSingle) {
-        copy_wait();
-        __syncwarp();
-      }
+      copy_wait();
+      __syncwarp();
       float2 a[K], b[K], A = bcast2(1.0f), H = bcast2(0.0f);
       const int live = p.L - t0;  // tokens of the sequence from here on
       {
         R rx[K], rr[K], rw[K];
-        gated_read<T, MODE, K>(p, 0, stage, bt, t0, ch, lane, rx);
-        gated_read<T, MODE, K>(p, 1, stage, bt, t0, ch, lane, rr);
-        gated_read<T, MODE, K>(p, 2, stage, bt, t0, ch, lane, rw);
+        reader.read(0, 0, lane, rx);
+        reader.read(1, 0, lane, rr);
+        reader.read(2, 0, lane, rw);
         __syncwarp();  // every lane has read its values
-        reader.copy(live - stride);
+        reader.copy(live - stride, lane);
+        // (also of warps beyond the sequence: a condition here makes the others spill, and costs 8%)
         if (near) gated_fwd_tokens<T, true>(rx, rr, rw, nu, root_nu, a, b);
         else gated_fwd_tokens<T, false>(rx, rr, rw, nu, root_nu, a, b);
       }
@@ -577,11 +597,11 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
           A = bcast2(1.0f), H = bcast2(0.0f);
 #pragma unroll
           for (int j = 0; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]));
-          exchange_push(s_cta, n, cs, rank, lane, cat4(A, H));
+          exchange_push(peers, n, rank, lane, cat4(A, H));
         }
-        exchange_wait(p, s_cta, n);
-        h = exchange_through<SEG>(s_cta, par, 0, rank, 1, lane, carry);
-        carry = exchange_through<SEG>(s_cta, par, rank, cs, 1, lane, h);
+        exchange_wait(p, peers, n);
+        h = exchange_through<SEG>(peers, par, 0, rank, 1, lane, carry);
+        carry = exchange_through<SEG>(peers, par, rank, cs, 1, lane, h);
       } else {
         h = first == 0 ? carry : s_out[par ^ 1][lane];
       }
@@ -618,11 +638,12 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
 // the adjoints are there, g, b (1 - s(write)) and 1 - s(retention).
 template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_bwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
-                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu, float2* put,
-                                                 float2 (&f)[K], float2 (&b)[K], float2 (&q1)[K], float2 (&q2)[K]) {
-  constexpr int N = 4;
+                                                 const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu, int live,
+                                                 float2* put, float2 (&f)[K], float2 (&b)[K], float2 (&q1)[K], float2 (&q2)[K]) {
+  constexpr int N = kGatedGroup;
 #pragma unroll
   for (int k0 = 0; k0 < K; k0 += N) {
+    if (k0 >= live) continue;
     float2 r[N], w[N];
     GatedGates<true, N> o;
 #pragma unroll
@@ -648,10 +669,10 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   using R = typename Duo<T>::type;
   using C = GatedBwdCut<T>;
   constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 4;
-  extern __shared__ __align__(16) unsigned char s_raw[];  // [warp][token][3][lane] put by, then the inputs
+  extern __shared__ __align__(16) unsigned char s_raw[];  // the cluster's maps, [warp][token][3][lane] put by, the inputs
   __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
-  __shared__ GatedExchange s_cta;                    // (A, G) of each CTA of the cluster
+  __shared__ unsigned long long s_bar[2];
   __shared__ float2 s_out[2][32];                    // one CTA: the adjoint leaving its tile
   __shared__ double2 s_nu[NW][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
@@ -660,13 +681,14 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
   const bool on = ch < p.D;
   const int stride = cs * TILE, steps = (p.chunks + cs - 1) / cs;
-  float2* put = reinterpret_cast<float2*>(s_raw) + wp * K * 96 + lane;
-  R* stage = reinterpret_cast<R*>(s_raw + NW * K * 96 * sizeof(float2)) + wp * NT * K * 32;
+  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, G) of each CTA
+  float2* put = reinterpret_cast<float2*>(s_raw + gated_map_bytes(cs)) + wp * K * 96 + lane;
+  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * NT * K * GatedReader<T, MODE, K, NT>::kStride;
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
   GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, -stride);
-  if (cs > 1) exchange_init(s_cta);
+  if (cs > 1) exchange_init(peers);
   unsigned n = 0;  // steps so far
   double dnu_x = 0.0, dnu_y = 0.0;
 
@@ -675,29 +697,27 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     float2 carry = load_pair(p.grad_last, bt * p.D + ch, ch, p.D);  // c_{t+1} lam_{t+1} entering the step's last token
     long long base = (bt * p.L + (long long)tile * TILE) * p.D;     // of the CTA's first token and channel in the gradients
     reader.start(p, bt, t0, ch0, lane);
-    reader.copy(p.L - t0);
+    reader.copy(p.L - t0, lane);
     for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, ++n) {
       const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
       // the state entering this CTA's tile
       float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (bt * p.chunks + tile) * p.D + ch, ch, p.D);
-      if constexpr (MODE != kModeSingle) {
-        copy_wait();
-        __syncwarp();
-      }
+      copy_wait();
+      __syncwarp();
       const int live = p.L - t0;
       float2 f[K], b[K], q1[K], q2[K], A = bcast2(1.0f), H = bcast2(0.0f), G = bcast2(0.0f);
       R rd[K];
       {
         R rx[K], rr[K], rw[K];
-        gated_read<T, MODE, K>(p, 0, stage, bt, t0, ch, lane, rx);
-        gated_read<T, MODE, K>(p, 1, stage, bt, t0, ch, lane, rr);
-        gated_read<T, MODE, K>(p, 2, stage, bt, t0, ch, lane, rw);
-        gated_read<T, MODE, K>(p, 3, stage, bt, t0, ch, lane, rd);
+        reader.read(0, 0, lane, rx);
+        reader.read(1, 0, lane, rr);
+        reader.read(2, 0, lane, rw);
+        reader.read(3, 0, lane, rd);
         __syncwarp();
-        reader.copy(step > 0 ? live + stride : 0);
-        if (near) gated_bwd_tokens<T, true>(rx, rr, rw, nu, root_nu, put, f, b, q1, q2);
-        else gated_bwd_tokens<T, false>(rx, rr, rw, nu, root_nu, put, f, b, q1, q2);
+        reader.copy(step > 0 ? live + stride : 0, lane);
+        if (near) gated_bwd_tokens<T, true>(rx, rr, rw, nu, root_nu, live, put, f, b, q1, q2);
+        else gated_bwd_tokens<T, false>(rx, rr, rw, nu, root_nu, live, put, f, b, q1, q2);
       }
       if (SEG && seg != 0) {
 #pragma unroll
@@ -723,7 +743,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
             if (i == NW - 1) A = lo2(s_map[par][i][lane]), G = s_adj[par][i][lane];
             else compose<SEG>(A, G, lo2(s_map[par][i][lane]), s_adj[par][i][lane]);
           }
-          exchange_push(s_cta, n, cs, rank, lane, cat4(A, G));
+          exchange_push(peers, n, rank, lane, cat4(A, G));
         }
       }
 #pragma unroll
@@ -738,9 +758,9 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       }
       float2 c;  // the adjoint entering this CTA's tile, then this warp's tokens
       if (cs > 1) {
-        exchange_wait(p, s_cta, n);
-        c = exchange_through<SEG>(s_cta, par, cs - 1, rank, -1, lane, carry);
-        carry = exchange_through<SEG>(s_cta, par, rank, -1, -1, lane, c);
+        exchange_wait(p, peers, n);
+        c = exchange_through<SEG>(peers, par, cs - 1, rank, -1, lane, carry);
+        carry = exchange_through<SEG>(peers, par, rank, -1, -1, lane, c);
       } else {
         c = step == steps - 1 ? carry : s_out[par ^ 1][lane];
       }
@@ -859,8 +879,10 @@ struct GatedPlan {
 // 64 channels a cluster. A CTA's throughput does not depend on how many others share its sequence,
 // but their exchange costs (B=8 T=16384 D=2048 bf16, 256 rows x groups, backward: one CTA each 932 us,
 // clusters of eight 1017 us), and an SM with one CTA waits most of the time (one row of the same,
-// forward: clusters of one to eight 419, 249, 133, 95 us). So the cluster grows (to the portable 8
-// CTAs, no further than the tiles reach) until half the CTAs that are resident at once are there. More
+// forward: clusters of one to eight 419, 249, 133, 95 us). So the cluster grows, no further than the
+// tiles reach, until half the CTAs that are resident at once are there; to 16 CTAs only where eight
+// would leave SMs without one (3 rows T=24864 D=90, six rows x groups: 144 -> 89 us and backward 200 ->
+// 118 us; but the one row of 32 groups above 95 -> 121 us). More
 // rows than a few waves of CTAs need are walked by the same clusters, which bounds the partial sums.
 static GatedPlan gated_plan(long long B, long long L, long long D, bool backward, int dtype) {
   constexpr long long kSms = 148, kMost = kSms * 16;
@@ -873,7 +895,8 @@ static GatedPlan gated_plan(long long B, long long L, long long D, bool backward
   pl.groups = (int)((D + 63) / 64);
   const long long tiles = (L + tile - 1) / tile;
   pl.cluster = 1;
-  while (pl.cluster < kGatedMaxCluster && pl.cluster * 2 <= tiles && B * pl.groups * pl.cluster * 2 < kSms * blocks)
+  while (pl.cluster < kGatedMaxCluster && pl.cluster * 2 <= tiles &&
+         B * pl.groups * pl.cluster * 2 < (pl.cluster < 8 ? kSms * blocks : 2 * kSms))
     pl.cluster *= 2;
   const long long rows = std::max(1LL, kMost / ((long long)pl.groups * pl.cluster));
   pl.rows = (int)std::min(B, rows);
@@ -909,15 +932,16 @@ static GatedMode gated_mode(const GatedParams& p, int inputs, int size) {
 
 template <typename T, bool SEG, int MODE>
 static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_t s) {
-  constexpr int kRow = 32 * (int)sizeof(typename Duo<T>::type);
   using F = GatedFwdCut<T>;
   using W = GatedBwdCut<T>;
-  const int staged = MODE == kModeSingle ? 0 : backward ? W::TILE * 4 * kRow : F::TILE * 3 * kRow;
-  const int smem = staged + (backward ? W::TILE * 96 * (int)sizeof(float2) : 0);
+  constexpr int kRow = GatedReader<T, MODE, F::K, 3>::kStride * (int)sizeof(typename Duo<T>::type);
+  const int smem = gated_map_bytes(p.cluster) + (backward ? W::TILE * (4 * kRow + 96 * (int)sizeof(float2)) : F::TILE * 3 * kRow);
   const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
-  if (smem > 0) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  if (p.cluster > 8) {
+    const cudaError_t wide = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (wide != cudaSuccess) return wide;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.groups * (unsigned)p.rows * (unsigned)p.cluster);
