@@ -105,9 +105,8 @@ __device__ __forceinline__ bool gated_starts(const void* pos, int bytes, long lo
 }
 
 // How a warp reads its tokens, copied to shared memory ahead of their use: in pieces of 16 bytes, of
-// one pair of channels, or (odd widths, strides or bases) of four bytes. A bfloat16 token may then
-// begin in the middle of such a word: the words that hold its channels are copied as they lie, and a
-// lane joins its pair from two of them.
+// one pair of channels, or (odd widths, strides or bases) in the aligned 16-byte pieces that hold the
+// token's channels, from the middle of which the lanes then read.
 enum GatedMode { kModeWide, kModePair, kModeSingle };
 
 template <int BYTES>
@@ -129,19 +128,20 @@ struct GatedReader {
   static constexpr int kBytes = MODE == kModeWide ? 16 : (int)sizeof(R);
   static constexpr int kPieces = 32 * (int)sizeof(R) / kBytes;  // of a token
   static constexpr int kRows = MODE == kModeSingle ? 1 : 32 / kPieces;
-  static constexpr int kStride = MODE == kModeSingle && sizeof(T) == 2 ? 34 : 32;  // R from a token to the next
+  static constexpr int kWindow = 64 * (int)sizeof(T) / 16 + 1;                      // aligned pieces of an odd token
+  static constexpr int kRowBytes = MODE == kModeSingle ? kWindow * 16 : 32 * (int)sizeof(R);  // of a token in the stage
   const char* src[NT];
   long long row[NT], move[NT];  // bytes from a piece to the next, from a step to the next
   R* stage;
   unsigned dst;  // this lane's first piece in the stage
   int token;     // and its token of the step (none of this lane's where its channels are beyond D)
-  int chans;     // single elements: channels of the token, up to 64
+  int bytes;     // odd tokens: of the token's channels
 
   __device__ __forceinline__ GatedReader(const GatedParams& p, R* stage_, int ch0, int lane, int tokens) : stage(stage_) {
     const int chan = ch0 + lane % kPieces * (kBytes / (int)sizeof(T));
     token = chan < p.D ? lane / kPieces : K;
-    chans = min(64, p.D - ch0);
-    dst = smem_addr(stage) + lane * (MODE == kModeSingle ? 4 : kBytes);
+    bytes = min(64, p.D - ch0) * (int)sizeof(T);
+    dst = smem_addr(stage) + (MODE == kModeSingle ? 0 : lane * kBytes);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       row[n] = kRows * p.in[n].st * (int)sizeof(T);
@@ -155,29 +155,19 @@ struct GatedReader {
     for (int n = 0; n < NT; ++n)
       src[n] = reinterpret_cast<const char*>(static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + (long long)t * p.in[n].st + chan);
   }
-  // whether a bfloat16 token at `a` begins in the middle of a word
-  static __device__ __forceinline__ int odd(const char* a) { return (int)(reinterpret_cast<unsigned long long>(a) >> 1 & 1u); }
-
   // `left`: tokens of the sequence from this step's first on
   __device__ __forceinline__ void copy(int left, int lane) {
     if constexpr (MODE == kModeSingle) {
-      // (rolled: these are many small copies, and code that runs once is paid for in instruction fetches)
+      // (rolled: code that runs once is paid for in instruction fetches)
       const int some = min(K, left);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const char* a = src[n];
-        unsigned to = dst + n * K * kStride * (int)sizeof(R);
 #pragma unroll 1
-        for (int k = 0; k < some; ++k, a += row[n], to += kStride * (int)sizeof(R)) {
-          if constexpr (sizeof(T) == 2) {
-            const int o = odd(a);
-            const char* w = a - 2 * o + 4 * lane;
-            if (2 * lane - o < chans) copy_async<4>(to, w);
-            if (lane == 0 && 64 - o < chans) copy_async<4>(to + 128, w + 128);
-          } else {
-            if (lane < chans) copy_async<4>(to, a + 4 * lane);
-            if (lane + 32 < chans) copy_async<4>(to + 128, a + 128 + 4 * lane);
-          }
+      for (int c = lane; c < some * kWindow; c += 32) {
+        const int k = c / kWindow, at = c % kWindow * 16;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const char* a = src[n] + k * row[n];
+          const int off = (int)(reinterpret_cast<unsigned long long>(a) & 15u);
+          if (at - off < bytes) copy_async<16>(dst + n * K * kRowBytes + c * 16, a - off + at);
         }
       }
     } else if (left >= K) {
@@ -202,14 +192,23 @@ struct GatedReader {
   // tokens k0 .. k0 + N - 1 of tensor n of the step that was copied last, once it has come
   template <int N>
   __device__ __forceinline__ void read(int n, int k0, int lane, R (&v)[N]) const {
-    const R* q = stage + (n * K + k0) * kStride + lane;
-    const int first = MODE == kModeSingle ? odd(src[n] - move[n]) + k0 * odd(reinterpret_cast<const char*>(row[n])) : 0;
-    const int next = MODE == kModeSingle ? odd(reinterpret_cast<const char*>(row[n])) : 0;
+    const char* q = reinterpret_cast<const char*>(stage) + (n * K + k0) * kRowBytes + lane * (int)sizeof(R);
+    const unsigned step = (unsigned)row[n], first = (unsigned)reinterpret_cast<unsigned long long>(src[n] - move[n]) + k0 * step;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      v[k] = q[k * kStride];
-      if constexpr (MODE == kModeSingle && sizeof(T) == 2)
-        if (first + k * next & 1) v[k] = __funnelshift_r(v[k], q[k * kStride + 1], 16);
+      const char* w = q + k * kRowBytes;
+      if constexpr (MODE != kModeSingle) {
+        v[k] = *reinterpret_cast<const R*>(w);
+      } else {
+        const unsigned off = first + k * step & 15u;  // where the token begins in its first piece
+        if constexpr (sizeof(T) == 2) {
+          const unsigned* u = reinterpret_cast<const unsigned*>(w + (off & ~3u));
+          v[k] = off & 2u ? __funnelshift_r(u[0], u[1], 16) : u[0];
+        } else {
+          const float* f = reinterpret_cast<const float*>(w + off);
+          v[k] = make_float2(f[0], f[1]);
+        }
+      }
     }
   }
 };
@@ -545,7 +544,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const bool on = ch < p.D;
   const int stride = cs * TILE;  // tokens from a step to the next
   const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, H) of each CTA
-  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * NT * K * GatedReader<T, MODE, K, NT>::kStride;
+  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * NT * K * (GatedReader<T, MODE, K, NT>::kRowBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
@@ -683,7 +682,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const int stride = cs * TILE, steps = (p.chunks + cs - 1) / cs;
   const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, G) of each CTA
   float2* put = reinterpret_cast<float2*>(s_raw + gated_map_bytes(cs)) + wp * K * 96 + lane;
-  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * NT * K * GatedReader<T, MODE, K, NT>::kStride;
+  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * NT * K * (GatedReader<T, MODE, K, NT>::kRowBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
@@ -934,7 +933,7 @@ template <typename T, bool SEG, int MODE>
 static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_t s) {
   using F = GatedFwdCut<T>;
   using W = GatedBwdCut<T>;
-  constexpr int kRow = GatedReader<T, MODE, F::K, 3>::kStride * (int)sizeof(typename Duo<T>::type);
+  constexpr int kRow = GatedReader<T, MODE, F::K, 3>::kRowBytes;
   const int smem = gated_map_bytes(p.cluster) + (backward ? W::TILE * (4 * kRow + 96 * (int)sizeof(float2)) : F::TILE * 3 * kRow);
   const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
