@@ -4,10 +4,11 @@
 //
 // Both directions read every activation once: a row lives in the registers of one warp, or of one
 // CTA where it is wider, as NV vectors of VEC elements a thread (16 bytes where width, strides and
-// bases allow it, else single elements). CTAs walk the rows; of the 16-byte vectors each thread keeps
-// its share of the next kLnRing rows on the way into shared memory by asynchronous copies that only
-// it waits for (two rows in registers leave HBM a third idle), of single elements the next row in
-// registers. The statistics are exact two-step ones: each warp's mean,
+// bases allow it, else single elements). CTAs walk the rows and keep the next few on the way into
+// shared memory by asynchronous copies (two rows in registers leave HBM a third idle): of 16-byte
+// vectors each thread copies and waits for its own; rows that begin anywhere come in the aligned
+// 16-byte pieces that hold them, and every thread takes its elements once all pieces are there. The
+// statistics are exact two-step ones: each warp's mean,
 // then its squared deviations about that mean, joined over the warps with one barrier by
 //   mean = sum n_i mean_i / n,  M = sum M_i + n_i (mean_i - mean)^2,
 // so no sum of squares about zero cancels. In the backward a thread keeps the
@@ -117,57 +118,73 @@ struct LnRow {
   }
 };
 
-// A thread's share of the next rows of NT tensors: up to kLnRing of them in shared memory, slot by
-// slot, as far as kLnRingBytes a CTA go, or (single elements) one in registers. Rows are asked for in
-// order, one for each that is taken.
+// The next rows of NT tensors on their way into shared memory, slot by slot: up to kLnRing of them, as
+// far as kLnRingBytes a CTA go. Rows are asked for in order, one for each that is taken.
 constexpr int kLnRing = 4, kLnRingBytes = 96 * 1024;
 template <typename T, int VEC, int NV, int WARPS, int NT>
 struct LnAhead {
   using Row = LnRow<T, VEC, NV, WARPS>;
   using R = typename LnVec<T, VEC>::type;
-  static constexpr bool kRing = VEC > 1;
-  static constexpr int kRowBytes = NT * NV * 16 * kLnThreads<WARPS>;
-  static constexpr int kDepth = kRing ? std::min(kLnRing, kLnRingBytes / kRowBytes) : 1;
-  static constexpr int kBytes = kRing ? kDepth * kRowBytes : 0;
+  static constexpr bool kVectors = VEC > 1;
+  static constexpr int kRows = WARPS == 1 ? kLnRows : 1;  // of a CTA at a time
+  // of one tensor's row in a slot: the threads' vectors, or the row with the rest of its outer pieces
+  static constexpr int kTensorBytes = 32 * WARPS * NV * VEC * (int)sizeof(T) + (kVectors ? 0 : 16);
+  static constexpr int kSlotBytes = NT * kTensorBytes;
+  static constexpr int kDepth = std::min(kLnRing, kLnRingBytes / (kSlotBytes * kRows));
+  static constexpr int kBytes = kDepth * kSlotBytes * kRows;
   static_assert(kDepth >= 1);
-  R raw[kRing ? 1 : NT][NV];
-  R* mine;  // [slot][tensor][vector][thread]
-  int slot;
+  unsigned char* mine;  // [slot][tensor], of this thread's row
+  int i, slot;          // the thread's number among the row's; the slot asked for next
 
-  __device__ __forceinline__ explicit LnAhead(unsigned char* ring) : mine(reinterpret_cast<R*>(ring) + threadIdx.x), slot(0) {}
-  // tensor n's row at `q` (this thread's first column); none where not `valid`
-  __device__ __forceinline__ void ask(int n, const T* q, bool valid, int c0, int W) {
+  __device__ __forceinline__ explicit LnAhead(unsigned char* ring)
+      : mine(ring + (WARPS == 1 ? (threadIdx.x >> 5) * kDepth * kSlotBytes : 0)),
+        i(WARPS == 1 ? (int)(threadIdx.x & 31) : (int)threadIdx.x), slot(0) {}
+
+  // tensor n's row at `q`
+  __device__ __forceinline__ void ask(int n, const T* q, int W) {
+    unsigned char* to = mine + slot * kSlotBytes + n * kTensorBytes;
+    if constexpr (kVectors) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (valid && c0 + j * Row::kStep < W) {
-        if constexpr (kRing)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                           smem_addr(mine + ((slot * NT + n) * NV + j) * kLnThreads<WARPS>)),
-                       "l"(q + j * Row::kStep)
-                       : "memory");
-        else
-          raw[n][j] = __ldg(reinterpret_cast<const R*>(q + j * Row::kStep));
-      }
+      for (int j = 0; j < NV; ++j)
+        if (i * VEC + j * Row::kStep < W) copy(to + (j * 32 * WARPS + i) * 16, q + i * VEC + j * Row::kStep);
+    } else {
+      const char* a = reinterpret_cast<const char*>(q);
+      const int off = (int)(reinterpret_cast<unsigned long long>(a) & 15u), end = off + W * (int)sizeof(T);
+      for (int at = i * 16; at < end; at += 32 * WARPS * 16) copy(to + at, a - off + at);
+    }
+  }
+  static __device__ __forceinline__ void copy(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
   }
   __device__ __forceinline__ void asked() {  // the row's tensors are complete
-    if constexpr (kRing) {
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      slot = slot + 1 == kDepth ? 0 : slot + 1;
-    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
   }
   // with kDepth rows asked for and not taken, the first of them has come (its slot is the next one asked for)
   __device__ __forceinline__ void wait() {
-    if constexpr (kRing) asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    if constexpr (!kVectors) {
+      if constexpr (WARPS == 1) __syncwarp();
+      else __syncthreads();
+    }
   }
-  __device__ __forceinline__ void take(int n, int c0, int W, float (&f)[NV * VEC]) {
-    if constexpr (kRing) {
+  __device__ __forceinline__ void take(int n, const T* q, int W, float (&f)[NV * VEC]) {
+    const unsigned char* from = mine + slot * kSlotBytes + n * kTensorBytes;
+    if constexpr (kVectors) {
       R v[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) v[j] = mine[((slot * NT + n) * NV + j) * kLnThreads<WARPS>];
-      Row::get(v, c0, W, f);
+      for (int j = 0; j < NV; ++j) v[j] = reinterpret_cast<const R*>(from)[j * 32 * WARPS + i];
+      Row::get(v, i * VEC, W, f);
     } else {
-      Row::get(raw[n], c0, W, f);
+      const T* e = reinterpret_cast<const T*>(from + (reinterpret_cast<unsigned long long>(q) & 15u));
+#pragma unroll
+      for (int j = 0; j < NV; ++j) f[j] = j * 32 * WARPS + i < W ? to_float(e[j * 32 * WARPS + i]) : 0.0f;
     }
+  }
+  // Between a row's last take and the next ask, which writes its slot: every thread has taken it. (With
+  // several warps a row, the barrier of the row's sums stands between the two.)
+  __device__ __forceinline__ void taken() {
+    if constexpr (!kVectors && WARPS == 1) __syncwarp();
   }
 };
 
@@ -196,7 +213,7 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_fwd_kernel(const LnParam
   using Ahead = LnAhead<T, VEC, NV, WARPS, 1>;
   Ahead ahead(s_ring);
   auto ask = [&](long long r) {
-    ahead.ask(0, static_cast<const T*>(p.x) + r * p.sx + c0, r < p.R, c0, p.W);
+    if (r < p.R) ahead.ask(0, static_cast<const T*>(p.x) + r * p.sx, p.W);
     ahead.asked();
   };
 #pragma unroll
@@ -208,8 +225,9 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_fwd_kernel(const LnParam
   for (long long r = first; r < p.R; r += step, par ^= 1) {
     float x[E], sum = 0.0f, m2 = 0.0f;
     ahead.wait();
-    ahead.take(0, c0, p.W, x);
-    ask(r + Ahead::kDepth * step);
+    ahead.take(0, static_cast<const T*>(p.x) + r * p.sx, p.W, x);
+    ahead.taken();
+    if (Ahead::kVectors || WARPS == 1) ask(r + Ahead::kDepth * step);
 #pragma unroll
     for (int k = 0; k < E; ++k) sum += x[k];
     float mean = warp_sum(sum) * inv_count;
@@ -226,6 +244,7 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_fwd_kernel(const LnParam
     if constexpr (WARPS > 1) {
       if (lane == 0) s_stat[par][wp] = make_float4(mean, m2, count, 0.0f);
       __syncthreads();
+      if (!Ahead::kVectors) ask(r + Ahead::kDepth * step);
       float all = 0.0f;
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) all = fmaf(s_stat[par][k].z, s_stat[par][k].x, all);
@@ -263,8 +282,10 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_bwd_kernel(const LnParam
   using Ahead = LnAhead<T, VEC, NV, WARPS, 2>;
   Ahead ahead(s_ring);
   auto ask = [&](long long r) {
-    ahead.ask(0, static_cast<const T*>(p.x) + r * p.sx + c0, r < p.R, c0, p.W);
-    ahead.ask(1, static_cast<const T*>(p.dy) + r * p.sdy + c0, r < p.R, c0, p.W);
+    if (r < p.R) {
+      ahead.ask(0, static_cast<const T*>(p.x) + r * p.sx, p.W);
+      ahead.ask(1, static_cast<const T*>(p.dy) + r * p.sdy, p.W);
+    }
     ahead.asked();
   };
 #pragma unroll
@@ -279,9 +300,10 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_bwd_kernel(const LnParam
   for (long long r = first; r < p.R; r += step, par ^= 1) {
     float n[E], d[E], s1 = 0.0f, s2 = 0.0f;
     ahead.wait();
-    ahead.take(0, c0, p.W, n);
-    ahead.take(1, c0, p.W, d);
-    ask(r + Ahead::kDepth * step);
+    ahead.take(0, static_cast<const T*>(p.x) + r * p.sx, p.W, n);
+    ahead.take(1, static_cast<const T*>(p.dy) + r * p.sdy, p.W, d);
+    ahead.taken();
+    if (Ahead::kVectors || WARPS == 1) ask(r + Ahead::kDepth * step);
     mean = next_mean;
     rstd = next_rstd;
     if (r + step < p.R) next_mean = __ldg(p.mean + r + step), next_rstd = __ldg(p.rstd + r + step);
@@ -299,6 +321,7 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_bwd_kernel(const LnParam
     if constexpr (WARPS > 1) {
       if (lane == 0) s_sum[par][wp] = make_float2(s1, s2);
       __syncthreads();
+      if (!Ahead::kVectors) ask(r + Ahead::kDepth * step);
       s1 = s2 = 0.0f;
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) s1 += s_sum[par][k].x, s2 += s_sum[par][k].y;
@@ -365,9 +388,11 @@ __global__ void __launch_bounds__(kLnWide) ln_wide_fwd_kernel(const LnParams p) 
   for (long long r = blockIdx.x; r < p.R; r += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + r * p.sx;
     float sum = 0.0f;
+#pragma unroll 4
     for (int c = threadIdx.x; c < p.W; c += kLnWide) sum += Io<T>::load(x + c);
     float mean = block_sum(sum, s) * inv_w;
     float m2 = 0.0f, m1 = 0.0f;
+#pragma unroll 4
     for (int c = threadIdx.x; c < p.W; c += kLnWide) {
       const float d = Io<T>::load(x + c) - mean;
       m1 += d;
@@ -378,6 +403,7 @@ __global__ void __launch_bounds__(kLnWide) ln_wide_fwd_kernel(const LnParams p) 
     const float var = block_sum(m2, s) * inv_w - off * off, rstd = 1.0f / sqrtf(var + p.eps);
     mean += off;
     if (threadIdx.x == 0 && p.mean != nullptr) p.mean[r] = mean, p.rstd[r] = rstd;
+#pragma unroll 4
     for (int c = threadIdx.x; c < p.W; c += kLnWide) {
       const float n = (Io<T>::load(x + c) - mean) * rstd;
       Io<T>::store(static_cast<T*>(p.out) + r * p.W + c, p.b != nullptr ? fmaf(n, p.w[c], p.b[c]) : n * p.w[c]);
@@ -394,6 +420,7 @@ __global__ void __launch_bounds__(kLnWide) ln_wide_bwd_kernel(const LnParams p) 
     const T* dy = static_cast<const T*>(p.dy) + r * p.sdy;
     const float mean = p.mean[r], rstd = p.rstd[r];
     float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll 4
     for (int c = threadIdx.x; c < p.W; c += kLnWide) {
       const float d = Io<T>::load(dy + c) * p.w[c];
       s1 += d;
@@ -401,6 +428,7 @@ __global__ void __launch_bounds__(kLnWide) ln_wide_bwd_kernel(const LnParams p) 
     }
     s1 = block_sum(s1, s) * inv_w;
     s2 = block_sum(s2, s) * inv_w;
+#pragma unroll 4
     for (int c = threadIdx.x; c < p.W; c += kLnWide) {
       const float n = (Io<T>::load(x + c) - mean) * rstd;
       Io<T>::store(static_cast<T*>(p.out) + r * p.W + c, rstd * (Io<T>::load(dy + c) * p.w[c] - s1 - n * s2));
@@ -414,6 +442,7 @@ __global__ void __launch_bounds__(256) ln_wide_cols_kernel(const LnParams p) {
   const int c = blockIdx.y * 256 + threadIdx.x;
   if (c >= p.W) return;
   float dw = 0.0f, db = 0.0f;
+#pragma unroll 4
   for (long long r = blockIdx.x; r < p.R; r += gridDim.x) {
     const float d = Io<T>::load(static_cast<const T*>(p.dy) + r * p.sdy + c);
     dw = fmaf(d, (Io<T>::load(static_cast<const T*>(p.x) + r * p.sx + c) - p.mean[r]) * p.rstd[r], dw);
@@ -523,7 +552,8 @@ template <typename T>
 static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, bool backward, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   if (pl.warps == 0) {
-    *grid = (int)std::min<long long>(p.R, kLnSumGrid);
+    // (fewer rows of column sums than rows: each is worth four rows at least)
+    *grid = (int)std::min<long long>(backward ? (p.R + 3) / 4 : p.R, kLnSms * 2);
     TimedLaunch tl(backward ? kTimeLnBwd : kTimeLnFwd, s);
     if (!backward) {
       ln_wide_fwd_kernel<T><<<*grid, kLnWide, 0, s>>>(p);
@@ -531,7 +561,7 @@ static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, b
       ln_wide_bwd_kernel<T><<<*grid, kLnWide, 0, s>>>(p);
       const cudaError_t e = cudaGetLastError();
       if (e != cudaSuccess) return e;
-      if (p.part != nullptr) ln_wide_cols_kernel<T><<<dim3(*grid, (p.W + 255) / 256), 256, 0, s>>>(p);
+      if (p.part != nullptr) ln_wide_cols_kernel<T><<<dim3((unsigned)*grid, (unsigned)(p.W + 255) / 256), 256, 0, s>>>(p);
     }
     return cudaGetLastError();
   }
