@@ -4,7 +4,7 @@
 //
 // Both directions read every activation once: a row lives in the registers of one warp, or of one
 // CTA where it is wider, as NV vectors of VEC elements a thread (16 bytes where width, strides and
-// bases allow it, else single elements). CTAs walk the rows and keep the next few on the way into
+// bases allow it, else pairs, else single elements). CTAs walk the rows and keep the next few on the way into
 // shared memory by asynchronous copies (two rows in registers leave HBM a third idle): of 16-byte
 // vectors each thread copies and waits for its own; rows that begin anywhere come in the aligned
 // 16-byte pieces that hold them, and every thread takes its elements once all pieces are there. The
@@ -16,6 +16,7 @@
 // a second kernel adds those rows in a fixed order (bitwise reproducible). Rows wider than the
 // registers hold go to kernels that read them again from cache.
 #include <algorithm>
+#include <initializer_list>
 
 #include "common.cuh"
 #include "sparc_b200.h"
@@ -44,6 +45,11 @@ template <> struct LnVec<float, 1> {
   static __device__ __forceinline__ void get(float v, float* f) { f[0] = v; }
   static __device__ __forceinline__ float make(const float* f) { return f[0]; }
 };
+template <> struct LnVec<float, 2> {
+  using type = float2;
+  static __device__ __forceinline__ void get(float2 v, float* f) { f[0] = v.x, f[1] = v.y; }
+  static __device__ __forceinline__ float2 make(const float* f) { return make_float2(f[0], f[1]); }
+};
 template <> struct LnVec<float, 4> {
   using type = float4;
   static __device__ __forceinline__ void get(float4 v, float* f) { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
@@ -54,6 +60,16 @@ template <> struct LnVec<__nv_bfloat16, 1> {
   static __device__ __forceinline__ void get(unsigned short v, float* f) { f[0] = __uint_as_float((unsigned)v << 16); }
   static __device__ __forceinline__ unsigned short make(const float* f) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(f[0]));
+  }
+};
+template <> struct LnVec<__nv_bfloat16, 2> {
+  using type = unsigned;
+  static __device__ __forceinline__ void get(unsigned v, float* f) {
+    f[0] = __uint_as_float(v << 16), f[1] = __uint_as_float(v & 0xffff0000u);
+  }
+  static __device__ __forceinline__ unsigned make(const float* f) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(f[0], f[1]);
+    return *reinterpret_cast<const unsigned*>(&v);
   }
 };
 template <> struct LnVec<__nv_bfloat16, 8> {
@@ -125,7 +141,7 @@ template <typename T, int VEC, int NV, int WARPS, int NT>
 struct LnAhead {
   using Row = LnRow<T, VEC, NV, WARPS>;
   using R = typename LnVec<T, VEC>::type;
-  static constexpr bool kVectors = VEC > 1;
+  static constexpr bool kVectors = VEC * sizeof(T) == 16;
   static constexpr int kRows = WARPS == 1 ? kLnRows : 1;  // of a CTA at a time
   // of one tensor's row in a slot: the threads' vectors, or the row with the rest of its outer pieces
   static constexpr int kTensorBytes = 32 * WARPS * NV * VEC * (int)sizeof(T) + (kVectors ? 0 : 16);
@@ -176,9 +192,16 @@ struct LnAhead {
       for (int j = 0; j < NV; ++j) v[j] = reinterpret_cast<const R*>(from)[j * 32 * WARPS + i];
       Row::get(v, i * VEC, W, f);
     } else {
-      const T* e = reinterpret_cast<const T*>(from + (reinterpret_cast<unsigned long long>(q) & 15u));
+      const R* e = reinterpret_cast<const R*>(from + (reinterpret_cast<unsigned long long>(q) & 15u)) + i;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) f[j] = j * 32 * WARPS + i < W ? to_float(e[j * 32 * WARPS + i]) : 0.0f;
+      for (int j = 0; j < NV; ++j) {
+        if ((j * 32 * WARPS + i) * VEC < W) {
+          LnVec<T, VEC>::get(e[j * 32 * WARPS], f + j * VEC);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) f[j * VEC + k] = 0.0f;
+        }
+      }
     }
   }
   // Between a row's last take and the next ask, which writes its slot: every thread has taken it. (With
@@ -490,9 +513,8 @@ struct LnPlan {
   int vec, nv, warps;  // warps == 0: the wide kernels
 };
 
-// The narrowest of the instances that holds a row; vectors where `vectors` (16-byte aligned rows).
-static LnPlan ln_plan(int W, bool vectors, int size) {
-  const int vec = vectors ? 16 / size : 1;
+// The narrowest of the instances that holds a row.
+static LnPlan ln_plan(int W, int vec) {
   if (W <= 256) return LnPlan{vec, 8 / vec, 1};
   if (W <= 512) return LnPlan{vec, 16 / vec, 1};
   if (W <= 1024) return LnPlan{vec, 8 / vec, 4};
@@ -568,6 +590,9 @@ static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, b
   if (pl.vec == 1) {
     return pl.nv == 8 ? ln_warps<T, 1, 8>(p, pl, grid, backward, s) : ln_warps<T, 1, 16>(p, pl, grid, backward, s);
   }
+  if (pl.vec == 2) {
+    return pl.nv == 4 ? ln_warps<T, 2, 4>(p, pl, grid, backward, s) : ln_warps<T, 2, 8>(p, pl, grid, backward, s);
+  }
   if constexpr (V == 8) {
     return pl.nv == 1 ? ln_warps<T, 8, 1>(p, pl, grid, backward, s) : ln_warps<T, 8, 2>(p, pl, grid, backward, s);
   } else {
@@ -575,8 +600,19 @@ static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, b
   }
 }
 
-static bool ln_aligned(const void* q, long long stride, long long R, int size) {
-  return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (R <= 1 || (stride * size) % 16 == 0);
+// Elements that width, bases and row strides let be read and written at once: 16 bytes, a pair, or one.
+struct LnTensor {
+  const void* p;
+  long long stride;
+};
+static int ln_vec(long long R, int W, std::initializer_list<LnTensor> tensors, int size) {
+  auto fits = [&](int bytes) {
+    bool ok = (long long)W * size % bytes == 0;
+    for (const LnTensor& t : tensors)
+      ok = ok && reinterpret_cast<uintptr_t>(t.p) % bytes == 0 && (R <= 1 || t.stride * size % bytes == 0);
+    return ok;
+  };
+  return fits(16) ? 16 / size : fits(2 * size) ? 2 : 1;
 }
 
 }  // namespace sparc
@@ -612,8 +648,7 @@ int sparc_layer_norm_forward(const SparcLayerNormFwdArgs* a, void* stream) {
   p.sx = a->x_row_stride;
   p.W = (int)a->width;
   p.eps = a->eps;
-  const bool vectors = p.W * size % 16 == 0 && ln_aligned(a->x, p.sx, p.R, size) && ln_aligned(a->y, p.W, p.R, size);
-  const LnPlan pl = ln_plan(p.W, vectors, size);
+  const LnPlan pl = ln_plan(p.W, ln_vec(p.R, p.W, {{a->x, p.sx}, {a->y, p.W}}, size));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   int grid = 0;
   const cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, &grid, false, s)
@@ -648,9 +683,7 @@ int sparc_layer_norm_backward(const SparcLayerNormBwdArgs* a, void* stream) {
   p.sx = a->x_row_stride;
   p.sdy = a->dy_row_stride;
   p.W = (int)a->width;
-  const bool vectors = p.W * size % 16 == 0 && ln_aligned(a->x, p.sx, p.R, size) &&
-                       ln_aligned(a->dy, p.sdy, p.R, size) && ln_aligned(a->dx, p.W, p.R, size);
-  const LnPlan pl = ln_plan(p.W, vectors, size);
+  const LnPlan pl = ln_plan(p.W, ln_vec(p.R, p.W, {{a->x, p.sx}, {a->dy, p.sdy}, {a->dx, p.W}}, size));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   int grid = 0;
   cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, &grid, true, s)
