@@ -97,6 +97,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // Threads per row = 32 WARPS; with WARPS == 1 a CTA's kLnRows warps take a row each.
 constexpr int kLnRows = 8;
+constexpr int kLnHeld = 16;  // a thread's columns whose parameters it holds in registers
 template <int WARPS> constexpr int kLnThreads = WARPS == 1 ? 32 * kLnRows : 32 * WARPS;
 
 // A thread's share of a row: element e of its vector j is column (j * 32 WARPS + i) VEC + e, i the
@@ -241,9 +242,20 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_fwd_kernel(const LnParam
   };
 #pragma unroll
   for (int k = 0; k < Ahead::kDepth; ++k) ask(first + k * step);
-  float w[E], b[E];
-  Row::params(p.w, c0, p.W, w);
-  Row::params(p.b, c0, p.W, b);
+  constexpr bool kHeld = E <= kLnHeld;  // the parameters of the thread's columns in registers, else in shared memory
+  float w[kHeld ? E : 1], b[kHeld ? E : 1];
+  constexpr int kColumns = 32 * WARPS * E;
+  float* s_w = reinterpret_cast<float*>(s_ring + Ahead::kBytes);  // [2][kColumns]
+  if constexpr (kHeld) {
+    Row::params(p.w, c0, p.W, w);
+    Row::params(p.b, c0, p.W, b);
+  } else {
+    for (int c = threadIdx.x; c < kColumns; c += kLnThreads<WARPS>) {
+      s_w[c] = c < p.W ? __ldg(p.w + c) : 0.0f;
+      s_w[kColumns + c] = p.b != nullptr && c < p.W ? __ldg(p.b + c) : 0.0f;
+    }
+    __syncthreads();
+  }
   int par = 0;
   for (long long r = first; r < p.R; r += step, par ^= 1) {
     float x[E], sum = 0.0f, m2 = 0.0f;
@@ -282,10 +294,17 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_fwd_kernel(const LnParam
     }
     const float rstd = 1.0f / sqrtf(fmaf(m2, inv_w, p.eps));
     if (i == 0 && p.mean != nullptr) p.mean[r] = mean, p.rstd[r] = rstd;
+    // (without a bias b = 0: fmaf(n, w, 0) is n w but for the sign of a zero)
+    if constexpr (kHeld) {
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-      const float n = (x[k] - mean) * rstd;
-      x[k] = p.b != nullptr ? fmaf(n, w[k], b[k]) : n * w[k];
+      for (int k = 0; k < E; ++k) x[k] = fmaf((x[k] - mean) * rstd, w[k], b[k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const float* q = s_w + c0 + j * Row::kStep;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[j * VEC + e] = fmaf((x[j * VEC + e] - mean) * rstd, q[e], q[kColumns + e]);
+      }
     }
     Row::put(p.out, r * p.W, c0, p.W, x);
   }
@@ -510,16 +529,24 @@ constexpr int kLnSms = 148;
 constexpr int kLnSumGrid = kLnSms * 8;  // the most CTAs that walk the rows
 
 struct LnPlan {
-  int vec, nv, warps;  // warps == 0: the wide kernels
+  int vec, elements, warps;  // elements a thread; warps a row (0: the wide kernels)
 };
 
-// The narrowest of the instances that holds a row.
-static LnPlan ln_plan(int W, int vec) {
-  if (W <= 256) return LnPlan{vec, 8 / vec, 1};
-  if (W <= 512) return LnPlan{vec, 16 / vec, 1};
-  if (W <= 1024) return LnPlan{vec, 8 / vec, 4};
+// The narrowest of the instances that holds a row. The forward gives a row of up to 2048 to one warp,
+// which needs no barrier, once there are rows enough to fill the SMs with such warps (131072 x 2048
+// bf16: four warps a row 202 us, one 194; 138996 x 1374: 249, 216); with fewer, four warps are done
+// sooner.
+static LnPlan ln_plan(long long R, int W, int vec, bool backward) {
+  if (W <= 256) return LnPlan{vec, 8, 1};
+  if (W <= 512) return LnPlan{vec, 16, 1};
+  if (!backward && R >= kLnSms * 16) {
+    if (W <= 1024) return LnPlan{vec, 32, 1};
+    if (W <= 2048) return LnPlan{vec, 64, 1};
+  }
+  if (W <= 1024) return LnPlan{vec, 8, 4};
   for (int warps : {4, 8, 16})
-    if (W <= 32 * 16 * warps) return LnPlan{vec, 16 / vec, warps};
+    if (W <= 32 * 16 * warps) return LnPlan{vec, 16, warps};
+  if (!backward && W <= 32 * 32 * 16) return LnPlan{vec, 32, 16};
   return LnPlan{1, 0, 0};
 }
 
@@ -538,10 +565,17 @@ static size_t ln_ws_bytes(long long R, long long W) {
 // sums each (kLnSumGrid of them at most).
 template <typename T, int VEC, int NV, int WARPS>
 static cudaError_t ln_launch(const LnParams& p, int* grid, bool backward, cudaStream_t s) {
-  const auto kernel = backward ? ln_bwd_kernel<T, VEC, NV, WARPS> : ln_fwd_kernel<T, VEC, NV, WARPS>;
-  const int ring = backward ? LnAhead<T, VEC, NV, WARPS, 2>::kBytes : LnAhead<T, VEC, NV, WARPS, 1>::kBytes;
+  void (*kernel)(const LnParams) = ln_fwd_kernel<T, VEC, NV, WARPS>;
+  if constexpr (VEC * NV <= kLnHeld) {  // (the backward's sums are in registers too)
+    if (backward) kernel = ln_bwd_kernel<T, VEC, NV, WARPS>;
+  }
+  int ring = LnAhead<T, VEC, NV, WARPS, 1>::kBytes;
+  if constexpr (VEC * NV <= kLnHeld) {
+    if (backward) ring = LnAhead<T, VEC, NV, WARPS, 2>::kBytes;
+  }
   // (one warp a row: the warps' sums meet in the same memory)
-  const int smem = backward && WARPS == 1 ? std::max(ring, kLnRows * 2 * 32 * VEC * NV * (int)sizeof(float)) : ring;
+  int smem = backward && WARPS == 1 ? std::max(ring, kLnRows * 2 * 32 * VEC * NV * (int)sizeof(float)) : ring;
+  if (!backward && VEC * NV > kLnHeld) smem += 2 * 32 * WARPS * VEC * NV * (int)sizeof(float);
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
@@ -560,14 +594,19 @@ static cudaError_t ln_launch(const LnParams& p, int* grid, bool backward, cudaSt
   return cudaGetLastError();
 }
 
-template <typename T, int VEC, int NV>
-static cudaError_t ln_warps(const LnParams& p, const LnPlan& pl, int* grid, bool backward, cudaStream_t s) {
-  if (pl.warps == 1) return ln_launch<T, VEC, NV, 1>(p, grid, backward, s);
-  if constexpr (VEC * NV == 16) {
-    if (pl.warps == 8) return ln_launch<T, VEC, NV, 8>(p, grid, backward, s);
-    if (pl.warps == 16) return ln_launch<T, VEC, NV, 16>(p, grid, backward, s);
+template <typename T, int VEC>
+static cudaError_t ln_instance(const LnParams& p, const LnPlan& pl, int* grid, bool backward, cudaStream_t s) {
+  switch (pl.warps * 100 + pl.elements) {
+    case 108: return ln_launch<T, VEC, 8 / VEC, 1>(p, grid, backward, s);
+    case 116: return ln_launch<T, VEC, 16 / VEC, 1>(p, grid, backward, s);
+    case 132: return ln_launch<T, VEC, 32 / VEC, 1>(p, grid, backward, s);
+    case 164: return ln_launch<T, VEC, 64 / VEC, 1>(p, grid, backward, s);
+    case 408: return ln_launch<T, VEC, 8 / VEC, 4>(p, grid, backward, s);
+    case 416: return ln_launch<T, VEC, 16 / VEC, 4>(p, grid, backward, s);
+    case 816: return ln_launch<T, VEC, 16 / VEC, 8>(p, grid, backward, s);
+    case 1632: return ln_launch<T, VEC, 32 / VEC, 16>(p, grid, backward, s);
+    default: return ln_launch<T, VEC, 16 / VEC, 16>(p, grid, backward, s);
   }
-  return ln_launch<T, VEC, NV, 4>(p, grid, backward, s);
 }
 
 template <typename T>
@@ -587,17 +626,9 @@ static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, b
     }
     return cudaGetLastError();
   }
-  if (pl.vec == 1) {
-    return pl.nv == 8 ? ln_warps<T, 1, 8>(p, pl, grid, backward, s) : ln_warps<T, 1, 16>(p, pl, grid, backward, s);
-  }
-  if (pl.vec == 2) {
-    return pl.nv == 4 ? ln_warps<T, 2, 4>(p, pl, grid, backward, s) : ln_warps<T, 2, 8>(p, pl, grid, backward, s);
-  }
-  if constexpr (V == 8) {
-    return pl.nv == 1 ? ln_warps<T, 8, 1>(p, pl, grid, backward, s) : ln_warps<T, 8, 2>(p, pl, grid, backward, s);
-  } else {
-    return pl.nv == 2 ? ln_warps<T, 4, 2>(p, pl, grid, backward, s) : ln_warps<T, 4, 4>(p, pl, grid, backward, s);
-  }
+  if (pl.vec == 1) return ln_instance<T, 1>(p, pl, grid, backward, s);
+  if (pl.vec == 2) return ln_instance<T, 2>(p, pl, grid, backward, s);
+  return ln_instance<T, V>(p, pl, grid, backward, s);
 }
 
 // Elements that width, bases and row strides let be read and written at once: 16 bytes, a pair, or one.
@@ -648,7 +679,7 @@ int sparc_layer_norm_forward(const SparcLayerNormFwdArgs* a, void* stream) {
   p.sx = a->x_row_stride;
   p.W = (int)a->width;
   p.eps = a->eps;
-  const LnPlan pl = ln_plan(p.W, ln_vec(p.R, p.W, {{a->x, p.sx}, {a->y, p.W}}, size));
+  const LnPlan pl = ln_plan(p.R, p.W, ln_vec(p.R, p.W, {{a->x, p.sx}, {a->y, p.W}}, size), false);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   int grid = 0;
   const cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, &grid, false, s)
@@ -683,7 +714,7 @@ int sparc_layer_norm_backward(const SparcLayerNormBwdArgs* a, void* stream) {
   p.sx = a->x_row_stride;
   p.sdy = a->dy_row_stride;
   p.W = (int)a->width;
-  const LnPlan pl = ln_plan(p.W, ln_vec(p.R, p.W, {{a->x, p.sx}, {a->dy, p.sdy}, {a->dx, p.W}}, size));
+  const LnPlan pl = ln_plan(p.R, p.W, ln_vec(p.R, p.W, {{a->x, p.sx}, {a->dy, p.sdy}, {a->dx, p.W}}, size), true);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   int grid = 0;
   cudaError_t e = a->dtype == SPARC_DTYPE_BF16 ? ln_dispatch<__nv_bfloat16>(p, pl, &grid, true, s)
