@@ -20,8 +20,8 @@
 // per kGatedChunk tokens, so that the states are not rounded to the activations' type), the
 // adjoints from the step before. The cluster size grows as rows x channels shrink. All orders are
 // fixed: results are bitwise reproducible. Each warp copies its own tokens to shared memory
-// asynchronously, a step ahead (into the place whose values it has just taken into registers), so
-// nothing but the copies' own completion orders them.
+// asynchronously, one or two steps ahead (into the place whose values it has just taken into registers),
+// so nothing but the copies' own completion orders them.
 //
 // A segment start drops what came before it, infinities and NaN included: its factor is kept as
 // -0 (a_t >= +0, so the sign marks it through products), and composing with it selects instead of
@@ -38,17 +38,18 @@ constexpr int kGatedChunk = 32;  // tokens per saved carry
 constexpr int kGatedMaxCluster = 16;  // (above 8 a kernel has to allow it)
 constexpr unsigned kGatedSpin = 1u << 22;  // default bound of a wait's polls (each may sleep in hardware)
 
-// How a CTA cuts its tile: WARPS spans of K tokens; BLOCKS CTAs per SM that the registers are held to.
-template <int K_, int WARPS_, int BLOCKS_>
+// How a CTA cuts its tile: WARPS spans of K tokens; BLOCKS CTAs per SM that the registers are held to;
+// STAGES steps of inputs on their way.
+template <int K_, int WARPS_, int BLOCKS_, int STAGES_>
 struct GatedCut {
-  static constexpr int K = K_, WARPS = WARPS_, BLOCKS = BLOCKS_, TILE = K * WARPS;
+  static constexpr int K = K_, WARPS = WARPS_, BLOCKS = BLOCKS_, STAGES = STAGES_, TILE = K * WARPS;
 };
 template <typename T> struct GatedFwdCut;
-template <> struct GatedFwdCut<__nv_bfloat16> : GatedCut<16, 4, 4> {};
-template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2> {};
+template <> struct GatedFwdCut<__nv_bfloat16> : GatedCut<16, 4, 4, 1> {};
+template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2, 1> {};
 template <typename T> struct GatedBwdCut;
-template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 3> {};
-template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2> {};
+template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 3, 2> {};
+template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2, 2> {};
 // the backward's tile is one chunk
 static_assert(GatedBwdCut<float>::TILE == kGatedChunk && GatedBwdCut<__nv_bfloat16>::TILE == kGatedChunk);
 
@@ -116,13 +117,17 @@ __device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {  // for all but the last N groups
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // A warp's reads of its next tokens: K of them a step, of NT tensors, into stage[tensor][token][lane].
 // What lies beyond the sequence or the channels is not copied: those values are never used.
 // Each lane owns pieces kRows tokens apart, and keeps a pointer per tensor that moves by a constant
 // from step to step (with single elements the warp's pointers are of the tokens' first channel).
-template <typename T, int MODE, int K, int NT>
+template <typename T, int MODE, int K, int NT, int S>
 struct GatedReader {
   using R = typename Duo<T>::type;
   static constexpr int kBytes = MODE == kModeWide ? 16 : (int)sizeof(R);
@@ -155,8 +160,11 @@ struct GatedReader {
     for (int n = 0; n < NT; ++n)
       src[n] = reinterpret_cast<const char*>(static_cast<const T*>(p.in[n].p) + bt * p.in[n].sb + (long long)t * p.in[n].st + chan);
   }
-  // `left`: tokens of the sequence from this step's first on
-  __device__ __forceinline__ void copy(int left, int lane) {
+  static constexpr int kStageBytes = NT * K * kRowBytes;
+
+  // `left`: tokens of the sequence from this step's first on (none: an empty group, so that the groups count steps)
+  __device__ __forceinline__ void copy(int slot, int left, int lane) {
+    const unsigned to = dst + slot * kStageBytes;
     if constexpr (MODE == kModeSingle) {
       // (rolled: code that runs once is paid for in instruction fetches)
       const int some = min(K, left);
@@ -167,7 +175,7 @@ struct GatedReader {
         for (int n = 0; n < NT; ++n) {
           const char* a = src[n] + k * row[n];
           const int off = (int)(reinterpret_cast<unsigned long long>(a) & 15u);
-          if (at - off < bytes) copy_async<16>(dst + n * K * kRowBytes + c * 16, a - off + at);
+          if (at - off < bytes) copy_async<16>(to + n * K * kRowBytes + c * 16, a - off + at);
         }
       }
     } else if (left >= K) {
@@ -176,7 +184,7 @@ struct GatedReader {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < K / kRows; ++i)
-            copy_async<kBytes>(dst + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
+            copy_async<kBytes>(to + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
       }
     } else {
 #pragma unroll
@@ -184,16 +192,17 @@ struct GatedReader {
 #pragma unroll
         for (int i = 0; i < K / kRows; ++i)
           if (token < K && token + i * kRows < left)
-            copy_async<kBytes>(dst + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
+            copy_async<kBytes>(to + (n * K + i * kRows) * 32 * (int)sizeof(R), src[n] + i * row[n]);
     }
+    copy_commit();
 #pragma unroll
     for (int n = 0; n < NT; ++n) src[n] += move[n];
   }
-  // tokens k0 .. k0 + N - 1 of tensor n of the step that was copied last, once it has come
+  // tokens k0 .. k0 + N - 1 of tensor n of the step in `slot`, the first of the S that are on their way, once it has come
   template <int N>
-  __device__ __forceinline__ void read(int n, int k0, int lane, R (&v)[N]) const {
-    const char* q = reinterpret_cast<const char*>(stage) + (n * K + k0) * kRowBytes + lane * (int)sizeof(R);
-    const unsigned step = (unsigned)row[n], first = (unsigned)reinterpret_cast<unsigned long long>(src[n] - move[n]) + k0 * step;
+  __device__ __forceinline__ void read(int slot, int n, int k0, int lane, R (&v)[N]) const {
+    const char* q = reinterpret_cast<const char*>(stage) + slot * kStageBytes + (n * K + k0) * kRowBytes + lane * (int)sizeof(R);
+    const unsigned step = (unsigned)row[n], first = (unsigned)reinterpret_cast<unsigned long long>(src[n] - S * move[n]) + k0 * step;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const char* w = q + k * kRowBytes;
@@ -510,14 +519,13 @@ __device__ __forceinline__ unsigned gated_segments(const GatedParams& p, long lo
 }
 
 // ---------------------------------------------------------------- forward
-// A thread's tokens go through the gates four at a time (more take too many registers).
-constexpr int kGatedGroup = 4;
+// A thread's tokens go through the gates eight at a time, in the backward four (more take too many registers).
 
 template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
                                                  const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu,
                                                  float2 (&a)[K], float2 (&b)[K]) {
-  constexpr int N = kGatedGroup;
+  constexpr int N = 8;
 #pragma unroll
   for (int k0 = 0; k0 < K; k0 += N) {
     float2 x[N], r[N], w[N];
@@ -532,7 +540,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
     gated_fwd_kernel(const __grid_constant__ GatedParams p) {
   using R = typename Duo<T>::type;
   using C = GatedFwdCut<T>;
-  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 3;
+  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, S = C::STAGES, NT = 3;
   extern __shared__ __align__(16) unsigned char s_raw[];  // the cluster's maps, then [warp][tensor][token][lane]
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
   __shared__ unsigned long long s_bar[2];
@@ -544,11 +552,11 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const bool on = ch < p.D;
   const int stride = cs * TILE;  // tokens from a step to the next
   const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, H) of each CTA
-  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * NT * K * (GatedReader<T, MODE, K, NT>::kRowBytes / (int)sizeof(R));
+  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
-  GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, stride);
+  GatedReader<T, MODE, K, NT, S> reader(p, stage, ch0, lane, stride);
   if (cs > 1) exchange_init(peers);
   unsigned n = 0;  // steps so far
 
@@ -557,21 +565,24 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
     float2 carry = load_pair(p.h0, bt * p.D + ch, ch, p.D);  // the state entering the step
     T* y = static_cast<T*>(p.y) + (bt * p.L + rank * TILE) * p.D;  // of the CTA's first token and channel
     reader.start(p, bt, t0, ch0, lane);
-    reader.copy(p.L - t0, lane);
+    int slot = 0;
+#pragma unroll
+    for (int k = 0; k < S; ++k) reader.copy(k, p.L - t0 - k * stride, lane);
     for (int first = 0; first < p.L; first += stride, t0 += stride, ++n) {
       const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
-      copy_wait();
+      copy_wait<S - 1>();
       __syncwarp();
       float2 a[K], b[K], A = bcast2(1.0f), H = bcast2(0.0f);
       const int live = p.L - t0;  // tokens of the sequence from here on
       {
         R rx[K], rr[K], rw[K];
-        reader.read(0, 0, lane, rx);
-        reader.read(1, 0, lane, rr);
-        reader.read(2, 0, lane, rw);
+        reader.read(slot, 0, 0, lane, rx);
+        reader.read(slot, 1, 0, lane, rr);
+        reader.read(slot, 2, 0, lane, rw);
         __syncwarp();  // every lane has read its values
-        reader.copy(live - stride, lane);
+        reader.copy(slot, live - S * stride, lane);
+        if (S > 1) slot = slot + 1 == S ? 0 : slot + 1;
         // (also of warps beyond the sequence: a condition here makes the others spill, and costs 8%)
         if (near) gated_fwd_tokens<T, true>(rx, rr, rw, nu, root_nu, a, b);
         else gated_fwd_tokens<T, false>(rx, rr, rw, nu, root_nu, a, b);
@@ -639,7 +650,7 @@ template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_bwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
                                                  const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu, int live,
                                                  float2* put, float2 (&f)[K], float2 (&b)[K], float2 (&q1)[K], float2 (&q2)[K]) {
-  constexpr int N = kGatedGroup;
+  constexpr int N = 4;
 #pragma unroll
   for (int k0 = 0; k0 < K; k0 += N) {
     if (k0 >= live) continue;
@@ -667,7 +678,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     gated_bwd_kernel(const __grid_constant__ GatedParams p) {
   using R = typename Duo<T>::type;
   using C = GatedBwdCut<T>;
-  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, NT = 4;
+  constexpr int K = C::K, NW = C::WARPS, TILE = C::TILE, S = C::STAGES, NT = 4;
   extern __shared__ __align__(16) unsigned char s_raw[];  // the cluster's maps, [warp][token][3][lane] put by, the inputs
   __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
@@ -682,11 +693,11 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const int stride = cs * TILE, steps = (p.chunks + cs - 1) / cs;
   const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, G) of each CTA
   float2* put = reinterpret_cast<float2*>(s_raw + gated_map_bytes(cs)) + wp * K * 96 + lane;
-  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * NT * K * (GatedReader<T, MODE, K, NT>::kRowBytes / (int)sizeof(R));
+  R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
   const bool near = __all_sync(0xffffffffu, nu.x <= kGatedNear && nu.y <= kGatedNear);
-  GatedReader<T, MODE, K, NT> reader(p, stage, ch0, lane, -stride);
+  GatedReader<T, MODE, K, NT, S> reader(p, stage, ch0, lane, -stride);
   if (cs > 1) exchange_init(peers);
   unsigned n = 0;  // steps so far
   double dnu_x = 0.0, dnu_y = 0.0;
@@ -696,25 +707,28 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     float2 carry = load_pair(p.grad_last, bt * p.D + ch, ch, p.D);  // c_{t+1} lam_{t+1} entering the step's last token
     long long base = (bt * p.L + (long long)tile * TILE) * p.D;     // of the CTA's first token and channel in the gradients
     reader.start(p, bt, t0, ch0, lane);
-    reader.copy(p.L - t0, lane);
+    int slot = 0;
+#pragma unroll
+    for (int k = 0; k < S; ++k) reader.copy(k, k < steps ? p.L - t0 + k * stride : 0, lane);
     for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, ++n) {
       const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
       // the state entering this CTA's tile
       float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (bt * p.chunks + tile) * p.D + ch, ch, p.D);
-      copy_wait();
+      copy_wait<S - 1>();
       __syncwarp();
       const int live = p.L - t0;
       float2 f[K], b[K], q1[K], q2[K], A = bcast2(1.0f), H = bcast2(0.0f), G = bcast2(0.0f);
       R rd[K];
       {
         R rx[K], rr[K], rw[K];
-        reader.read(0, 0, lane, rx);
-        reader.read(1, 0, lane, rr);
-        reader.read(2, 0, lane, rw);
-        reader.read(3, 0, lane, rd);
+        reader.read(slot, 0, 0, lane, rx);
+        reader.read(slot, 1, 0, lane, rr);
+        reader.read(slot, 2, 0, lane, rw);
+        reader.read(slot, 3, 0, lane, rd);
         __syncwarp();
-        reader.copy(step > 0 ? live + stride : 0, lane);
+        reader.copy(slot, step >= S ? live + S * stride : 0, lane);
+        if (S > 1) slot = slot + 1 == S ? 0 : slot + 1;
         if (near) gated_bwd_tokens<T, true>(rx, rr, rw, nu, root_nu, live, put, f, b, q1, q2);
         else gated_bwd_tokens<T, false>(rx, rr, rw, nu, root_nu, live, put, f, b, q1, q2);
       }
@@ -933,8 +947,10 @@ template <typename T, bool SEG, int MODE>
 static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_t s) {
   using F = GatedFwdCut<T>;
   using W = GatedBwdCut<T>;
-  constexpr int kRow = GatedReader<T, MODE, F::K, 3>::kRowBytes;
-  const int smem = gated_map_bytes(p.cluster) + (backward ? W::TILE * (4 * kRow + 96 * (int)sizeof(float2)) : F::TILE * 3 * kRow);
+    constexpr int kFwdBytes = F::WARPS * F::STAGES * GatedReader<T, MODE, F::K, 3, F::STAGES>::kStageBytes;
+  constexpr int kBwdBytes = W::WARPS * W::STAGES * GatedReader<T, MODE, W::K, 4, W::STAGES>::kStageBytes +
+                            W::TILE * 96 * (int)sizeof(float2);
+  const int smem = gated_map_bytes(p.cluster) + (backward ? kBwdBytes : kFwdBytes);
   const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
