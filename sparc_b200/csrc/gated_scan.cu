@@ -50,8 +50,10 @@ template <> struct GatedFwdCut<float> : GatedCut<8, 8, 2, 1> {};
 template <typename T> struct GatedBwdCut;
 template <> struct GatedBwdCut<__nv_bfloat16> : GatedCut<8, 4, 3, 2> {};
 template <> struct GatedBwdCut<float> : GatedCut<8, 4, 2, 2> {};
-// the backward's tile is one chunk
-static_assert(GatedBwdCut<float>::TILE == kGatedChunk && GatedBwdCut<__nv_bfloat16>::TILE == kGatedChunk);
+// some warp's tokens begin each chunk
+template <typename C> constexpr bool kGatedWhole = C::TILE % kGatedChunk == 0 && kGatedChunk % C::K == 0;
+static_assert(kGatedWhole<GatedFwdCut<float>> && kGatedWhole<GatedFwdCut<__nv_bfloat16>> &&
+              kGatedWhole<GatedBwdCut<float>> && kGatedWhole<GatedBwdCut<__nv_bfloat16>>);
 
 struct GatedIn {
   const void* p;
@@ -690,7 +692,8 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const unsigned id = blockIdx.x / (unsigned)cs;
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
   const bool on = ch < p.D;
-  const int stride = cs * TILE, steps = (p.chunks + cs - 1) / cs;
+  const int stride = cs * TILE, steps = ((p.L + TILE - 1) / TILE + cs - 1) / cs;
+  constexpr int kSpan = kGatedChunk / K;  // warps of a chunk
   const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, G) of each CTA
   float2* put = reinterpret_cast<float2*>(s_raw + gated_map_bytes(cs)) + wp * K * 96 + lane;
   R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
@@ -713,8 +716,8 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
     for (int step = steps - 1; step >= 0; --step, tile -= cs, t0 -= stride, ++n) {
       const int par = n & 1;
       const unsigned seg = SEG ? gated_segments<K>(p, bt, t0, lane) : 0u;
-      // the state entering this CTA's tile
-      float2 h = load_pair(tile < p.chunks ? p.carry : nullptr, (bt * p.chunks + tile) * p.D + ch, ch, p.D);
+      // the state entering this warp's chunk
+      float2 h = load_pair(t0 < p.L ? p.carry : nullptr, (bt * p.chunks + t0 / kGatedChunk) * p.D + ch, ch, p.D);
       copy_wait<S - 1>();
       __syncwarp();
       const int live = p.L - t0;
@@ -761,7 +764,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       }
 #pragma unroll
       for (int j = 0; j < NW - 1; ++j)
-        if (j < wp) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
+        if (j < wp && j >= wp / kSpan * kSpan) h = through<SEG>(lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]), h);
       // states forward: q1 <- q1 h_{t-1} + q2 (nothing of h_{t-1} at a segment start)
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -903,7 +906,8 @@ static GatedPlan gated_plan(long long B, long long L, long long D, bool backward
   const bool half = dtype == SPARC_DTYPE_BF16;
   const int blocks = backward ? (half ? GatedBwdCut<bf16>::BLOCKS : GatedBwdCut<float>::BLOCKS)
                               : (half ? GatedFwdCut<bf16>::BLOCKS : GatedFwdCut<float>::BLOCKS);
-  const int tile = backward ? kGatedChunk : half ? GatedFwdCut<bf16>::TILE : GatedFwdCut<float>::TILE;
+  const int tile = backward ? (half ? GatedBwdCut<bf16>::TILE : GatedBwdCut<float>::TILE)
+                            : (half ? GatedFwdCut<bf16>::TILE : GatedFwdCut<float>::TILE);
   GatedPlan pl;
   pl.groups = (int)((D + 63) / 64);
   const long long tiles = (L + tile - 1) / tile;
