@@ -582,7 +582,7 @@ static cudaError_t ln_launch(const LnParams& p, int* grid, bool backward, cudaSt
   int smem = backward && WARPS == 1 ? std::max(ring, kLnRows * 2 * 32 * VEC * NV * (int)sizeof(float)) : ring;
   if (!backward && VEC * NV > kLnHeld) smem += 2 * 32 * WARPS * VEC * NV * (int)sizeof(float);
   cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   static int resident[2] = {0, 0};
   int per_sm = __atomic_load_n(&resident[backward], __ATOMIC_RELAXED);

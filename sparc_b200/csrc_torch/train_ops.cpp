@@ -7,6 +7,7 @@
 // (TypeError), then the device (RuntimeError: there is no CPU path).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -81,6 +82,7 @@ unsigned* status_word(const Tensor& like) {
   Tensor& word = status_words().at(d);
   if (!word.defined()) {
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return nullptr;
+    const c10::InferenceMode ordinary(false);  // (the word outlives the call, whatever mode that is in)
     word = at::zeros({1}, like.options().dtype(at::kInt).requires_grad(false));
   }
   return reinterpret_cast<unsigned*>(word.mutable_data_ptr<int>());
@@ -446,7 +448,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     for (size_t i = 0; i < n; ++i) {
       Tensor t = target[i];
       if (!t.is_same(dst[i])) t.copy_(dst[i]);
-      else torch::autograd::impl::bump_version(t);
+      else if (!t.is_inference()) torch::autograd::impl::bump_version(t);
     }
   }
   return norm;

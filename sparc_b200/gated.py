@@ -30,7 +30,7 @@ def gated_scan(x: torch.Tensor, retention_gate: torch.Tensor, write_gate: torch.
     """The recurrence over [B, T, D]: y [B, T, D] in x's dtype, or with `return_last` (y, last)
     with the state after the last token, float32 [B, D]. Starts from `state` ([B, D]) or zero.
     Differentiable (once) with respect to x, the gates, nu_log and the state, through y and last."""
-    out = torch_ops.op("gated_scan")(x, retention_gate, write_gate, nu_log, state, segment_pos, return_last)
+    out = torch_ops.call("gated_scan", x, retention_gate, write_gate, nu_log, state, segment_pos, return_last)
     return tuple(out) if return_last else out[0]
 
 
@@ -39,4 +39,4 @@ def gated_scan_step(x: torch.Tensor, retention_gate: torch.Tensor, write_gate: t
     """One token: x and the gates [B, D], the state [B, D]; returns (y [B, D] in x's dtype, the new
     state, float32). Without autograd, as ``sparc_decode_step``; a length-1 ``gated_scan`` with the
     state is the differentiable form. `segment_pos` ([B]) restarts the rows whose position is 0."""
-    return torch_ops.op("gated_scan_step")(x, retention_gate, write_gate, nu_log, state, segment_pos)
+    return torch_ops.call("gated_scan_step", x, retention_gate, write_gate, nu_log, state, segment_pos)

@@ -19,7 +19,7 @@ from . import torch_ops
 
 def grad_norm(grads) -> torch.Tensor:
     """The norm of all elements of `grads` (an iterable of tensors) together: float32, one element."""
-    return torch_ops.op("grad_clip")(list(grads), [], False, 0.0, 0.0)
+    return torch_ops.call("grad_clip", list(grads), [], False, 0.0, 0.0)
 
 
 def clip_grads(grads, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
@@ -31,7 +31,7 @@ def clip_grads(grads, max_norm: float, out=None, eps: float = 1e-6) -> torch.Ten
         out = list(out)
         if len(out) != len(grads):
             raise ValueError("clip grads expects one output for each gradient")
-    return torch_ops.op("grad_clip")(grads, out or [], True, max_norm, eps)
+    return torch_ops.call("grad_clip", grads, out or [], True, max_norm, eps)
 
 
 def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6) -> torch.Tensor:

@@ -18,7 +18,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over x's last dimension, in x's dtype; differentiable (once) with respect to x,
     the weight and the bias."""
-    return torch_ops.op("layer_norm")(x, weight, bias, eps)
+    return torch_ops.call("layer_norm", x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

@@ -12,7 +12,7 @@ states and last states are marked non-differentiable.
 
 The operators of csrc_torch/train_ops.cpp (``gated_scan``, ``gated_scan_step``, ``layer_norm``,
 ``grad_clip``) carry their own checks and autograd in C++ and are what `gated.py`, `norm.py` and
-`grads.py` call; they have no fake kernels."""
+`grads.py` call; they have no fake kernels, and run between two graphs under torch.compile."""
 from __future__ import annotations
 
 import ctypes
@@ -59,6 +59,16 @@ def op(name: str):
     if f is None:
         f = _operators[name] = getattr(load(), name).default
     return f
+
+
+@torch.compiler.disable
+def _call_uncompiled(name, *args):
+    return op(name)(*args)
+
+
+def call(name: str, *args):
+    """An operator's call; under torch.compile it breaks the graph (there is nothing to trace it by)."""
+    return _call_uncompiled(name, *args) if torch.compiler.is_compiling() else op(name)(*args)
 
 
 def wait_status():

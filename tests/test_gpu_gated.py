@@ -67,14 +67,22 @@ def _check(t, nu, h0, pos, seed=1, dy=None):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 66), (2, 3, 5), (3, 8, 64), (1, 9, 2), (2, 33, 64), (3, 64, 66), (2, 65, 130), (1, 129, 31),
-          (1, 1000, 34), (2, 513, 7), (1, 2049, 2), (4, 300, 65)]
+          (1, 1000, 34), (2, 513, 7), (1, 2049, 2), (4, 300, 65), (1, 1100, 64), (5, 515, 128)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [0.5, 0.7])  # the least decay: nu above 1/2 in some channels, in none
 @pytest.mark.parametrize("B,T,D", SHAPES)
-def test_matches_oracle(B, T, D, dtype):
-    """One token to many tiles, odd channels, clusters of one to eight CTAs, ragged last tiles."""
-    _check(*_inputs(B, T, D, dtype, seed=B * T + D))
+def test_matches_oracle(B, T, D, low, dtype):
+    """One token to many tiles, odd channels, clusters of one to sixteen CTAs, ragged last tiles."""
+    _check(*_inputs(B, T, D, dtype, seed=B * T + D, low=low))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [64, 66, 33])
+def test_long_rows_without_segments(D, dtype):
+    """Clusters of sixteen over many steps, each kind of read."""
+    _check(*_inputs(1, 2500, D, dtype, segments=False, low=0.7))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -98,9 +106,11 @@ def test_strong_and_weak_decay():
     _check(t, nu, h0, pos)
 
 
-def test_gates_at_infinity():
+@pytest.mark.parametrize("nu_value", [1.0, 0.25])
+def test_gates_at_infinity(nu_value):
     """s(-inf) is exactly 0 and s(inf) exactly 1: a closed retention gate keeps the state (and
-    writes nothing, as 1 - a^2 = 0), a closed write gate writes nothing; gradients are finite."""
+    writes nothing, as 1 - a^2 = 0), a closed write gate writes nothing; gradients are finite, and
+    those of a closed write gate's x are exactly zero."""
     import sparc_b200
 
     inf = float("inf")
@@ -109,7 +119,7 @@ def test_gates_at_infinity():
         h0 = torch.randn(1, 8, device="cuda")
         closed = torch.full((1, 4, 8), -inf, device="cuda", dtype=dtype)
         opened = torch.full((1, 4, 8), inf, device="cuda", dtype=dtype)
-        nu = torch.zeros(8, device="cuda")
+        nu = torch.full((8,), float(np.log(nu_value)), device="cuda")
         xx = x.to(dtype)
         args = [v.clone().requires_grad_(True) for v in (xx, closed, opened, nu, h0)]
         y, last = sparc_b200.gated_scan(*args[:4], state=args[4], return_last=True)
@@ -117,7 +127,10 @@ def test_gates_at_infinity():
         for g in torch.autograd.grad((y, last), args, (torch.ones_like(y), torch.ones_like(last))):
             assert torch.isfinite(g).all()
         y = sparc_b200.gated_scan(xx, opened, closed, nu, state=h0)
-        a = torch.exp(torch.tensor(-1.0, dtype=torch.float64))
+        xc = xx.clone().requires_grad_(True)
+        yc = sparc_b200.gated_scan(xc, opened, closed, nu, state=h0)
+        assert not torch.autograd.grad(yc, xc, torch.ones_like(yc))[0].any()
+        a = torch.exp(torch.tensor(-nu_value, dtype=torch.float64))
         want = torch.stack([h0.double() * a ** (k + 1) for k in range(4)], 1)
         # four exp2 values, each off by 6 units, and their products
         assert ((y.double() - want).abs() <= want.abs() * (40 * G.U + torch.finfo(dtype).eps / 2)).all()
@@ -162,12 +175,13 @@ def test_nothing_crosses_a_segment_start(dtype):
             assert torch.equal(a[:, :cut], b[:, :cut]) and torch.isfinite(b[:, :cut]).all()
 
 
-def test_nan_inputs_are_not_lost():
+@pytest.mark.parametrize("low", [0.5, 0.7])
+def test_nan_inputs_are_not_lost(low):
     import sparc_b200
 
     for which in range(3):
         for dtype in (F32, BF16):
-            t, nu, _, _ = _inputs(1, 70, 33, dtype, state=False, segments=False)
+            t, nu, _, _ = _inputs(1, 70, 33, dtype, state=False, segments=False, low=low)
             t[which][0, 20, 3] = float("nan")
             y = sparc_b200.gated_scan(*t, nu)
             assert torch.isnan(y[0, 20:, 3]).all()
@@ -327,15 +341,87 @@ def test_streams_and_graphs():
         assert all(torch.equal(a, b) for a, b in zip(out, _check_only(tt, nn, hh, pos)))
 
 
+def test_stays_in_bounds():
+    """Nothing outside the outputs is written: through the C ABI, outputs inside canaried buffers at
+    every alignment an element allows, odd and even widths, ragged lengths, one and many CTAs."""
+    import ctypes
+
+    from sparc_b200 import _lib
+
+    L = _lib.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    for B, T, D, dtype, shift in ((2, 37, 33, BF16, 1), (1, 700, 64, BF16, 0), (3, 65, 10, F32, 1), (2, 100, 66, BF16, 2),
+                                  (1, 1, 7, F32, 3), (1, 1030, 31, F32, 0)):
+        t, nu, h0, pos = _inputs(B, T, D, dtype)
+        dy = torch.randn(B, T, D, device="cuda").to(dtype)
+
+        def guarded(n, kind):
+            buf = torch.full((n + 1024,), -9.0, dtype=kind, device="cuda")
+            return buf, buf[512 + shift:512 + shift + n]
+
+        chunks = L.sparc_gated_carry_chunks(T)
+        bufs = [guarded(B * T * D, dtype) for _ in range(4)] + [guarded(B * D, F32), guarded(B * chunks * D, F32),
+                                                               guarded(D, F32), guarded(B * D, F32)]
+        y, dx, dr, dw, last, carry, dnu, dh0 = (v for _, v in bufs)
+        nb = L.sparc_gated_workspace_bytes(B, T, D)
+        wsb = torch.full((nb + 512,), 77, dtype=torch.uint8, device="cuda")
+        ws = wsb[256:256 + nb]
+        st = (T * D, D)
+        f = _lib.GatedFwdArgs(*[v.data_ptr() for v in t], nu.data_ptr(), h0.data_ptr(), pos.data_ptr(), 8, y.data_ptr(),
+                              last.data_ptr(), carry.data_ptr(), *st, *st, *st, B, T, D, _lib.dtype_code(dtype))
+        assert L.sparc_gated_scan_forward(ctypes.byref(f), stream) == 0
+        b = _lib.GatedBwdArgs(*[v.data_ptr() for v in t], nu.data_ptr(), dy.data_ptr(), carry.data_ptr(), None,
+                              pos.data_ptr(), 8, dx.data_ptr(), dr.data_ptr(), dw.data_ptr(), dnu.data_ptr(), dh0.data_ptr(),
+                              ws.data_ptr(), nb, *st, *st, *st, *st, B, T, D, _lib.dtype_code(dtype))
+        assert L.sparc_gated_scan_backward(ctypes.byref(b), stream) == 0
+        torch.cuda.synchronize()
+        for buf, v in bufs:
+            assert (buf[:512 + shift] == -9).all() and (buf[512 + shift + v.numel():] == -9).all()
+            assert not (v == -9).any()
+        assert (wsb[:256] == 77).all() and (wsb[256 + nb:] == 77).all()
+        h, _ = G.forward(*[_np(v) for v in (*t, nu)], _np(h0), pos.cpu().numpy() == 0)
+        bd = G.bounds(*[_np(v) for v in (*t, nu)], None, _np(h0), pos.cpu().numpy() == 0)
+        _close(y.view(B, T, D), h, bd["h"], "y")
+
+
+def test_modes_of_the_caller():
+    """Under inference mode, and compiled (the graph breaks around the operators): the eager bits."""
+    import sparc_b200
+
+    t, nu, h0, pos = _inputs(2, 70, 40, BF16)
+    want = sparc_b200.gated_scan(*t, nu, state=h0, segment_pos=pos)
+    w = torch.ones(40, device="cuda")
+    with torch.inference_mode():
+        assert torch.equal(sparc_b200.gated_scan(*t, nu, state=h0, segment_pos=pos), want)
+        g = [torch.ones(10, device="cuda")]
+        sparc_b200.clip_grads(g, 0.5)
+        ln = sparc_b200.layer_norm(want, w)
+    sparc_b200.check_status()
+
+    def f(x, r, w_, n):
+        y = sparc_b200.layer_norm(x * 1.0, w)
+        return sparc_b200.gated_scan(y, r, w_, n, state=h0, segment_pos=pos) * 2.0
+
+    leaves = [v.clone().requires_grad_(True) for v in (*t, nu)]
+    y = f(*leaves)
+    grads = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    c = torch.compile(f, backend="eager")
+    yc = c(*leaves)
+    assert torch.equal(y, yc) and ln.shape == want.shape
+    for a, b in zip(grads, torch.autograd.grad(yc, leaves, torch.ones_like(yc))):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------ one token
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [0.5, 0.7])
 @pytest.mark.parametrize("B,D", [(1, 1), (1, 512), (3, 65), (257, 130), (40000, 2), (64, 2048)])
-def test_step(B, D, dtype):
+def test_step(B, D, low, dtype):
     """Against the oracle, and bit for bit the length-1 scan."""
     import sparc_b200
 
-    t, nu, h0, pos = _inputs(B, 1, D, dtype)
+    t, nu, h0, pos = _inputs(B, 1, D, dtype, low=low)
     pos = torch.where(torch.arange(B, device="cuda") % 3 == 1, 0, 4)
     q = [v[:, 0] for v in t]
     y, new = sparc_b200.gated_scan_step(*q, nu, h0, segment_pos=pos)
