@@ -389,7 +389,9 @@ int sparc_complex_scan_backward(const SparcComplexBwdArgs* args, void* stream);
  * (NULL when no backward follows) receives the state entering every chunk of
  * sparc_gated_chunk_tokens() tokens, [batch, sparc_gated_carry_chunks(length), channels] float32.
  * The backward takes dy (its own strides) and optionally the gradient of the last state, and
- * writes the gradients of x, the gates, nu_log ([channels]) and, optionally, h0. Its workspace,
+ * writes the gradients of x, the gates, nu_log ([channels]) and, optionally, h0. No output may
+ * overlap an input; inputs are read in aligned 16-byte pieces (bytes beside a tensor's ends within
+ * such a piece may be read, and are not used). Its workspace,
  * sparc_gated_workspace_bytes bytes, 8-byte aligned, needs no initial contents. Results are
  * bitwise reproducible. */
 typedef struct SparcGatedFwdArgs {
@@ -482,7 +484,7 @@ int sparc_gated_step(const SparcGatedStepArgs* args, void* stream);
  * sparc-impl/sparc/networks/sequence_classifier.py): y = (x - mean) rstd weight + bias with
  * rstd = (var + eps)^(-1/2), per row of x [rows, width] (dtype; row strides in elements, the
  * columns adjacent). weight, bias (optional), the statistics and the sums are float32; y and dx
- * are dense, in dtype. `mean` and `rstd` ([rows], together, NULL when no backward follows) are
+ * are dense, in dtype, and overlap no input. `mean` and `rstd` ([rows], together, NULL when no backward follows) are
  * what the backward reads. The backward writes dx and, where given, the weight's and bias's
  * gradients [width] (then with a workspace of sparc_layer_norm_workspace_bytes bytes, 4-byte
  * aligned, no initial contents needed), summed in a fixed order. */

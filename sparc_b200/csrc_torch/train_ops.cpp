@@ -47,13 +47,19 @@ void require_device(const Tensor& t, const char* name, const Tensor& like) {
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
-Tensor f32(const Tensor& t) { return t.detach().to(at::kFloat).contiguous(); }
+// t as a dense float32 array (itself where it is one).
+Tensor f32(const Tensor& t) {
+  if (t.scalar_type() == at::kFloat && t.is_contiguous() && !t.is_neg()) return t;
+  return t.detach().to(at::kFloat).contiguous().resolve_neg();
+}
 const float* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 float* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr<float>() : nullptr; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // t as the kernels read it: any strides but adjacent values in the last dimension.
-Tensor adjacent(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor adjacent(const Tensor& t) {
+  return (t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous()).resolve_neg();
+}
 
 // The gradients of a first-order backward; where a graph of them is asked for, it ends in an error.
 variable_list once(variable_list grads, const char* what) {
@@ -390,7 +396,7 @@ void grads_check(const char* what, const std::vector<Tensor>& tensors) {
 }
 
 // A tensor's values as one dense array (any order of its dimensions), or a dense copy.
-Tensor dense(const Tensor& t) { return t.is_non_overlapping_and_dense() ? t : t.contiguous(); }
+Tensor dense(const Tensor& t) { return (t.is_non_overlapping_and_dense() ? t : t.contiguous()).resolve_neg(); }
 
 // The norm of `grads`, and with `clip` the gradients scaled into `out` (in place where it is empty).
 Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, bool clip, double max_norm, double eps) {
@@ -420,7 +426,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     if (clip) {
       // in place: the gradient's own array or the copy of it; else an array in the source's order
       dst[i] = out.empty() ? src[i]
-               : out[i].strides() == src[i].strides() && out[i].is_non_overlapping_and_dense() ? out[i]
+               : out[i].strides() == src[i].strides() && out[i].is_non_overlapping_and_dense() && !out[i].is_neg() ? out[i]
                                                                                                : at::empty_like(src[i]);
       out_ptrs[i] = dst[i].mutable_data_ptr();
     }

@@ -195,3 +195,23 @@ def test_reproducible_streams_and_graphs():
     torch.cuda.synchronize()
     for _, static, n in runs:
         assert torch.equal(n, norms[0]) and all(torch.equal(a, b) for a, b in zip(static, want))
+
+
+@pytest.mark.parametrize("shape", [(1,), (5, 3)])
+def test_negated_views(shape):
+    """Gradients that PyTorch holds with the sign of their memory reversed, in place and into such outputs."""
+    import sparc_b200
+
+    g = torch.full(shape, 2.0, device="cuda")
+    n = float(g.square().sum().sqrt())
+
+    def negated(v):
+        return torch.complex(torch.zeros_like(v), -v).conj().imag
+
+    a = negated(g)
+    assert a.is_neg()
+    assert abs(float(sparc_b200.clip_grads([a], n / 2, eps=0.0)) - n) <= 6 * U * n
+    assert bool(((a - 1.0).abs() <= 16 * U).all())
+    o = negated(torch.zeros_like(g))
+    sparc_b200.clip_grads([g], n / 2, out=[o], eps=0.0)
+    assert bool(((o - 1.0).abs() <= 16 * U).all()) and bool((g == 2.0).all())
