@@ -447,7 +447,10 @@ __global__ void __launch_bounds__(kLnWide) ln_wide_fwd_kernel(const LnParams p) 
     }
     // the deviations' own mean is what rounding left of the mean
     const float off = block_sum(m1, s) * inv_w;
-    const float var = block_sum(m2, s) * inv_w - off * off, rstd = 1.0f / sqrtf(var + p.eps);
+    // (what is left of a row without variance may be below zero by rounding)
+    float var = block_sum(m2, s) * inv_w - off * off;
+    if (var < 0.0f) var = 0.0f;
+    const float rstd = 1.0f / sqrtf(var + p.eps);
     mean += off;
     if (threadIdx.x == 0 && p.mean != nullptr) p.mean[r] = mean, p.rstd[r] = rstd;
 #pragma unroll 4
@@ -483,20 +486,20 @@ __global__ void __launch_bounds__(kLnWide) ln_wide_bwd_kernel(const LnParams p) 
   }
 }
 
-// Partial sums of dw and db over a span of rows per CTA row, a thread per column.
+// Partial sums of dw and db over every gridDim.y-th row, a thread per column.
 template <typename T>
 __global__ void __launch_bounds__(256) ln_wide_cols_kernel(const LnParams p) {
-  const int c = blockIdx.y * 256 + threadIdx.x;
+  const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= p.W) return;
   float dw = 0.0f, db = 0.0f;
 #pragma unroll 4
-  for (long long r = blockIdx.x; r < p.R; r += gridDim.x) {
+  for (long long r = blockIdx.y; r < p.R; r += gridDim.y) {
     const float d = Io<T>::load(static_cast<const T*>(p.dy) + r * p.sdy + c);
     dw = fmaf(d, (Io<T>::load(static_cast<const T*>(p.x) + r * p.sx + c) - p.mean[r]) * p.rstd[r], dw);
     db += d;
   }
-  p.part[(long long)blockIdx.x * 2 * p.W + c] = dw;
-  p.part[(long long)blockIdx.x * 2 * p.W + p.W + c] = db;
+  p.part[(long long)blockIdx.y * 2 * p.W + c] = dw;
+  p.part[(long long)blockIdx.y * 2 * p.W + p.W + c] = db;
 }
 
 // dw, db from the partial rows: a block owns 32 of the 2 W columns, its 32 warps every 32nd row, in
@@ -627,7 +630,7 @@ static cudaError_t ln_dispatch(const LnParams& p, const LnPlan& pl, int* grid, b
       ln_wide_bwd_kernel<T><<<*grid, kLnWide, 0, s>>>(p);
       const cudaError_t e = cudaGetLastError();
       if (e != cudaSuccess) return e;
-      if (p.part != nullptr) ln_wide_cols_kernel<T><<<dim3((unsigned)*grid, (unsigned)(p.W + 255) / 256), 256, 0, s>>>(p);
+      if (p.part != nullptr) ln_wide_cols_kernel<T><<<dim3((unsigned)(p.W + 255) / 256, (unsigned)*grid), 256, 0, s>>>(p);
     }
     return cudaGetLastError();
   }

@@ -316,3 +316,40 @@ def test_canaries():
             assert (buf[:256] == -7).all() and (buf[256 + view.numel():] == -7).all()
             assert not (view == -7).all()
         assert (wsb[:256] == 77).all() and (wsb[256 + nb:] == 77).all()
+
+
+def test_the_widest_row():
+    """The width limit, with the parameters' gradients: as many columns as the launches have to cover."""
+    import sparc_b200
+
+    W = 1 << 24
+    x = torch.zeros(1, W, device="cuda", dtype=BF16)
+    x[0, ::2] = 1.0
+    w = torch.ones(W, device="cuda", requires_grad=True)
+    b = torch.zeros(W, device="cuda", requires_grad=True)
+    y = sparc_b200.layer_norm(x, w, b, 0.0)  # mean 1/2, deviation 1/2, both exact: y is +-1
+    assert torch.equal(y, x * 2 - 1)
+    dw, db = torch.autograd.grad(y, (w, b), torch.ones_like(y))
+    assert torch.equal(dw, (x[0] * 2 - 1).float()) and torch.equal(db, torch.ones_like(db))
+
+
+@pytest.mark.parametrize("value", [1e20, -7e18, 12345.678])
+def test_wide_rows_without_variance(value):
+    """What rounding leaves of the variance may not turn it negative."""
+    import sparc_b200
+
+    x = torch.full((2, 20001), value, device="cuda")
+    w = torch.ones(20001, device="cuda")
+    assert bool(torch.isfinite(sparc_b200.layer_norm(x, w)).all())
+
+
+def test_negated_views():
+    """A view that PyTorch holds with the sign of its memory reversed."""
+    import sparc_b200
+
+    x = torch.randn(7, 1, device="cuda")
+    n = torch.complex(torch.zeros_like(x), -x).conj().imag
+    w = torch.full((1,), 2.0, device="cuda")
+    b = torch.complex(torch.zeros(1, device="cuda"), torch.full((1,), -3.0, device="cuda")).conj().imag
+    assert n.is_neg() and b.is_neg()
+    assert bool((sparc_b200.layer_norm(n, w, b) == 3.0).all())
