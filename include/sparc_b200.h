@@ -417,7 +417,8 @@ typedef struct SparcGatedFwdArgs {
   int dtype;
   unsigned max_spin;                   /* bound of the waits within a cluster (0 = default) */
   unsigned* status;                    /* device word, or'ed with SPARC_STATUS_TIMEOUT if such a
-                                          wait ran out (the launch still completes), or NULL */
+                                          wait ran out (the kernel then stops, its
+                                          outputs unfinished), or NULL */
 } SparcGatedFwdArgs;
 
 typedef struct SparcGatedBwdArgs {

@@ -43,7 +43,7 @@
 
 namespace sparc {
 
-constexpr int kGatedChunk = 32;  // tokens per saved carry
+constexpr int kGatedChunk = 32;       // tokens per saved carry
 constexpr int kGatedMaxCluster = 16;  // (above 8 a kernel has to allow it)
 constexpr unsigned kGatedSpin = 1u << 22;  // default bound of a wait's polls (each may sleep in hardware)
 
@@ -486,6 +486,7 @@ __host__ __device__ constexpr int gated_map_bytes(int cs) { return cs > 1 ? 2 * 
 struct GatedExchange {
   float4* map;              // [2][CTAs of the cluster][32], at the same place in every CTA
   unsigned long long* bar;  // [2]
+  int* late;                // [2]: a wait of the step ran out
   int cs;
   __device__ __forceinline__ float4* at(int par, int rank) const { return map + (par * cs + rank) * 32; }
 };
@@ -495,6 +496,7 @@ __device__ __forceinline__ void exchange_init(const GatedExchange& x) {
     mbar_init(&x.bar[0], 1);
     mbar_init(&x.bar[1], 1);
     mbar_init_fence();
+    x.late[0] = x.late[1] = 0;
   }
   // every CTA of the cluster has started, and its barriers stand, before anything is pushed
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -518,8 +520,16 @@ __device__ __forceinline__ float2 exchange_through(const GatedExchange& x, int p
   if (q0 != q1) v = through<SEG>(lo2(x.at(par, q0)[lane]), hi2(x.at(par, q0)[lane]), v);
   return v;
 }
+// A wait that runs out is marked, and the CTA leaves at its next step, between the barrier that all its
+// warps pass (so that all see the mark) and its push; its peers' waits then run out and they leave too.
 __device__ __forceinline__ void exchange_wait(const GatedParams& p, const GatedExchange& x, unsigned n) {
-  if (!mbar_wait_cluster(&x.bar[n & 1], n >> 1 & 1u, p.max_spin) && p.status != nullptr) atomicOr(p.status, kStatusTimeout);
+  if (!mbar_wait_cluster(&x.bar[n & 1], n >> 1 & 1u, p.max_spin)) {
+    x.late[n & 1] = 1;
+    if (p.status != nullptr) atomicOr(p.status, kStatusTimeout);
+  }
+}
+__device__ __forceinline__ bool exchange_late(const GatedExchange& x, unsigned n) {  // of the step before
+  return *reinterpret_cast<volatile int*>(x.late + (n & 1 ^ 1)) != 0;
 }
 
 // Which of a warp's K tokens from t0 on start a segment, as bits.
@@ -531,7 +541,6 @@ __device__ __forceinline__ unsigned gated_segments(const GatedParams& p, long lo
 
 // ---------------------------------------------------------------- forward
 // A thread's tokens go through the gates eight at a time, in the backward four (more take too many registers).
-
 template <typename T, bool NEAR, int K>
 __device__ __forceinline__ void gated_fwd_tokens(const typename Duo<T>::type (&rx)[K], const typename Duo<T>::type (&rr)[K],
                                                  const typename Duo<T>::type (&rw)[K], float2 nu, float2 root_nu,
@@ -555,6 +564,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   extern __shared__ __align__(16) unsigned char s_raw[];  // the cluster's maps, then [warp][tensor][token][lane]
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
   __shared__ unsigned long long s_bar[2];
+  __shared__ int s_late[2];
   __shared__ float2 s_out[2][32];                         // one CTA: the state leaving its tile
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
@@ -562,7 +572,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
   const bool on = ch < p.D;
   const int stride = cs * TILE;  // tokens from a step to the next
-  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, H) of each CTA
+  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, s_late, cs};  // (A, H) of each CTA
   R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
@@ -614,6 +624,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
       __syncthreads();
       float2 h;  // the state entering this CTA's tile, then this warp's tokens
       if (cs > 1) {
+        if (exchange_late(peers, n)) goto leave;
         if (wp == NW - 1) {
           A = bcast2(1.0f), H = bcast2(0.0f);
 #pragma unroll
@@ -650,6 +661,8 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
       if (cs == 1 && wp == NW - 1) s_out[par][lane] = h;
     }
   }
+leave:
+  copy_wait<0>();
   if (cs > 1) cluster_sync_relaxed();  // no CTA leaves while a peer may still push to it
 }
 
@@ -694,6 +707,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   __shared__ float4 s_map[2][NW][32];                // (A, H) of each warp: states, forward
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
   __shared__ unsigned long long s_bar[2];
+  __shared__ int s_late[2];
   __shared__ float2 s_out[2][32];                    // one CTA: the adjoint leaving its tile
   __shared__ double2 s_nu[NW][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
@@ -703,7 +717,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const bool on = ch < p.D;
   const int stride = cs * TILE, steps = ((p.L + TILE - 1) / TILE + cs - 1) / cs;
   constexpr int kSpan = kGatedChunk / K;  // warps of a chunk
-  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, cs};  // (A, G) of each CTA
+  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, s_late, cs};  // (A, G) of each CTA
   float2* put = reinterpret_cast<float2*>(s_raw + gated_map_bytes(cs)) + wp * K * 96 + lane;
   R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
@@ -762,6 +776,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       s_adj[par][wp][lane] = G;
       __syncthreads();
       if (cs > 1) {
+        if (exchange_late(peers, n)) goto leave;
         if (wp == 0) {
 #pragma unroll
           for (int i = NW - 1; i >= 0; --i) {
@@ -823,6 +838,8 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
       }
     }
   }
+leave:
+  copy_wait<0>();
   if (cs > 1) cluster_sync_relaxed();
   // the CTA's sum of dnu_log per channel, over its warps in order
   s_nu[wp][lane] = make_double2(dnu_x, dnu_y);
@@ -960,7 +977,7 @@ template <typename T, bool SEG, int MODE>
 static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_t s) {
   using F = GatedFwdCut<T>;
   using W = GatedBwdCut<T>;
-    constexpr int kFwdBytes = F::WARPS * F::STAGES * GatedReader<T, MODE, F::K, 3, F::STAGES>::kStageBytes;
+  constexpr int kFwdBytes = F::WARPS * F::STAGES * GatedReader<T, MODE, F::K, 3, F::STAGES>::kStageBytes;
   constexpr int kBwdBytes = W::WARPS * W::STAGES * GatedReader<T, MODE, W::K, 4, W::STAGES>::kStageBytes +
                             W::TILE * 96 * (int)sizeof(float2);
   const int smem = gated_map_bytes(p.cluster) + (backward ? kBwdBytes : kFwdBytes);

@@ -384,6 +384,54 @@ def test_stays_in_bounds():
         _close(y.view(B, T, D), h, bd["h"], "y")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_short_waits_end(dtype):
+    """One poll for each wait between the CTAs of a cluster: where none ran out the results are those of
+    the ordinary bound, else the status says so; either way both directions end."""
+    from sparc_b200 import _lib
+
+    L = _lib.lib()
+    B, T, D = 1, 6000, 66
+    t, nu, h0, pos = _inputs(B, T, D, dtype, segments=False)
+    dy = torch.randn(B, T, D, device="cuda").to(dtype)
+    st, nb = (T * D, D), L.sparc_gated_workspace_bytes(B, T, D)
+    s = torch.cuda.current_stream().cuda_stream
+    got = {}
+    for spin in (0, 1):
+        y, gx, gr, gw = (torch.zeros(B, T, D, device="cuda", dtype=dtype) for _ in range(4))
+        carry = torch.zeros(B, L.sparc_gated_carry_chunks(T), D, device="cuda")
+        gn, ws = torch.zeros(D, device="cuda"), torch.zeros(nb, device="cuda", dtype=torch.uint8)
+        fw, bw = torch.zeros(1, device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+        f = _lib.GatedFwdArgs(*[v.data_ptr() for v in t], nu.data_ptr(), h0.data_ptr(), None, 0, y.data_ptr(), None,
+                              carry.data_ptr(), *st, *st, *st, B, T, D, _lib.dtype_code(dtype), spin, fw.data_ptr())
+        assert L.sparc_gated_scan_forward(f, s) == 0
+        c = got[0][0][1] if spin else carry  # the backward's own waits, on good carries
+        b = _lib.GatedBwdArgs(*[v.data_ptr() for v in t], nu.data_ptr(), dy.data_ptr(), c.data_ptr(), None, None, 0,
+                              gx.data_ptr(), gr.data_ptr(), gw.data_ptr(), gn.data_ptr(), None, ws.data_ptr(), nb, *st, *st,
+                              *st, *st, B, T, D, _lib.dtype_code(dtype), spin, bw.data_ptr())
+        assert L.sparc_gated_scan_backward(b, s) == 0
+        torch.cuda.synchronize()
+        got[spin] = (y, carry), (gx, gr, gw, gn), (int(fw), int(bw))
+    assert got[0][2] == (0, 0) and all(v in (0, 4) for v in got[1][2])
+    for k in (0, 1):
+        if got[1][2][k] == 0:
+            assert all(torch.equal(a, b) for a, b in zip(got[0][k], got[1][k]))
+
+
+def test_negated_views():
+    """Views that PyTorch holds with the sign of their memory reversed."""
+    import sparc_b200
+
+    t, nu, h0, _ = _inputs(2, 9, 1, F32, segments=False)
+    z = [torch.complex(torch.zeros_like(v), -v).conj().imag for v in (*t, h0)]
+    assert all(v.is_neg() for v in z)
+    x, r, w, s = z
+    assert torch.equal(sparc_b200.gated_scan(x, r, w, nu, state=s), sparc_b200.gated_scan(*t, nu, state=h0))
+    a = sparc_b200.gated_scan_step(x[:, 0], r[:, 0], w[:, 0], nu, s)
+    b = sparc_b200.gated_scan_step(*(v[:, 0] for v in t), nu, h0)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_modes_of_the_caller():
     """Under inference mode, and compiled (the graph breaks around the operators): the eager bits."""
     import sparc_b200
