@@ -27,8 +27,8 @@
 // -0 (a_t >= +0, so the sign marks it through products), and composing with it selects instead of
 // multiplying.
 //
-// Measured on a B200 (B=8 T=16384 D=2048 bfloat16, 268M channels x tokens): forward 480 us = 4.5 TB/s
-// of its 8 bytes each (68% of what a copy reaches), backward 905 us = 4.2 TB/s of 14 bytes (63%). Neither
+// Measured on a B200 (B=8 T=16384 D=2048 bfloat16, 268M channels x tokens): forward 475 us = 4.5 TB/s
+// of its 8 bytes each (69% of what a copy reaches), backward 874 us = 4.3 TB/s of 14 bytes (66%). Neither
 // bytes nor any one unit bounds them but instructions: 33 and 64 thread-instructions an element issue on
 // 52-54% of the cycles, the rest being the latency of a step's chain (gates, barrier, maps, replay) that
 // the 7-16 warps an SM holds (128 and 166 registers) do not cover; more warps at fewer registers issue

@@ -414,6 +414,85 @@ __global__ void __launch_bounds__(kLnThreads<WARPS>) ln_bwd_kernel(const LnParam
   }
 }
 
+// The backward of rows whose column sums do not fit the registers beside them: a row in the registers of 32
+// warps, weights and sums in shared memory (every thread its own columns), which leaves none for rows
+// ahead: the next row is asked for into L2 while this one is worked on. (2690 x 14960 float32 100 us,
+// 4000 x 16384 bfloat16 117 us, of floors 74 and 60; two reads of each row and a third for the sums took
+// 199 and 259. One CTA an SM walks its rows without overlap of a row's loads and its stores.)
+constexpr int kLnTallWarps = 32;
+template <typename T, int VEC, int NV>
+__global__ void __launch_bounds__(32 * kLnTallWarps) ln_tall_bwd_kernel(const LnParams p) {
+  constexpr int WARPS = kLnTallWarps, E = NV * VEC, N = 32 * WARPS;
+  using V = LnVec<T, VEC>;
+  using Row = LnRow<T, VEC, NV, WARPS>;
+  __shared__ float2 s_sum[2][WARPS];
+  extern __shared__ float s_columns[];  // [w, dw, db][element of a thread][thread]
+  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = threadIdx.x * VEC;
+  const float inv_w = 1.0f / (float)p.W;
+  const bool sums = p.part != nullptr;
+  float *w = s_columns + threadIdx.x, *dw = w + E * N, *db = dw + E * N;
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    const int c = c0 + k / VEC * Row::kStep + k % VEC;
+    w[k * N] = c < p.W ? __ldg(p.w + c) : 0.0f;
+    if (sums) dw[k * N] = db[k * N] = 0.0f;
+  }
+  int par = 0;
+  for (long long r = blockIdx.x; r < p.R; r += gridDim.x, par ^= 1) {
+    const T *x = static_cast<const T*>(p.x) + r * p.sx, *dy = static_cast<const T*>(p.dy) + r * p.sdy;
+    typename V::type rx[NV], rd[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (c0 + j * Row::kStep < p.W) {
+        rx[j] = *reinterpret_cast<const typename V::type*>(x + c0 + j * Row::kStep);
+        rd[j] = *reinterpret_cast<const typename V::type*>(dy + c0 + j * Row::kStep);
+      }
+    const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
+    if (r + gridDim.x < p.R) {
+      constexpr int kLine = 128 / (int)sizeof(T);
+      for (int c = threadIdx.x * kLine; c < p.W; c += 32 * WARPS * kLine) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(x + gridDim.x * p.sx + c));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(dy + gridDim.x * p.sdy + c));
+      }
+    }
+    float n[E], d[E], s1 = 0.0f, s2 = 0.0f;
+    Row::get(rx, c0, p.W, n);
+    Row::get(rd, c0, p.W, d);
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      n[k] = (n[k] - mean) * rstd;  // (beyond the row d = 0, so n does not matter)
+      if (sums) {
+        dw[k * N] = fmaf(d[k], n[k], dw[k * N]);
+        db[k * N] += d[k];
+      }
+      d[k] *= w[k * N];
+      s1 += d[k];
+      s2 = fmaf(d[k], n[k], s2);
+    }
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
+    if (lane == 0) s_sum[par][wp] = make_float2(s1, s2);
+    __syncthreads();
+    const float2 part = s_sum[par][lane];  // (a warp's sum a lane)
+    s1 = warp_sum(part.x) * (inv_w * rstd);
+    s2 = warp_sum(part.y) * (inv_w * rstd);
+#pragma unroll
+    for (int k = 0; k < E; ++k) d[k] = fmaf(rstd, d[k], fmaf(-n[k], s2, -s1));
+    Row::put(p.out, r * p.W, c0, p.W, d);
+  }
+  if (!sums) return;
+  float* out = p.part + (long long)blockIdx.x * 2 * p.W;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (c0 + j * Row::kStep < p.W) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = c0 + j * Row::kStep + e;
+        out[c] = dw[(j * VEC + e) * N], out[p.W + c] = db[(j * VEC + e) * N];
+      }
+    }
+}
+
 // Rows wider than the registers hold: one CTA per row, three passes (mean, deviations, output),
 // the later ones from cache.
 constexpr int kLnWide = 1024;
@@ -554,7 +633,7 @@ static LnPlan ln_plan(long long R, int W, int vec, bool backward) {
   if (W <= 1024) return LnPlan{vec, 8, 4};
   for (int warps : {4, 8, 16})
     if (W <= 32 * 16 * warps) return LnPlan{vec, 16, warps};
-  if (!backward && W <= 32 * 32 * 16) return LnPlan{vec, 32, 16};
+  if (W <= 32 * 32 * 16) return backward ? LnPlan{vec, 16, kLnTallWarps} : LnPlan{vec, 32, 16};
   return LnPlan{1, 0, 0};
 }
 
@@ -603,6 +682,18 @@ static cudaError_t ln_launch(const LnParams& p, int* grid, bool backward, cudaSt
 }
 
 template <typename T, int VEC>
+static cudaError_t ln_tall_launch(const LnParams& p, int* grid, cudaStream_t s) {
+  const auto kernel = ln_tall_bwd_kernel<T, VEC, 16 / VEC>;
+  const int smem = (p.part != nullptr ? 3 : 1) * 32 * kLnTallWarps * 16 * (int)sizeof(float);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  *grid = (int)std::min<long long>(p.R, kLnSms);
+  TimedLaunch tl(kTimeLnBwd, s);
+  kernel<<<*grid, 32 * kLnTallWarps, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int VEC>
 static cudaError_t ln_instance(const LnParams& p, const LnPlan& pl, int* grid, bool backward, cudaStream_t s) {
   switch (pl.warps * 100 + pl.elements) {
     case 108: return ln_launch<T, VEC, 8 / VEC, 1>(p, grid, backward, s);
@@ -612,6 +703,7 @@ static cudaError_t ln_instance(const LnParams& p, const LnPlan& pl, int* grid, b
     case 408: return ln_launch<T, VEC, 8 / VEC, 4>(p, grid, backward, s);
     case 416: return ln_launch<T, VEC, 16 / VEC, 4>(p, grid, backward, s);
     case 816: return ln_launch<T, VEC, 16 / VEC, 8>(p, grid, backward, s);
+    case kLnTallWarps * 100 + 16: return ln_tall_launch<T, VEC>(p, grid, s);
     case 1632: return ln_launch<T, VEC, 32 / VEC, 16>(p, grid, backward, s);
     default: return ln_launch<T, VEC, 16 / VEC, 16>(p, grid, backward, s);
   }

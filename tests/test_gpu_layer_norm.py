@@ -318,6 +318,20 @@ def test_canaries():
         assert (wsb[:256] == 77).all() and (wsb[256 + nb:] == 77).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("W", [8200, 9001, 12290, 16383])
+def test_tall_rows(W, dtype):
+    """Rows that CTAs walk two and three of, of every vector width, in place in wider rows; and dx alone."""
+    import sparc_b200
+
+    x, w, b, dy = _inputs((333, W + 8), dtype, seed=W)
+    x, dy, w, b = x[:, 8:], dy[:, :W], w[8:], b[8:]
+    _, grads = _check(x, w, b, dy)
+    lx = x.detach().requires_grad_(True)
+    y = sparc_b200.layer_norm(lx, w, b)
+    assert torch.equal(torch.autograd.grad(y, lx, dy)[0], grads[0])
+
+
 def test_the_widest_row():
     """The width limit, with the parameters' gradients: as many columns as the launches have to cover."""
     import sparc_b200
