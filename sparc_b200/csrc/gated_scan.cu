@@ -988,8 +988,11 @@ static cudaError_t gated_launch(const GatedParams& p, bool backward, cudaStream_
   constexpr int kBwdBytes = W::WARPS * W::STAGES * GatedReader<T, MODE, W::K, 4, W::STAGES>::kStageBytes +
                             W::TILE * 96 * (int)sizeof(float2);
   const int smem = gated_map_bytes(p.cluster) + (backward ? kBwdBytes : kFwdBytes);
+  // The limit belongs to the kernel, not to a launch: every call sets that of the largest cluster, as a
+  // smaller one could come between another thread's setting and its launch.
+  const int most = gated_map_bytes(kGatedMaxCluster) + (backward ? kBwdBytes : kFwdBytes);
   const auto kernel = backward ? gated_bwd_kernel<T, SEG, MODE> : gated_fwd_kernel<T, SEG, MODE>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e != cudaSuccess) return e;
   if (p.cluster > 8) {
     const cudaError_t wide = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
