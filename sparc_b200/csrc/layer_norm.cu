@@ -684,8 +684,10 @@ static cudaError_t ln_launch(const LnParams& p, int* grid, bool backward, cudaSt
 template <typename T, int VEC>
 static cudaError_t ln_tall_launch(const LnParams& p, int* grid, cudaStream_t s) {
   const auto kernel = ln_tall_bwd_kernel<T, VEC, 16 / VEC>;
-  const int smem = (p.part != nullptr ? 3 : 1) * 32 * kLnTallWarps * 16 * (int)sizeof(float);
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr int kArray = 32 * kLnTallWarps * 16 * (int)sizeof(float);
+  const int smem = (p.part != nullptr ? 3 : 1) * kArray;
+  // (the limit is the kernel's, not the launch's: always the largest, as another thread may launch between)
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * kArray);
   if (e != cudaSuccess) return e;
   *grid = (int)std::min<long long>(p.R, kLnSms);
   TimedLaunch tl(kTimeLnBwd, s);

@@ -59,3 +59,25 @@ def test_gated_scan(dtype):
         keep += [t, out, nu, gnu, carry, ws]
     assert _at_once(forward) == [[], []]
     assert _at_once(backward) == [[], []]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_norm_backward(dtype):
+    """Rows of 16384 columns with and without the parameters' gradients."""
+    L = _lib.lib()
+    R, W, code = 2, 16384, _lib.dtype_code(dtype)
+    keep, calls = [], []
+    for sums in (True, False):
+        x, dy = (torch.randn(R, W, device="cuda").to(dtype) for _ in range(2))
+        dx = torch.empty_like(x)
+        w, gw, gb = (torch.ones(W, device="cuda") for _ in range(3))
+        stats = torch.ones(2, R, device="cuda")
+        nb = L.sparc_layer_norm_workspace_bytes(R, W)
+        ws = torch.empty(nb, device="cuda", dtype=torch.uint8)
+        calls.append((L.sparc_layer_norm_backward,
+                      _lib.LayerNormBwdArgs(x.data_ptr(), dy.data_ptr(), w.data_ptr(), stats[0].data_ptr(),
+                                            stats[1].data_ptr(), dx.data_ptr(), gw.data_ptr() if sums else None,
+                                            gb.data_ptr() if sums else None, ws.data_ptr() if sums else None,
+                                            nb if sums else 0, W, W, R, W, code)))
+        keep += [x, dy, dx, w, gw, gb, stats, ws]
+    assert _at_once(calls) == [[], []]
