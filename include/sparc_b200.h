@@ -419,6 +419,9 @@ typedef struct SparcGatedFwdArgs {
   unsigned* status;                    /* device word, or'ed with SPARC_STATUS_TIMEOUT if such a
                                           wait ran out (the kernel then stops, its
                                           outputs unfinished), or NULL */
+  unsigned inject_withhold_step;       /* tests only: at this step (from 1; 0: never) the last CTA of
+                                          every cluster withholds its map, so that the waits for
+                                          it run out (a step: the tokens that a cluster takes at once) */
 } SparcGatedFwdArgs;
 
 typedef struct SparcGatedBwdArgs {
@@ -452,6 +455,7 @@ typedef struct SparcGatedBwdArgs {
   int dtype;
   unsigned max_spin;
   unsigned* status;
+  unsigned inject_withhold_step;
 } SparcGatedBwdArgs;
 
 /* One token of it: x and the gates [batch, channels] (dtype, row strides in elements), state

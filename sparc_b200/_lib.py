@@ -114,7 +114,7 @@ class GatedFwdArgs(ctypes.Structure):
         ("x_batch_stride", _ll), ("x_token_stride", _ll), ("retention_batch_stride", _ll),
         ("retention_token_stride", _ll), ("write_batch_stride", _ll), ("write_token_stride", _ll),
         ("batch", _ll), ("length", _ll), ("channels", _ll), ("dtype", ctypes.c_int),
-        ("max_spin", ctypes.c_uint), ("status", _vp),
+        ("max_spin", ctypes.c_uint), ("status", _vp), ("inject_withhold_step", ctypes.c_uint),
     ]
 
 
@@ -128,7 +128,7 @@ class GatedBwdArgs(ctypes.Structure):
         ("retention_token_stride", _ll), ("write_batch_stride", _ll), ("write_token_stride", _ll),
         ("dy_batch_stride", _ll), ("dy_token_stride", _ll),
         ("batch", _ll), ("length", _ll), ("channels", _ll), ("dtype", ctypes.c_int),
-        ("max_spin", ctypes.c_uint), ("status", _vp),
+        ("max_spin", ctypes.c_uint), ("status", _vp), ("inject_withhold_step", ctypes.c_uint),
     ]
 
 

@@ -46,6 +46,7 @@ namespace sparc {
 constexpr int kGatedChunk = 32;       // tokens per saved carry
 constexpr int kGatedMaxCluster = 16;  // (above 8 a kernel has to allow it)
 constexpr unsigned kGatedSpin = 1u << 22;  // default bound of a wait's polls (each may sleep in hardware)
+constexpr unsigned kGatedDrain = 1u << 12;  // and of the wait on the way out for stores that have been issued
 
 // How a CTA cuts its tile: WARPS spans of K tokens; BLOCKS CTAs per SM that the registers are held to;
 // STAGES steps of inputs on their way.
@@ -87,6 +88,7 @@ struct GatedParams {
   int D, groups, cluster, rows;  // rows: clusters per channel group, each walking rows of the batch
   unsigned max_spin;             // polls of a wait for the cluster's maps
   unsigned* status;              // or'ed with kStatusTimeout where one ran out, or null
+  unsigned withhold;             // tests: the step (from 1) at which a cluster's last CTA pushes nothing, or 0
 };
 
 // ---------------------------------------------------------------- two adjacent channels
@@ -492,6 +494,7 @@ struct GatedExchange {
   float4* map;              // [2][CTAs of the cluster][32], at the same place in every CTA
   unsigned long long* bar;  // [2]
   int* late;                // [2]: a wait of the step ran out
+  unsigned* pushed;         // [1 + CTAs of the cluster]: steps pushed, by this CTA and (on the way out) by each
   int cs;
   __device__ __forceinline__ float4* at(int par, int rank) const { return map + (par * cs + rank) * 32; }
 };
@@ -502,11 +505,12 @@ __device__ __forceinline__ void exchange_init(const GatedExchange& x) {
     mbar_init(&x.bar[1], 1);
     mbar_init_fence();
     x.late[0] = x.late[1] = 0;
+    x.pushed[0] = 0;
   }
   // every CTA of the cluster has started, and its barriers stand, before anything is pushed
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void exchange_push(const GatedExchange& x, unsigned n, int rank, int lane, float4 v) {
+__device__ __forceinline__ void exchange_send(const GatedExchange& x, unsigned n, int rank, int lane, float4 v) {
   const int par = n & 1;
   if (lane == 0) mbar_arrive_expect_tx(&x.bar[par], (unsigned)x.cs * 32u * 16u);
   for (int q = 0; q < x.cs; ++q)
@@ -514,6 +518,12 @@ __device__ __forceinline__ void exchange_push(const GatedExchange& x, unsigned n
                      cluster_smem_addr(x.at(par, rank) + lane, q)),
                  "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(cluster_smem_addr(&x.bar[par], q))
                  : "memory");
+}
+__device__ __forceinline__ void exchange_push(const GatedParams& p, const GatedExchange& x, unsigned n, int rank, int lane,
+                                              float4 v) {
+  if (p.withhold == n + 1 && rank == x.cs - 1) return;
+  exchange_send(x, n, rank, lane, v);
+  if (lane == 0) x.pushed[0] = n + 1;
 }
 // v through the maps of CTAs q0, q0 + d, ... up to before q1; they are read two ahead of their use
 template <bool SEG>
@@ -525,7 +535,7 @@ __device__ __forceinline__ float2 exchange_through(const GatedExchange& x, int p
   if (q0 != q1) v = through<SEG>(lo2(x.at(par, q0)[lane]), hi2(x.at(par, q0)[lane]), v);
   return v;
 }
-// A wait that runs out is marked, and the CTA leaves at its next step, between the barrier that all its
+// A wait that runs out is marked, and the CTA leaves its loop at the next step, between the barrier that all its
 // warps pass (so that all see the mark) and its push; its peers' waits then run out and they leave too.
 __device__ __forceinline__ void exchange_wait(const GatedParams& p, const GatedExchange& x, unsigned n) {
   if (!mbar_wait_cluster(&x.bar[n & 1], n >> 1 & 1u, p.max_spin)) {
@@ -535,6 +545,41 @@ __device__ __forceinline__ void exchange_wait(const GatedParams& p, const GatedE
 }
 __device__ __forceinline__ bool exchange_late(const GatedExchange& x, unsigned n) {  // of the step before
   return *reinterpret_cast<volatile int*>(x.late + (n & 1 ^ 1)) != 0;
+}
+
+// The way out of the kernel, for every warp at once: no CTA exits while a push to it may be on its way. Every
+// CTA comes to the barrier, and all pushes that the loops make have then been issued. A CTA none of whose
+// waits ran out has every push, and may go. The others settle it (out of line and with the count of
+// pushes in shared memory: in the kernel's body, or with the count in a register, the loops lose 2%). Where
+// a CTA could go every step was pushed everywhere, so one that pushed every step itself waits for the last
+// again. If that does not come, or not every step was pushed, no CTA can have gone, and they agree on the
+// steps that were: a CTA pushes a step only if its wait for the one before did not run out, that is once
+// every CTA had pushed that one, so their counts differ by one at most. Those behind push once more (no
+// one reads it), which completes the last two phases everywhere, and each CTA waits until they have
+// come. (These waits are for stores that have been issued, or are right behind the barrier: only a fault
+// of the hardware could outlast their bound.)
+__device__ __noinline__ void exchange_settle(const GatedExchange x, unsigned all) {
+  const int lane = threadIdx.x & 31, rank = (int)(blockIdx.x % (unsigned)x.cs);
+  auto come = [&](unsigned k) { return mbar_wait_cluster(&x.bar[k & 1], k >> 1 & 1u, kGatedDrain); };
+  const unsigned pushed = x.pushed[0];
+  if (pushed == all && __syncthreads_and(come(all - 1))) return;
+  if (threadIdx.x < (unsigned)x.cs)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_smem_addr(x.pushed + 1 + rank, threadIdx.x)), "r"(pushed)
+                 : "memory");
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  unsigned most = 0;
+  for (int q = 1; q <= x.cs; ++q) most = max(most, *reinterpret_cast<volatile unsigned*>(x.pushed + q));
+  if (threadIdx.x < 32 && pushed < most) exchange_send(x, pushed, rank, lane, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+  for (unsigned k = most < 2 ? 0 : most - 2; k < most; ++k) come(k);
+}
+// (behind a barrier of the CTA that follows its last wait)
+__device__ __forceinline__ void exchange_leave(const GatedParams& p, const GatedExchange& x, int tile) {
+  cluster_sync_relaxed();
+  if ((x.late[0] | x.late[1]) == 0) return;
+  const unsigned steps = (unsigned)(((p.L + tile - 1) / tile + x.cs - 1) / x.cs);
+  const long long first = blockIdx.x / (unsigned)x.cs / (unsigned)p.groups;
+  exchange_settle(x, (unsigned)((p.B - first + p.rows - 1) / p.rows) * steps);
 }
 
 // Which of a warp's K tokens from t0 on start a segment, as bits.
@@ -570,6 +615,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   __shared__ float4 s_map[2][NW][32];                     // (A, H) of each warp
   __shared__ unsigned long long s_bar[2];
   __shared__ int s_late[2];
+  __shared__ unsigned s_pushed[1 + kGatedMaxCluster];
   __shared__ float2 s_out[2][32];                         // one CTA: the state leaving its tile
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
   const int cs = p.cluster, rank = (int)(blockIdx.x % (unsigned)cs);
@@ -577,7 +623,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   const int ch0 = (int)(id % (unsigned)p.groups) * 64, ch = ch0 + 2 * lane;
   const bool on = ch < p.D;
   const int stride = cs * TILE;  // tokens from a step to the next
-  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, s_late, cs};  // (A, H) of each CTA
+  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, s_late, s_pushed, cs};  // (A, H) of each CTA
   R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
   const float2 root_nu = make_float2(sqrtf(nu.x), sqrtf(nu.y));
@@ -635,7 +681,7 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
           A = bcast2(1.0f), H = bcast2(0.0f);
 #pragma unroll
           for (int j = 0; j < NW; ++j) compose<SEG>(A, H, lo2(s_map[par][j][lane]), hi2(s_map[par][j][lane]));
-          exchange_push(peers, n, rank, lane, cat4(A, H));
+          exchange_push(p, peers, n, rank, lane, cat4(A, H));
         }
         exchange_wait(p, peers, n);
         h = exchange_through<SEG>(peers, par, 0, rank, 1, lane, carry);
@@ -669,7 +715,10 @@ __global__ void __launch_bounds__(GatedFwdCut<T>::WARPS * 32, GatedFwdCut<T>::BL
   }
 leave:
   copy_wait<0>();
-  if (cs > 1) cluster_sync_relaxed();  // no CTA leaves while a peer may still push to it
+  if (cs > 1) {
+    __syncthreads();
+    exchange_leave(p, peers, TILE);
+  }
 }
 
 // ---------------------------------------------------------------- backward
@@ -714,6 +763,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   __shared__ float2 s_adj[2][NW][32];                // G: adjoints, in reverse, out = A in + G
   __shared__ unsigned long long s_bar[2];
   __shared__ int s_late[2];
+  __shared__ unsigned s_pushed[1 + kGatedMaxCluster];
   __shared__ float2 s_out[2][32];                    // one CTA: the adjoint leaving its tile
   __shared__ double2 s_nu[NW][32];
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
@@ -723,7 +773,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   const bool on = ch < p.D;
   const int stride = cs * TILE, steps = ((p.L + TILE - 1) / TILE + cs - 1) / cs;
   constexpr int kSpan = kGatedChunk / K;  // warps of a chunk
-  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, s_late, cs};  // (A, G) of each CTA
+  const GatedExchange peers{reinterpret_cast<float4*>(s_raw), s_bar, s_late, s_pushed, cs};  // (A, G) of each CTA
   float2* put = reinterpret_cast<float2*>(s_raw + gated_map_bytes(cs)) + wp * K * 96 + lane;
   R* stage = reinterpret_cast<R*>(s_raw + gated_map_bytes(cs) + NW * K * 96 * sizeof(float2)) + wp * S * (GatedReader<T, MODE, K, NT, S>::kStageBytes / (int)sizeof(R));
   const float2 nu = make_float2(on ? gated_nu(p.nu_log[ch]) : 0.0f, ch + 1 < p.D ? gated_nu(p.nu_log[ch + 1]) : 0.0f);
@@ -790,7 +840,7 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
             if (i == NW - 1) A = lo2(s_map[par][i][lane]), G = s_adj[par][i][lane];
             else compose<SEG>(A, G, lo2(s_map[par][i][lane]), s_adj[par][i][lane]);
           }
-          exchange_push(peers, n, rank, lane, cat4(A, G));
+          exchange_push(p, peers, n, rank, lane, cat4(A, G));
         }
       }
 #pragma unroll
@@ -847,7 +897,6 @@ __global__ void __launch_bounds__(GatedBwdCut<T>::WARPS * 32, GatedBwdCut<T>::BL
   }
 leave:
   copy_wait<0>();
-  if (cs > 1) cluster_sync_relaxed();
   // the CTA's sum of dnu_log per channel, over its warps in order
   s_nu[wp][lane] = make_double2(dnu_x, dnu_y);
   __syncthreads();
@@ -857,6 +906,10 @@ leave:
     double* part = p.part + ((long long)(id / (unsigned)p.groups) * cs + rank) * p.D;
     if (on) part[ch] = sx;
     if (ch + 1 < p.D) part[ch + 1] = sy;
+  }
+  if (cs > 1) {
+    __syncwarp();
+    exchange_leave(p, peers, TILE);
   }
 }
 
@@ -1083,6 +1136,7 @@ int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {
   p.chunks = (int)sparc_gated_carry_chunks(a->length);
   p.max_spin = a->max_spin != 0 ? a->max_spin : kGatedSpin;
   p.status = a->status;
+  p.withhold = a->inject_withhold_step;
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const void* q : {a->x, a->retention_gate, a->write_gate, (const void*)a->y})
     if (!gated_aligned(q, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");
@@ -1132,6 +1186,7 @@ int sparc_gated_scan_backward(const SparcGatedBwdArgs* a, void* stream) {
   p.chunks = (int)sparc_gated_carry_chunks(a->length);
   p.max_spin = a->max_spin != 0 ? a->max_spin : kGatedSpin;
   p.status = a->status;
+  p.withhold = a->inject_withhold_step;
   const int size = a->dtype == SPARC_DTYPE_BF16 ? 2 : 4;
   for (const GatedIn& in : p.in)
     if (!gated_aligned(in.p, size)) return fail(SPARC_ERR_ARG, "misaligned activation pointer");

@@ -1,5 +1,6 @@
 """The gated linear recurrence on the GPU where its inputs, its callers or its waits go wrong: NaN gates
-behind a segment start."""
+behind a segment start, and waits between the CTAs of a cluster that run out."""
+import ctypes
 import math
 
 import pytest
@@ -61,3 +62,60 @@ def test_nan_gate_behind_a_start(B, T, D, after, sign, nu_max, dtype):
         first = s + max(after, 1)  # (of a start's own gate only the write's factor counts)
         assert torch.isnan(got[0][:, first:end]).all()
         assert torch.isnan(got[3][:, s + after]).all()
+
+
+# ------------------------------------------------------------------ waits that run out
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,tokens,reverse_tokens", [(6000, 1024, 512), (200, 256, 128), (130, 128, 128)])
+def test_withheld_map(T, tokens, reverse_tokens, dtype):
+    """A CTA that withholds its map at the first, a middle or the last step (of clusters of sixteen, four and
+    two CTAs, which take `tokens` a step): the others' waits run out, the kernel says so and ends, what
+    the steps before wrote is right, and the next call is none the worse for it."""
+    from sparc_b200 import _lib
+
+    L = _lib.lib()
+    B, D = 1, 66
+    t, nu, h0, dy, _ = _inputs(B, T, D, dtype)
+    st, nb = (T * D, D), L.sparc_gated_workspace_bytes(B, T, D)
+    stream = torch.cuda.current_stream().cuda_stream
+    p, code = [v.data_ptr() for v in t], _lib.dtype_code(dtype)
+    carry = torch.zeros(B, L.sparc_gated_carry_chunks(T), D, device="cuda")
+
+    def forward(step):
+        y, status = torch.zeros(B, T, D, device="cuda", dtype=dtype), torch.zeros(1, device="cuda", dtype=torch.int32)
+        kept = carry if step == 0 else torch.zeros_like(carry)
+        a = _lib.GatedFwdArgs(*p, nu.data_ptr(), h0.data_ptr(), None, 0, y.data_ptr(), None, kept.data_ptr(), *st, *st, *st,
+                              B, T, D, code, 4 if step else 0, status.data_ptr(), step)
+        assert L.sparc_gated_scan_forward(ctypes.byref(a), stream) == 0
+        return y, int(status)
+
+    def backward(step):
+        out = [torch.zeros(B, T, D, device="cuda", dtype=dtype) for _ in range(3)]
+        gnu, status = torch.zeros(D, device="cuda"), torch.zeros(1, device="cuda", dtype=torch.int32)
+        ws = torch.zeros(nb, device="cuda", dtype=torch.uint8)
+        a = _lib.GatedBwdArgs(*p, nu.data_ptr(), dy.data_ptr(), carry.data_ptr(), None, None, 0, *(v.data_ptr() for v in out),
+                              gnu.data_ptr(), None, ws.data_ptr(), nb, *st, *st, *st, *st, B, T, D, code, 4 if step else 0,
+                              status.data_ptr(), step)
+        assert L.sparc_gated_scan_backward(ctypes.byref(a), stream) == 0
+        return out, int(status)
+
+    y, status = forward(0)
+    assert status == 0
+    steps = -(-T // tokens)
+    for step in {1, (steps + 1) // 2, steps}:
+        got, status = forward(step)
+        assert status == _lib.STATUS_TIMEOUT, f"forward, step {step} of {steps}"
+        assert torch.equal(got[:, :(step - 1) * tokens], y[:, :(step - 1) * tokens])
+        again, status = forward(0)
+        assert status == 0 and torch.equal(again, y)
+    out, status = backward(0)
+    assert status == 0
+    steps = -(-T // reverse_tokens)
+    for step in {1, (steps + 1) // 2, steps}:
+        got, status = backward(step)
+        assert status == _lib.STATUS_TIMEOUT, f"backward, step {step} of {steps}"
+        done = (steps - step + 1) * reverse_tokens
+        assert all(torch.equal(a[:, done:], b[:, done:]) for a, b in zip(got, out))
+        again, status = backward(0)
+        assert status == 0 and all(torch.equal(a, b) for a, b in zip(again, out))
