@@ -4,9 +4,11 @@
 // (a decode step, a norm) next to what a Python autograd function costs. No arithmetic here.
 //
 // Checks come in the order of the package's Python functions: shapes (ValueError), dtypes
-// (TypeError), then the device (RuntimeError: there is no CPU path).
+// (TypeError), forward-mode derivatives (NotImplementedError), then the device (RuntimeError: there
+// is no CPU path).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -55,6 +57,12 @@ Tensor f32(const Tensor& t) {
 const float* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 float* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr<float>() : nullptr; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// No operator here carries a forward-mode derivative on; a result without it would pass for one that is zero.
+void refuse_tangent(const char* what, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
+                              what, " has no forward-mode derivative (its inputs may hold no tangent)");
+}
 
 // t as the kernels read it: any strides but adjacent values in the last dimension.
 Tensor adjacent(const Tensor& t) {
@@ -122,6 +130,8 @@ void gated_check(const char* what, const Tensor& x, const Tensor& r, const Tenso
                    "nu_log and state must be floating-point tensors");
   TORCH_CHECK_TYPE(!pos || (at::isIntegralType(pos->scalar_type(), true) && pos->element_size() <= 8),
                    "segment_pos must be an integer tensor, got ", pos ? pos->scalar_type() : at::kLong);
+  for (const Tensor* t : {&x, &r, &w, &nu}) refuse_tangent(what, *t);
+  if (state) refuse_tangent(what, *state);
   require_device(x, "x", x);
   require_device(r, "retention_gate", x);
   require_device(w, "write_gate", x);
@@ -372,6 +382,8 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
   dtype_code(x);
   TORCH_CHECK_TYPE(weight.is_floating_point() && (!bias || bias->is_floating_point()),
                    "layer norm expects floating-point parameters");
+  for (const Tensor* t : {&x, &weight}) refuse_tangent("layer norm", *t);
+  if (bias) refuse_tangent("layer norm", *bias);
   require_device(x, "x", x);
   require_device(weight, "weight", x);
   if (bias) require_device(*bias, "bias", x);
@@ -387,7 +399,10 @@ void grads_check(const char* what, const std::vector<Tensor>& tensors) {
   for (const Tensor& t : tensors) {
     TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, " expects dense tensors, got ", t.layout());
     dtype_code(t);
+    refuse_tangent(what, t);
   }
+}
+void grads_check_device(const char* what, const std::vector<Tensor>& tensors) {
   for (const Tensor& t : tensors) {
     TORCH_CHECK(t.is_cuda(), "sparc_b200: every gradient must be a CUDA tensor (there is no CPU path)");
     TORCH_CHECK(t.device() == tensors[0].device(), what, " expects tensors of one device, got ", tensors[0].device(), " and ",
@@ -408,8 +423,10 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     TORCH_CHECK_VALUE(out[i].sizes() == grads[i].sizes() && out[i].scalar_type() == grads[i].scalar_type(),
                       "clip grads expects out to match the gradients' shapes and dtypes");
   grads_check(what, grads);
+  grads_check(what, out);
+  grads_check_device(what, grads);
   if (!out.empty()) {
-    grads_check(what, out);
+    grads_check_device(what, out);
     TORCH_CHECK(out[0].device() == grads[0].device(), "clip grads expects out on the gradients' device");
   }
   const c10::cuda::CUDAGuard guard(grads[0].device());

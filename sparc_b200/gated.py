@@ -14,8 +14,8 @@ position is 0 (packed sequences): nothing of the earlier segment is kept, not it
 NaN either. The token's write keeps its factor sqrt(1 - a_t^2).
 
 Both are operators of csrc_torch/train_ops.cpp, which checks the arguments (shapes: ValueError,
-dtypes: TypeError, a tensor that is not on the GPU: RuntimeError) and calls the kernels of
-csrc/gated_scan.cu on the current stream.
+dtypes: TypeError, a forward-mode tangent: NotImplementedError, a tensor that is not on the GPU:
+RuntimeError) and calls the kernels of csrc/gated_scan.cu on the current stream.
 """
 from __future__ import annotations
 

@@ -8,7 +8,8 @@ the same clipped gradients bit for bit.
 
 Gradients are float32 or bfloat16 CUDA tensors of one device. The norm is a float32 tensor with
 one element, right also where a square would overflow or underflow in float32. A norm that is NaN
-makes every gradient NaN; whether to skip such a step is the caller's decision.
+makes every gradient NaN; whether to skip such a step is the caller's decision. No gradient goes
+through norm or scaling, and a tensor with a forward-mode tangent is refused (NotImplementedError).
 """
 from __future__ import annotations
 

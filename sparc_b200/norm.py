@@ -4,7 +4,8 @@ the reference's networks put before each layer (sparc-impl/sparc/networks/sequen
 next to the RMSNorm of `stack.py`, whose stack takes either (``norm="layer"``).
 
 x is float32 or bfloat16 with any leading dimensions (rows whose columns are adjacent are read in
-place, others copied first); the statistics, the sums and the parameters are float32.
+place, others copied first); the statistics, the sums and the parameters are float32. There is no
+forward-mode derivative: an input with a tangent is refused (NotImplementedError).
 """
 from __future__ import annotations
 

@@ -1,0 +1,40 @@
+"""What the operators of recurrent training refuse or declare, without a GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import sparc_b200
+from sparc_b200 import torch_ops
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    from sparc_b200 import _build
+
+    _build.build()
+    _build.build_torch_ops()
+
+
+def test_forward_mode_is_refused():
+    """A tangent that an operator cannot carry on is refused, in whichever input it comes, also where no
+    gradient is recorded; without forward mode the same call goes on to the check of its device."""
+    x3, x2, w, s = torch.ones(2, 3, 8), torch.ones(2, 8), torch.ones(8), torch.ones(2, 8)
+    calls = {
+        "gated_scan": (lambda *a: sparc_b200.gated_scan(*a[:4], state=a[4]), [x3, x3, x3, w, s]),
+        "gated_scan_step": (sparc_b200.gated_scan_step, [x2, x2, x2, w, s]),
+        "layer_norm": (sparc_b200.layer_norm, [x3, w, w]),
+        "grad_norm": (lambda *a: sparc_b200.grad_norm(a), [x2, w]),
+        "clip_grads": (lambda *a: sparc_b200.clip_grads(a[:2], 1.0, out=a[2:]), [x2, w, x2.clone(), w.clone()]),
+    }
+    for name, (f, args) in calls.items():
+        for k in range(len(args)):
+            with fwAD.dual_level():
+                dual = [fwAD.make_dual(a, torch.ones_like(a)) if i == k else a for i, a in enumerate(args)]
+                with pytest.raises(NotImplementedError, match="forward"):
+                    f(*dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+                    f(*dual)
+                with fwAD._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA"):
+                    f(*dual)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f(*args)
