@@ -481,6 +481,9 @@ typedef struct SparcGatedStepArgs {
 long long sparc_gated_chunk_tokens(void);
 long long sparc_gated_carry_chunks(long long length);
 size_t sparc_gated_workspace_bytes(long long batch, long long length, long long channels);
+/* A device word of the library for `status`, one per device (the current one's), zero at first and
+ * never cleared by the library. */
+int sparc_gated_status_word(unsigned** word);
 int sparc_gated_scan_forward(const SparcGatedFwdArgs* args, void* stream);
 int sparc_gated_scan_backward(const SparcGatedBwdArgs* args, void* stream);
 int sparc_gated_step(const SparcGatedStepArgs* args, void* stream);

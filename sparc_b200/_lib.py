@@ -237,6 +237,7 @@ SIGNATURES = {
     "sparc_gated_chunk_tokens": (_ll, []),
     "sparc_gated_carry_chunks": (_ll, [_ll]),
     "sparc_gated_workspace_bytes": (ctypes.c_size_t, [_ll, _ll, _ll]),
+    "sparc_gated_status_word": (ctypes.c_int, [ctypes.POINTER(_vp)]),
     "sparc_gated_scan_forward": (ctypes.c_int, [ctypes.POINTER(GatedFwdArgs), _vp]),
     "sparc_gated_scan_backward": (ctypes.c_int, [ctypes.POINTER(GatedBwdArgs), _vp]),
     "sparc_gated_step": (ctypes.c_int, [ctypes.POINTER(GatedStepArgs), _vp]),

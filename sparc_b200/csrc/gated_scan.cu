@@ -974,6 +974,8 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p
 }
 
 // ---------------------------------------------------------------- host
+__device__ unsigned g_gated_status;  // zero from the module's loading on: no stream orders its clearing
+
 struct GatedPlan {
   int groups, cluster, rows;
 };
@@ -1107,6 +1109,21 @@ long long sparc_gated_carry_chunks(long long length) {
 size_t sparc_gated_workspace_bytes(long long batch, long long length, long long channels) {
   if (gated_check_shape(batch, length, channels) != SPARC_OK) return 0;
   return gated_ws_bytes(batch, length, channels);
+}
+
+int sparc_gated_status_word(unsigned** word) {
+  if (word == nullptr) return fail(SPARC_ERR_ARG, "null pointer");
+  void* p = nullptr;
+  // (the first call on a device may load the module, also while the thread captures a graph)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) {
+    e = cudaGetSymbolAddress(&p, g_gated_status);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+  if (e != cudaSuccess) return fail(SPARC_ERR_LAUNCH, cudaGetErrorString(e));
+  *word = static_cast<unsigned*>(p);
+  return SPARC_OK;
 }
 
 int sparc_gated_scan_forward(const SparcGatedFwdArgs* a, void* stream) {

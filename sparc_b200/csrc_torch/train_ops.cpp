@@ -9,7 +9,6 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/AutogradState.h>
-#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -17,8 +16,8 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
+#include <atomic>
 #include <cmath>
-#include <mutex>
 #include <optional>
 #include <vector>
 
@@ -84,28 +83,26 @@ variable_list once(variable_list grads, const char* what) {
   return grads;
 }
 
-// A device word per device, or'ed by kernels whose bounded waits ran out.
-std::mutex g_status_mutex;
-std::vector<Tensor>& status_words() {
-  static auto* words = new std::vector<Tensor>(64);  // (not destroyed: the context may be gone by then)
-  return *words;
-}
-unsigned* status_word(const Tensor& like) {
+// The library's status words, or'ed by kernels whose bounded waits ran out, of the devices that such kernels have
+// been launched on.
+constexpr int kDevices = 64;
+std::atomic<unsigned*> g_status[kDevices];
+
+unsigned* status_word(const Tensor& like) {  // (of the current device, like's)
   const int d = like.get_device();
-  std::lock_guard<std::mutex> lock(g_status_mutex);
-  Tensor& word = status_words().at(d);
-  if (!word.defined()) {
-    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return nullptr;
-    const c10::InferenceMode ordinary(false);  // (the word outlives the call, whatever mode that is in)
-    word = at::zeros({1}, like.options().dtype(at::kInt).requires_grad(false));
+  TORCH_CHECK(d < kDevices, "sparc_b200: device ", d, " is beyond the ", kDevices, " that are supported");
+  unsigned* word = g_status[d].load(std::memory_order_acquire);
+  if (word == nullptr) {
+    check(sparc_gated_status_word(&word), "sparc_gated_status_word");
+    g_status[d].store(word, std::memory_order_release);
   }
-  return reinterpret_cast<unsigned*>(word.mutable_data_ptr<int>());
+  return word;
 }
 std::vector<Tensor> wait_status() {
-  std::lock_guard<std::mutex> lock(g_status_mutex);
   std::vector<Tensor> out;
-  for (const Tensor& w : status_words())
-    if (w.defined()) out.push_back(w);
+  for (int d = 0; d < kDevices; ++d)
+    if (unsigned* word = g_status[d].load(std::memory_order_acquire))
+      out.push_back(at::from_blob(word, {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, d)));
   return out;
 }
 

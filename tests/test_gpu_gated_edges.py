@@ -2,6 +2,9 @@
 behind a segment start, and waits between the CTAs of a cluster that run out."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -9,6 +12,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 F32, BF16 = torch.float32, torch.bfloat16
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def _inputs(B, T, D, dtype, seed=0):
@@ -119,3 +123,48 @@ def test_withheld_map(T, tokens, reverse_tokens, dtype):
         assert all(torch.equal(a[:, done:], b[:, done:]) for a, b in zip(got, out))
         again, status = backward(0)
         assert status == 0 and all(torch.equal(a, b) for a, b in zip(again, out))
+
+
+FIRST_CALL_CAPTURED = """
+import torch, sparc_b200
+from sparc_b200 import torch_ops
+x, nu = torch.randn(2, 300, 32, device="cuda"), torch.full((32,), -3.0, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = sparc_b200.gated_scan(x, x, x, nu)
+words = torch_ops.wait_status()
+assert len(words) == 1 and words[0].device == x.device and int(words[0]) == 0, words
+g.replay()
+sparc_b200.check_status()
+assert torch.equal(y, sparc_b200.gated_scan(x, x, x, nu))
+again = torch_ops.wait_status()
+assert len(again) == 1 and again[0].data_ptr() == words[0].data_ptr()
+words[0].fill_(1)  # what a wait that ran out in a replay leaves
+try:
+    sparc_b200.check_status()
+except RuntimeError as e:
+    assert "timed out" in str(e)
+else:
+    raise AssertionError("no error")
+sparc_b200.check_status()
+print("captured first")
+"""
+
+
+def test_first_call_of_a_process_captured():
+    """The status word is there for a graph whose capture is a process's first call (a process of its own)."""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
+def test_status_word_of_the_device():
+    """The library's word is one per device, and what the operators' calls are given."""
+    import sparc_b200
+    from sparc_b200 import _lib, torch_ops
+
+    L, p = _lib.lib(), ctypes.c_void_p()
+    assert L.sparc_gated_status_word(ctypes.byref(p)) == 0 and p.value
+    t, nu, h0, _, _ = _inputs(1, 4, 8, F32)
+    sparc_b200.gated_scan(*t, nu, state=h0)
+    assert p.value in [w.data_ptr() for w in torch_ops.wait_status()]
+    assert L.sparc_gated_status_word(None) == -1
