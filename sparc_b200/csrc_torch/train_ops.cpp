@@ -7,6 +7,7 @@
 // (TypeError), forward-mode derivatives (NotImplementedError), then the device (RuntimeError: there
 // is no CPU path).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -410,6 +411,28 @@ void grads_check_device(const char* what, const std::vector<Tensor>& tensors) {
 // A tensor's values as one dense array (any order of its dimensions), or a dense copy.
 Tensor dense(const Tensor& t) { return (t.is_non_overlapping_and_dense() ? t : t.contiguous()).resolve_neg(); }
 
+// Whether a and b share memory, as far as that shows without a search: strided ones where they are the same view.
+bool overlaps(const Tensor& a, const Tensor& b) {
+  const auto status = at::get_overlap_status(a, b);
+  if (status == at::MemOverlapStatus::TooHard)
+    return a.const_data_ptr() == b.const_data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
+  return status != at::MemOverlapStatus::No;
+}
+
+// Outputs that are written through a copy, whose memory the kernels' own check does not see: not from several
+// places of themselves, and apart from every other tensor.
+void check_copied_outputs(const std::vector<Tensor>& grads, const std::vector<Tensor>& out) {
+  const std::vector<Tensor>& target = out.empty() ? grads : out;
+  for (size_t i = 0; i < target.size(); ++i) {
+    const Tensor& t = target[i];
+    if (t.numel() == 0 || (t.is_non_overlapping_and_dense() && !t.is_neg() && t.strides() == grads[i].strides())) continue;
+    TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "clip grads: an output overlaps itself (it is expanded)");
+    for (size_t j = 0; j < target.size(); ++j)
+      TORCH_CHECK((j == i || !overlaps(t, target[j])) && (out.empty() || !overlaps(t, grads[j]) || (j == i && t.is_same(grads[j]))),
+                  "clip grads: an output overlaps another tensor");
+  }
+}
+
 // The norm of `grads`, and with `clip` the gradients scaled into `out` (in place where it is empty).
 Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, bool clip, double max_norm, double eps) {
   const char* what = clip ? "clip grads" : "grad norm";
@@ -421,6 +444,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
                       "clip grads expects out to match the gradients' shapes and dtypes");
   grads_check(what, grads);
   grads_check(what, out);
+  if (clip) check_copied_outputs(grads, out);
   grads_check_device(what, grads);
   if (!out.empty()) {
     grads_check_device(what, out);

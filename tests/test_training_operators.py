@@ -38,3 +38,31 @@ def test_forward_mode_is_refused():
                     f(*dual)
         with pytest.raises(RuntimeError, match="CUDA"):
             f(*args)
+
+
+def test_clip_refuses_outputs_that_overlap():
+    """Outputs that are not dense are refused like dense ones, before anything is scaled: an expanded one, one
+    view twice, a transposed view of a gradient; halves of one matrix go on to the check of their device."""
+    m = torch.ones(4, 4)
+    half, square = m[:, ::2], torch.ones(4, 4)
+    bad = {
+        "expanded": ([torch.ones(3), torch.ones(1).expand(4)], None),
+        "expanded rows": ([torch.ones(3, 1).expand(3, 2)], None),
+        "one strided view twice": ([half, m[:, ::2]], None),
+        "one strided tensor twice": ([half, half], None),
+        "one strided output twice": ([torch.ones(4, 2), torch.ones(4, 2)], [half, m[:, ::2]]),
+        "an expanded output": ([torch.ones(4)], [torch.ones(1).expand(4)]),
+        "transposed onto its own gradient": ([square], [square.t()]),
+        "transposed onto another gradient": ([torch.ones(4, 4), square], [square.t(), torch.ones(4, 4)]),
+    }
+    for name, (grads, out) in bad.items():
+        with pytest.raises(RuntimeError, match="overlaps"):
+            sparc_b200.clip_grads(grads, 1.0, out=out)
+            raise AssertionError(name)
+    fine = [([half, m[:, 1::2]], None), ([half], [half]), ([half.contiguous(), half], [m[:, 1::2], half]),
+            ([square], [torch.ones(4, 4).t()]), ([torch.ones(0, 1).expand(0, 3)] * 2, None)]
+    for grads, out in fine:
+        with pytest.raises(RuntimeError, match="CUDA"):
+            sparc_b200.clip_grads(grads, 1.0, out=out)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        sparc_b200.grad_norm([half, half, torch.ones(1).expand(4)])  # (nothing is written)
