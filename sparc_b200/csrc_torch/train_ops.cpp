@@ -506,6 +506,6 @@ TORCH_LIBRARY_FRAGMENT(sparc_b200, m) {
   m.def("gated_scan_step(Tensor x, Tensor retention_gate, Tensor write_gate, Tensor nu_log, Tensor state, "
         "Tensor? segment_pos) -> (Tensor, Tensor)", &gated_scan_step);
   m.def("layer_norm(Tensor x, Tensor weight, Tensor? bias, float eps) -> Tensor", &layer_norm);
-  m.def("grad_clip(Tensor[] grads, Tensor[] out, bool clip, float max_norm, float eps) -> Tensor", &grad_clip);
+  m.def("grad_clip(Tensor(a!)[] grads, Tensor(b!)[] out, bool clip, float max_norm, float eps) -> Tensor", &grad_clip);
   m.def("wait_status() -> Tensor[]", &wait_status);
 }

@@ -66,3 +66,11 @@ def test_clip_refuses_outputs_that_overlap():
             sparc_b200.clip_grads(grads, 1.0, out=out)
     with pytest.raises(RuntimeError, match="CUDA"):
         sparc_b200.grad_norm([half, half, torch.ones(1).expand(4)])  # (nothing is written)
+
+
+def test_schemas_say_what_is_written():
+    ops = torch_ops.load()
+    written = {name: [a.name for a in getattr(ops, name).default._schema.arguments if a.alias_info and a.alias_info.is_write]
+               for name in ("gated_scan", "gated_scan_step", "layer_norm", "grad_clip")}
+    assert written == {"gated_scan": [], "gated_scan_step": [], "layer_norm": [], "grad_clip": ["grads", "out"]}
+    assert ops.grad_clip.default._schema.is_mutable
