@@ -259,12 +259,12 @@ def _own(s):
     if not s["train"]:
         return y, last
     leaves = [s[k] for k in ("x", "retention", "write", "nu_log", "state") if s[k] is not None]
+    out = [y.detach(), last.detach(), *torch.autograd.grad((y, last), leaves, (s["dy"], s["dlast"]))]
     if s["dy"].dtype == torch.float32:
-        # the plain form adds the last state's gradient to a float32 dy where it lies; so do these
-        # calls, so that both sides are given the same dy on every pass over a state
+        # the plain form adds the last state's gradient to a float32 dy where it lies; so does this, behind
+        # the calls, so that both sides are given the same dy on every pass over a state
         s["dy"][:, -1] += s["dlast"]
-        return [y.detach(), last.detach(), *torch.autograd.grad(y, leaves, s["dy"])]
-    return [y.detach(), last.detach(), *torch.autograd.grad((y, last), leaves, (s["dy"], s["dlast"]))]
+    return out
 
 
 def run(state):
