@@ -27,14 +27,14 @@
 // -0 (a_t >= +0 or NaN, so the sign marks it; composing keeps the sign of either side), and passing
 // through it selects instead of multiplying.
 //
-// Measured on a B200 (B=8 T=16384 D=2048 bfloat16, 268M channels x tokens): forward 475 us = 4.5 TB/s
-// of its 8 bytes each (69% of what a copy reaches), backward 874 us = 4.3 TB/s of 14 bytes (66%). Neither
-// bytes nor any one unit bounds them but instructions: 33 and 64 thread-instructions an element issue on
-// 52-54% of the cycles, the rest being the latency of a step's chain (gates, barrier, maps, replay) that
-// the 7-16 warps an SM holds (128 and 166 registers) do not cover; more warps at fewer registers issue
+// Measured on a B200 (B=8 T=16384 D=2048 bfloat16, 268M channels x tokens): forward 480 us = 4.5 TB/s
+// of its 8 bytes each (68% of what a copy reaches), backward 879 us = 4.3 TB/s of 14 bytes (65%). Neither
+// bytes nor any one unit bounds them but the latency of a step's chain (gates, barrier, maps, replay), which
+// the 7-16 warps an SM holds (128 and 162 registers) do not cover: their 34 and 60 thread-instructions an
+// element issue on 53-55% of the cycles; more warps at fewer registers issue
 // more instructions and were slower (backward with 128 registers: 1033 us with eight warps a CTA,
 // 1298 us with four CTAs). A copy in the same pattern (128-byte pieces of a token) takes 330-350 and
-// 650-680 us. float32 (B=8 T=2048 D=512): 30 and 48 us, of floors 20 and 36.
+// 650-680 us. float32 (B=8 T=2048 D=512): 30 and 46 us, of floors 20 and 36.
 #include <algorithm>
 
 #include "common.cuh"
@@ -312,8 +312,9 @@ __device__ __forceinline__ void logistic_of(const float2 (&e)[N], float2 (&s)[N]
 
 // For w = -u >= 0: a = e^{-w} and q = 1 - a. Below 1/2 from the series of q (through w^8 / 8!: the
 // next term is below 2^-26 of the first), which keeps 1 - a^2 = q (1 + a) exact to a few ulp where
-// a is near 1 and holds the decay of long sequences; else the hardware exp2, which keeps a to a few
-// ulp where it is small. NEAR: nu <= 1/2 in every channel of the warp, so w never leaves the series.
+// a is near 1 and holds the decay of long sequences; else the hardware exp2 of w log2 e, rounded once: a's
+// relative error grows with w, to about 1.2 w 2^-24 (at w = 40, where a = 4e-18, some 20 ulp). NEAR: nu <=
+// 1/2 in every channel of the warp, so w never leaves the series.
 constexpr float kGatedNear = 0.5f;
 template <bool NEAR, int N>
 __device__ __forceinline__ void decay(const float2 (&w)[N], float2 (&a)[N], float2 (&q)[N]) {
