@@ -411,16 +411,17 @@ void grads_check_device(const char* what, const std::vector<Tensor>& tensors) {
 // A tensor's values as one dense array (any order of its dimensions), or a dense copy.
 Tensor dense(const Tensor& t) { return (t.is_non_overlapping_and_dense() ? t : t.contiguous()).resolve_neg(); }
 
+bool same_view(const Tensor& a, const Tensor& b) {
+  return a.const_data_ptr() == b.const_data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides() && a.is_neg() == b.is_neg();
+}
 // Whether a and b share memory, as far as that shows without a search: strided ones where they are the same view.
 bool overlaps(const Tensor& a, const Tensor& b) {
   const auto status = at::get_overlap_status(a, b);
-  if (status == at::MemOverlapStatus::TooHard)
-    return a.const_data_ptr() == b.const_data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
-  return status != at::MemOverlapStatus::No;
+  return status == at::MemOverlapStatus::TooHard ? same_view(a, b) : status != at::MemOverlapStatus::No;
 }
 
 // Outputs that are written through a copy, whose memory the kernels' own check does not see: not from several
-// places of themselves, and apart from every other tensor.
+// places of themselves, and apart from every other tensor. (An output may be its own gradient.)
 void check_copied_outputs(const std::vector<Tensor>& grads, const std::vector<Tensor>& out) {
   const std::vector<Tensor>& target = out.empty() ? grads : out;
   for (size_t i = 0; i < target.size(); ++i) {
@@ -428,7 +429,7 @@ void check_copied_outputs(const std::vector<Tensor>& grads, const std::vector<Te
     if (t.numel() == 0 || (t.is_non_overlapping_and_dense() && !t.is_neg() && t.strides() == grads[i].strides())) continue;
     TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "clip grads: an output overlaps itself (it is expanded)");
     for (size_t j = 0; j < target.size(); ++j)
-      TORCH_CHECK((j == i || !overlaps(t, target[j])) && (out.empty() || !overlaps(t, grads[j]) || (j == i && t.is_same(grads[j]))),
+      TORCH_CHECK((j == i || !overlaps(t, target[j])) && (out.empty() || !overlaps(t, grads[j]) || (j == i && same_view(t, grads[j]))),
                   "clip grads: an output overlaps another tensor");
   }
 }

@@ -59,7 +59,7 @@ def test_clip_refuses_outputs_that_overlap():
         with pytest.raises(RuntimeError, match="overlaps"):
             sparc_b200.clip_grads(grads, 1.0, out=out)
             raise AssertionError(name)
-    fine = [([half, m[:, 1::2]], None), ([half], [half]), ([half.contiguous(), half], [m[:, 1::2], half]),
+    fine = [([half, m[:, 1::2]], None), ([half], [half]), ([half], [m[:, ::2]]), ([half.contiguous(), half], [m[:, 1::2], half]),
             ([square], [torch.ones(4, 4).t()]), ([torch.ones(0, 1).expand(0, 3)] * 2, None)]
     for grads, out in fine:
         with pytest.raises(RuntimeError, match="CUDA"):
